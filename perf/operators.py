@@ -59,29 +59,29 @@ def _emb(name, direction, tokens, vocab, width, kind, dtype="float32", index="in
 def listed():
     return [
         # one short chain's single representation (384 channels): a call that costs its launches
-        _ln("layernorm step, short chain", "step", 37, 384),
+        _ln("layernorm step: short chain", "step", 37, 384),
         # the LayerNorm of every triangle block over the pair tensor, N = 512
-        _ln("layernorm forward, pairs", "forward", 0, 128, grid=512),
+        _ln("layernorm forward: pairs", "forward", 0, 128, grid=512),
         # its backward around the ending node, which reads the pair tensor transposed
-        _ln("layernorm backward, swapped pairs", "backward", 0, 128, grid=512),
+        _ln("layernorm backward: swapped pairs", "backward", 0, 128, grid=512),
         # a bf16 model's hidden states, a batch of a few thousand tokens
-        _ln("layernorm step, hidden states", "step", 4096, 4096, "bfloat16", "bfloat16"),
+        _ln("layernorm step: hidden states", "step", 4096, 4096, "bfloat16", "bfloat16"),
         # a width that no vector divides, fp16 activations and fp32 parameters
-        _ln("layernorm backward, odd width", "backward", 1023, 5003, "float16", "float32"),
+        _ln("layernorm backward: odd width", "backward", 1023, 5003, "float16", "float32"),
         # the gradients of one layer after an ordinary step: below the limit, nothing to scale
-        _clip("clip, one layer in place", 1, 0, 0, 0, "float32", "in place", False, 128),
+        _clip("clip: one layer in place", 1, 0, 0, 0, "float32", "in place", False, 128),
         # an eight-layer stack's gradients clipped into the optimizer's own buffers
-        _clip("clip, eight layers", 8, 0, 0, 0, "float32", "same", True, 128),
+        _clip("clip: eight layers", 8, 0, 0, 0, "float32", "same", True, 128),
         # a larger bf16 model: clipped gradients go out in fp32 for the optimizer
-        _clip("clip, bf16 to fp32", 0, 200, 1 << 27, 5, "bfloat16", "float32", True, 1),
+        _clip("clip: bf16 to fp32", 0, 200, 1 << 27, 5, "bfloat16", "float32", True, 1),
         # residue types of one chain to its single representation, with the table's gradient
-        _emb("embedding step, residues", "step", 300, 21, 384, "uniform"),
+        _emb("embedding step: residues", "step", 300, 21, 384, "uniform"),
         # relative positions of a 512-residue chain into the pair tensor
-        _emb("embedding forward, relative positions", "forward", 512 * 512, 66, 128, "relative"),
+        _emb("embedding forward: relative positions", "forward", 512 * 512, 66, 128, "relative"),
         # the gradient of that table at 1024 residues: a few rows receive nearly all of the sum
-        _emb("embedding backward, relative positions", "backward", 1024 * 1024, 66, 128, "relative"),
+        _emb("embedding backward: relative positions", "backward", 1024 * 1024, 66, 128, "relative"),
         # a vocabulary of subwords in bf16, scaled by sqrt(width), and its gradient
-        _emb("embedding step, vocabulary", "step", 8192, 32000, 1024, "zipf", "bfloat16", "int64", 32.0, 0),
+        _emb("embedding step: vocabulary", "step", 8192, 32000, 1024, "zipf", "bfloat16", "int64", 32.0, 0),
     ]
 
 
