@@ -18,6 +18,7 @@ from .triangle_attention import (  # noqa: F401
     TriangleAttentionEndingNode,
 )
 from .pair_transform import PairEmbedding, PairTransformLayer, PairTransformNet  # noqa: F401
+from .primitives import LayerNorm  # noqa: F401
 from .stack import TrianglePairStack  # noqa: F401
 from .utils import has_cuda_kernels, get_device_info  # noqa: F401
 from . import library  # noqa: F401  (registers torch.ops.genie_tk.*)
@@ -33,6 +34,7 @@ __all__ = [
     "PairTransformNet",
     "PairEmbedding",
     "TrianglePairStack",
+    "LayerNorm",
     "has_cuda_kernels",
     "get_device_info",
 ]

@@ -61,6 +61,15 @@ class Dropout(ctypes.Structure):
     _fields_ = [("keep_bits", c_vp), ("scale", ctypes.c_float), ("shared_across_rows", c_int)]
 
 
+class Rows(ctypes.Structure):
+    """Mirror of ``gtk_rows`` (include/genie_tk_b200.h)."""
+
+    _fields_ = [("size", c_i64 * 3), ("stride", c_i64 * 3)]
+
+
+# Element types of the training operators (include/genie_tk_b200.h)
+GTK_F32, GTK_BF16, GTK_F16 = 0, 1, 2
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "gtk_version": (c_int, []),
@@ -111,6 +120,11 @@ _SIGNATURES = {
     "gtk_dropout_keep_bits_philox": (c_int, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, c_i64, c_vp, c_vp]),
     "gtk_dropout_pack_keep_bits": (c_int, [c_vp, c_i64, c_vp, c_vp]),
     "gtk_layernorm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, ctypes.c_float, c_vp]),
+    "gtk_layernorm_forward": (c_int, [c_vp, ctypes.POINTER(Rows), c_int, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_i64,
+                                      c_i64, ctypes.c_float, c_vp]),
+    "gtk_layernorm_backward_workspace_bytes": (c_size, [c_i64, c_i64]),
+    "gtk_layernorm_backward": (c_int, [c_vp, ctypes.POINTER(Rows), c_vp, ctypes.POINTER(Rows), c_int, c_vp, c_int,
+                                       c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_vp]),
     "gtk_attn_core_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, ctypes.c_float,
                                       c_vp, c_vp, c_vp]),
     "gtk_attn_core_backward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_float, c_i64, c_i64,

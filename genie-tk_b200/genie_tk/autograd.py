@@ -25,6 +25,10 @@ recomputation of the block's math on the GPU:
 * Pair transition (pair_transform.py:78-84): recomputed and differentiated with
   PyTorch ops.
 
+Every LayerNorm of the recomputations runs forward and backward on the library's kernels
+(``gtk_layernorm_forward`` / ``gtk_layernorm_backward``; around the ending node they read the
+transposed pair tensor in place).
+
 The recomputations are fp32. Their GEMMs in the multiplicative update and the attention
 run on TF32 tensor cores while ``RECOMPUTE_TF32`` is true (the default): products with a
 10-bit mantissa and fp32 accumulation, relative error ~1e-3 against fp32, where the
@@ -40,6 +44,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -105,6 +110,42 @@ def contract(a: Tensor, b: Tensor, outgoing: bool) -> Tensor:
 
 
 # --------------------------------------------------------------------------------------
+# LayerNorm on the library's kernels
+# --------------------------------------------------------------------------------------
+
+class LayerNormFn(torch.autograd.Function):
+    """y = LayerNorm(x) over the last axis (gtk_layernorm_forward / _backward)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layernorm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = ops.layernorm_backward(dy.to(x.dtype), x, weight, mean, rstd, ctx.needs_input_grad[1],
+                                            ctx.needs_input_grad[2])
+        return dx, dw, db, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = LN_EPS) -> Tensor:
+    """Differentiable LayerNorm over the last axis on the library's kernels: x [*, D] fp32, bf16
+    or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNormFn.apply(x, weight, bias, eps)
+    return ops.layernorm_forward(x, weight, bias, eps)[0]
+
+
+def _ln(x: Tensor, p: Dict[str, Tensor], name: str) -> Tensor:
+    """LayerNorm of a recompute: on the library's kernels (CPU tensors: PyTorch's)."""
+    w, b = p[name + ".weight"], p[name + ".bias"]
+    return layer_norm(x, w, b, LN_EPS) if x.is_cuda else F.layer_norm(x, (x.shape[-1],), w, b, LN_EPS)
+
+
+# --------------------------------------------------------------------------------------
 # Recomputations (the reference math, differentiable)
 # --------------------------------------------------------------------------------------
 
@@ -141,12 +182,12 @@ def trimul_recompute(z: Tensor, mask: Optional[Tensor], p: Dict[str, Tensor], ou
     with the contraction on the library's kernel."""
     p = _fp32(p)
     m = _mask_or_ones(z, mask).unsqueeze(-1)
-    zn = F.layer_norm(z, (z.shape[-1],), p["layer_norm_in.weight"], p["layer_norm_in.bias"], LN_EPS)
+    zn = _ln(z, p, "layer_norm_in")
     ap, ag, bp, bg, g = _linear_cat(zn, p, ["linear_a_p", "linear_a_g", "linear_b_p", "linear_b_g", "linear_g"])
     a = ap * torch.sigmoid(ag) * m
     b = bp * torch.sigmoid(bg) * m
     x = contract(a, b, outgoing)
-    x = F.layer_norm(x, (x.shape[-1],), p["layer_norm_out.weight"], p["layer_norm_out.bias"], LN_EPS)
+    x = _ln(x, p, "layer_norm_out")
     return _linear(x, p, "linear_z") * torch.sigmoid(g)
 
 
@@ -190,7 +231,7 @@ def triatt_recompute(z: Tensor, mask: Optional[Tensor], p: Dict[str, Tensor], st
     if not starting:
         x = x.transpose(-2, -3)
         m = None if m is None else m.transpose(-1, -2)
-    xn = F.layer_norm(x, (x.shape[-1],), p["layer_norm.weight"], p["layer_norm.bias"], LN_EPS)
+    xn = _ln(x, p, "layer_norm")
     q, k, v, g, tri = _linear_cat(xn, p, ["mha.linear_q", "mha.linear_k", "mha.linear_v", "mha.linear_g", "linear"])
     m = None if m is None else m.float().contiguous()
     o = _attn_core(q.contiguous(), k.contiguous(), v.contiguous(), tri.permute(0, 3, 1, 2).contiguous(), m, heads,
@@ -203,7 +244,7 @@ def triatt_recompute(z: Tensor, mask: Optional[Tensor], p: Dict[str, Tensor], st
 def transition_recompute(z: Tensor, p: Dict[str, Tensor]) -> Tensor:
     """PairTransition.forward (pair_transform.py:78-84) in fp32."""
     p = _fp32(p)
-    x = F.layer_norm(z, (z.shape[-1],), p["layer_norm.weight"], p["layer_norm.bias"], LN_EPS)
+    x = _ln(z, p, "layer_norm")
     return _linear(torch.relu(_linear(x, p, "linear_1")), p, "linear_2")
 
 

@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from . import ops
+from . import autograd, ops
 
 
 def _init_weights(linear: nn.Linear, init: str = "default", std: float = 0.02) -> None:
@@ -52,6 +52,22 @@ class Linear(nn.Linear):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, init: str = "default"):
         super().__init__(in_features, out_features, bias=bias)
         _init_weights(self, init)
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm whose forward and backward run on the library's kernels (CUDA tensors only;
+    fp32, bf16 or fp16 inputs with parameters in fp32 or the input's type). Same constructor,
+    parameters and state dict; several normalised axes are normalised as one."""
+
+    def forward(self, x: Tensor) -> Tensor:
+        shape = self.normalized_shape
+        if tuple(x.shape[x.dim() - len(shape):]) != tuple(shape):
+            raise ValueError(f"genie_tk (B200): LayerNorm over {tuple(shape)} got an input of shape {tuple(x.shape)}")
+        if len(shape) == 1:
+            return autograd.layer_norm(x, self.weight, self.bias, self.eps)
+        w = None if self.weight is None else self.weight.reshape(-1)
+        b = None if self.bias is None else self.bias.reshape(-1)
+        return autograd.layer_norm(x.flatten(-len(shape)), w, b, self.eps).view(x.shape)
 
 
 def _attention_math(mod: "Attention", q_x: Tensor, k_x: Tensor, v_x: Tensor, biases: List[Tensor],

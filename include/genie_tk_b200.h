@@ -473,6 +473,35 @@ GTK_API int gtk_mha_forward(const float* q, const float* k, const float* v, cons
 GTK_API int gtk_layernorm(const float* x, const float* gamma, const float* beta, float* out, int64_t rows,
                           int64_t D, float eps, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * LayerNorm for training: the forward that keeps its statistics, and the backward.
+ * x, y, dy, dx are GTK_F32, GTK_BF16 or GTK_F16 (x_dtype); weight, bias and their gradients
+ * GTK_F32 or x's type (w_dtype). weight NULL: ones; bias NULL: zeros. mean, rstd fp32 [rows].
+ * rows < 2^31, D <= 2^20. fp32 arithmetic; each 16-bit result is rounded once.
+ * y and dx are [rows, D] row-major. x and dy are too, or (x_rows / dy_rows not NULL) their
+ * rows lie at strides of up to three leading axes: row (a size[1] + b) size[2] + c begins at
+ * element a stride[0] + b stride[1] + c stride[2] (a pair tensor read transposed).
+ * The backward writes dx; dweight / dbias may be NULL (both: no workspace needed). It uses no
+ * atomics: the same inputs give the same bits. Outputs must not overlap inputs.
+ * ------------------------------------------------------------------------------- */
+#define GTK_F32 0
+#define GTK_BF16 1
+#define GTK_F16 2
+
+typedef struct gtk_rows {
+  int64_t size[3];
+  int64_t stride[3];
+} gtk_rows;
+
+GTK_API int gtk_layernorm_forward(const void* x, const gtk_rows* x_rows, int x_dtype, const void* weight,
+                                  const void* bias, int w_dtype, void* y, float* mean, float* rstd, int64_t rows,
+                                  int64_t D, float eps, void* stream);
+GTK_API size_t gtk_layernorm_backward_workspace_bytes(int64_t rows, int64_t D);
+GTK_API int gtk_layernorm_backward(const void* dy, const gtk_rows* dy_rows, const void* x, const gtk_rows* x_rows,
+                                   int x_dtype, const void* weight, int w_dtype, const float* mean,
+                                   const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                                   size_t workspace_bytes, int64_t rows, int64_t D, void* stream);
+
 /* The reference's `_C.fused_layernorm_linear(x, gamma, beta, weight, bias, eps)`
  * (kernels/bindings.cpp:97-101; layernorm.cu:46-76): out = LayerNorm(x) weight^T + bias in
  * one kernel -- each CTA normalises its 64 rows while loading them, so the normalised rows
