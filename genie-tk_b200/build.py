@@ -1,10 +1,12 @@
-"""Build ``genie_tk/lib/libgenie_tk_b200.so`` from ``csrc/`` with nvcc for sm_100a.
+"""Build ``genie_tk/lib/libgenie_tk_b200.so`` from ``csrc/`` with nvcc for sm_100a, and its
+PyTorch binding ``genie_tk/lib/_gtk_torch.so`` from ``csrc_torch/`` with g++.
 
 Usage: ``python genie-tk_b200/build.py [--force] [-j N]``. Objects go to
 ``genie-tk_b200/_build/`` (git-ignored); the shared library is written in-tree next to
 the Python package so it travels with the repository snapshot. The library links the
 CUDA runtime statically and resolves the driver's tensor-map encoder at run time, so it
-has no libcuda link dependency.
+has no libcuda link dependency. The binding is compiled against the installed PyTorch and
+gets the library's entry points by address when it is loaded.
 """
 
 from __future__ import annotations
@@ -25,6 +27,10 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
               "--expt-relaxed-constexpr", "-Xptxas", "-v", "-I", INCLUDE]
+
+
+BINDING_SRC = os.path.join(HERE, "csrc_torch", "binding.cpp")
+BINDING_OUT = os.path.join(HERE, "genie_tk", "lib", "_gtk_torch.so")
 
 
 def nvcc():
@@ -56,11 +62,33 @@ def _compile(src, force):
     return obj, r.stderr
 
 
+def _build_binding(force):
+    deps = [BINDING_SRC, os.path.join(INCLUDE, "genie_tk_b200.h")]
+    if not force and os.path.exists(BINDING_OUT) and os.path.getmtime(BINDING_OUT) >= max(map(os.path.getmtime, deps)):
+        return ""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem", cuda,
+           "-isystem", sysconfig.get_paths()["include"], BINDING_SRC, "-o", BINDING_OUT,
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stdout}\n{r.stderr}")
+    return r.stderr
+
+
 def build(force: bool = False, jobs: int = 4, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        binding = ex.submit(_build_binding, force)
         results = list(ex.map(lambda s: _compile(s, force), sources()))
+        binding.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, log in results:

@@ -1,0 +1,429 @@
+// Python binding of the training operators: checks, allocations and the call of the C ABI
+// (include/genie_tk_b200.h) in one step, for calls that cost less than the interpreter's work
+// around them (a list of some hundred gradients, a LayerNorm over a few rows).
+//
+// The entry points of libgenie_tk_b200.so are handed over by address (`bind`), so the module
+// always runs on the library that genie_tk._lib loaded. Memory comes from PyTorch's caching
+// allocator on the current stream, and the kernels run on the tensors' device and its current
+// stream. Workspaces are allocated per call: two streams or two captured graphs never share one.
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
+#include <limits>
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "../../include/genie_tk_b200.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+namespace {
+
+struct Api {
+  decltype(&gtk_last_error_string) last_error = nullptr;
+  decltype(&gtk_layernorm_forward) layernorm_forward = nullptr;
+  decltype(&gtk_layernorm_backward) layernorm_backward = nullptr;
+  decltype(&gtk_layernorm_backward_workspace_bytes) layernorm_backward_workspace_bytes = nullptr;
+  decltype(&gtk_grad_norm_workspace_bytes) grad_norm_workspace_bytes = nullptr;
+  decltype(&gtk_grad_norm) grad_norm = nullptr;
+  decltype(&gtk_clip_grad_norm) clip_grad_norm = nullptr;
+  decltype(&gtk_embedding_forward) embedding_forward = nullptr;
+  decltype(&gtk_embedding_backward) embedding_backward = nullptr;
+  decltype(&gtk_embedding_backward_workspace_bytes) embedding_backward_workspace_bytes = nullptr;
+} api;
+
+template <typename F>
+void bind_one(const py::dict& addresses, const char* name, F* out) {
+  if (!addresses.contains(name)) throw py::key_error(name);
+  *out = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
+}
+
+void bind(const py::dict& d) {
+  bind_one(d, "gtk_last_error_string", &api.last_error);
+  bind_one(d, "gtk_layernorm_forward", &api.layernorm_forward);
+  bind_one(d, "gtk_layernorm_backward", &api.layernorm_backward);
+  bind_one(d, "gtk_layernorm_backward_workspace_bytes", &api.layernorm_backward_workspace_bytes);
+  bind_one(d, "gtk_grad_norm_workspace_bytes", &api.grad_norm_workspace_bytes);
+  bind_one(d, "gtk_grad_norm", &api.grad_norm);
+  bind_one(d, "gtk_clip_grad_norm", &api.clip_grad_norm);
+  bind_one(d, "gtk_embedding_forward", &api.embedding_forward);
+  bind_one(d, "gtk_embedding_backward", &api.embedding_backward);
+  bind_one(d, "gtk_embedding_backward_workspace_bytes", &api.embedding_backward_workspace_bytes);
+}
+
+const std::string kPrefix = "genie_tk (B200): ";
+
+[[noreturn]] void type_error(const std::string& m) { throw py::type_error(kPrefix + m); }
+[[noreturn]] void value_error(const std::string& m) { throw py::value_error(kPrefix + m); }
+
+void check(int rc, const char* what) {
+  if (rc) {
+    const char* m = api.last_error();
+    throw std::runtime_error(std::string(what) + " failed (" + std::to_string(rc) + "): " + (m ? m : ""));
+  }
+}
+
+// The dtype code of a tensor's elements, or -1.
+int code_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat:
+      return GTK_F32;
+    case at::kBFloat16:
+      return GTK_BF16;
+    case at::kHalf:
+      return GTK_F16;
+    default:
+      return -1;
+  }
+}
+
+std::string name_of(at::ScalarType t) { return c10::toString(t); }
+
+int dtype_code(const Tensor& t, const char* name) {
+  const int c = code_of(t.scalar_type());
+  if (c < 0)
+    type_error(std::string(name) + " must be float32, bfloat16 or float16, got " + name_of(t.scalar_type()));
+  return c;
+}
+
+void require_cuda(const Tensor& t, const char* name) {
+  if (!t.is_cuda())
+    throw std::runtime_error(kPrefix + name + " must be a CUDA tensor; this package has no CPU path");
+  if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
+}
+
+void same_device(const Tensor& t, c10::Device d, const char* name) {
+  if (!t.is_cuda() || t.device() != d)
+    throw std::runtime_error(kPrefix + name + " must be a CUDA tensor on device " + std::to_string(d.index()));
+  if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
+}
+
+std::string shape_of(const Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + ")";
+}
+
+Tensor contiguous(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+
+void* stream_of(c10::Device d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
+
+Tensor scratch(size_t bytes, const Tensor& like) {
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ---- LayerNorm ------------------------------------------------------------------------------
+
+// The rows of x [*, D]: contiguous, or strided leading axes that merge into at most three
+// (`used`), else a contiguous copy of x.
+Tensor row_view(const Tensor& x, gtk_rows* rows, bool* used) {
+  *used = false;
+  if (x.is_contiguous()) return x;
+  const int64_t last = x.dim() - 1;
+  if (x.stride(last) != 1 && x.size(last) != 1) return x.contiguous();
+  int64_t size[3], stride[3];
+  int n = 0;
+  for (int64_t i = 0; i < last; ++i) {
+    if (x.size(i) == 1) continue;
+    if (n && stride[n - 1] == x.stride(i) * x.size(i)) {
+      size[n - 1] *= x.size(i);
+      stride[n - 1] = x.stride(i);
+      continue;
+    }
+    if (n == 3) return x.contiguous();
+    size[n] = x.size(i);
+    stride[n++] = x.stride(i);
+  }
+  for (int i = 0; i < 3; ++i) {
+    const int k = i - (3 - n);
+    rows->size[i] = k < 0 ? 1 : size[k];
+    rows->stride[i] = k < 0 ? 0 : stride[k];
+  }
+  *used = true;
+  return x;
+}
+
+// A parameter of LayerNorm, contiguous; sets *code to its dtype code (-1 while there is none).
+Tensor parameter(const OptTensor& p, const Tensor& x, const char* name, int* code) {
+  if (!p || !p->defined()) return Tensor();
+  same_device(*p, x.device(), name);
+  const int64_t D = x.size(-1);
+  if (p->numel() != D)
+    value_error(std::string(name) + " must have " + std::to_string(D) + " elements, got " + shape_of(*p));
+  const int c = code_of(p->scalar_type());
+  if (c < 0 || (c != GTK_F32 && p->scalar_type() != x.scalar_type()) || (*code >= 0 && c != *code))
+    type_error("LayerNorm parameters must both be float32 or " + name_of(x.scalar_type()) + ", got " +
+               name_of(p->scalar_type()));
+  *code = c;
+  return contiguous(*p);
+}
+
+py::tuple layernorm_forward(const Tensor& x_in, const OptTensor& weight, const OptTensor& bias, double eps) {
+  require_cuda(x_in, "x");
+  if (x_in.dim() < 1 || x_in.size(-1) < 1) value_error("x must have a last axis of at least one element");
+  const int xt = dtype_code(x_in, "x");
+  at::NoGradGuard no_grad;
+  c10::cuda::CUDAGuard guard(x_in.device());
+  int wt = -1;
+  const Tensor w = parameter(weight, x_in, "weight", &wt), b = parameter(bias, x_in, "bias", &wt);
+  const int64_t D = x_in.size(-1);
+  Tensor y = at::empty(x_in.sizes(), x_in.options());
+  const auto lead = x_in.sizes().slice(0, x_in.dim() - 1);
+  Tensor mean = at::empty(lead, x_in.options().dtype(at::kFloat));
+  Tensor rstd = at::empty(lead, mean.options());
+  const int64_t n = mean.numel();
+  if (n) {
+    gtk_rows rows;
+    bool used;
+    const Tensor x = row_view(x_in, &rows, &used);
+    check(api.layernorm_forward(x.data_ptr(), used ? &rows : nullptr, xt, ptr(w), ptr(b), wt < 0 ? xt : wt,
+                                y.data_ptr(), static_cast<float*>(mean.data_ptr()),
+                                static_cast<float*>(rstd.data_ptr()), n, D, static_cast<float>(eps),
+                                stream_of(x.device())),
+          "gtk_layernorm_forward");
+  }
+  return py::make_tuple(std::move(y), std::move(mean), std::move(rstd));
+}
+
+py::tuple layernorm_backward(const Tensor& dy_in, const Tensor& x_in, const OptTensor& weight, const Tensor& mean_in,
+                             const Tensor& rstd_in, bool need_weight, bool need_bias) {
+  require_cuda(x_in, "x");
+  const int xt = dtype_code(x_in, "x");
+  same_device(dy_in, x_in.device(), "dy");
+  same_device(mean_in, x_in.device(), "mean");
+  same_device(rstd_in, x_in.device(), "rstd");
+  if (dy_in.sizes() != x_in.sizes() || dy_in.scalar_type() != x_in.scalar_type())
+    value_error("dy must have x's shape and type, got " + shape_of(dy_in) + " " + name_of(dy_in.scalar_type()));
+  if (x_in.dim() < 1 || x_in.size(-1) < 1) value_error("x must have a last axis of at least one element");
+  const int64_t D = x_in.size(-1), n = mean_in.numel();
+  if (n * D != x_in.numel() || rstd_in.numel() != n)
+    value_error("mean and rstd must have one element for each row of x");
+  if (mean_in.scalar_type() != at::kFloat || rstd_in.scalar_type() != at::kFloat)
+    type_error("mean and rstd must be float32");
+  at::NoGradGuard no_grad;
+  c10::cuda::CUDAGuard guard(x_in.device());
+  int wt = -1;
+  const Tensor w = parameter(weight, x_in, "weight", &wt);
+  if (wt < 0) wt = xt;
+  const auto options = x_in.options().dtype(w.defined() ? w.scalar_type() : x_in.scalar_type());
+  Tensor dx = at::empty(x_in.sizes(), x_in.options()), dw, db;
+  if (need_weight) dw = n ? at::empty({D}, options) : at::zeros({D}, options);
+  if (need_bias) db = n ? at::empty({D}, options) : at::zeros({D}, options);
+  if (n) {
+    const size_t bytes = need_weight || need_bias ? api.layernorm_backward_workspace_bytes(n, D) : 0;
+    Tensor ws;
+    if (bytes) ws = scratch(bytes, x_in);
+    const Tensor mean = contiguous(mean_in), rstd = contiguous(rstd_in);
+    gtk_rows xr, dr;
+    bool xu, du;
+    const Tensor x = row_view(x_in, &xr, &xu), dy = row_view(dy_in, &dr, &du);
+    check(api.layernorm_backward(dy.data_ptr(), du ? &dr : nullptr, x.data_ptr(), xu ? &xr : nullptr, xt, ptr(w), wt,
+                                 static_cast<const float*>(mean.data_ptr()),
+                                 static_cast<const float*>(rstd.data_ptr()), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws),
+                                 bytes, n, D, stream_of(x.device())),
+          "gtk_layernorm_backward");
+  }
+  return py::make_tuple(dx, need_weight ? py::cast(dw) : py::none(), need_bias ? py::cast(db) : py::none());
+}
+
+// ---- The global gradient norm -----------------------------------------------------------------
+
+struct Gradients {
+  std::vector<const void*> in;
+  std::vector<void*> out;
+  std::vector<int64_t> numel;
+  std::vector<int> in_type, out_type;
+  std::vector<Tensor> keep;                           // copies of strided gradients
+  std::vector<std::pair<Tensor, Tensor>> write_back;  // (gradient, its clipped copy)
+};
+
+const Tensor& tensor_at(PyObject* o, const char* name, Py_ssize_t i) {
+  if (!THPVariable_Check(o)) type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
+  return THPVariable_Unpack(o);
+}
+
+// Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
+c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip, Gradients* g) {
+  py::object fast = py::reinterpret_steal<py::object>(PySequence_Fast(grads.ptr(), "grads must be a sequence"));
+  if (!fast) throw py::error_already_set();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
+  if (n == 0) value_error("the list of gradients is empty");
+  py::object fast_out;
+  if (outs) {
+    fast_out = py::reinterpret_steal<py::object>(PySequence_Fast(outs->ptr(), "out must be a sequence"));
+    if (!fast_out) throw py::error_already_set();
+    if (PySequence_Fast_GET_SIZE(fast_out.ptr()) != n) value_error("out must have one tensor for each gradient");
+  }
+  g->in.reserve(n);
+  g->numel.reserve(n);
+  g->in_type.reserve(n);
+  if (outs) {
+    g->out.reserve(n);
+    g->out_type.reserve(n);
+  }
+  std::optional<c10::Device> device;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor& t = tensor_at(PySequence_Fast_GET_ITEM(fast.ptr(), i), "grads", i);
+    if (!device) {
+      require_cuda(t, "grads[0]");
+      device = t.device();
+    } else {
+      if (!t.is_cuda() || t.device() != *device)
+        throw std::runtime_error(kPrefix + "all gradients must be CUDA tensors on one device");
+      if (t.layout() != at::kStrided) type_error("gradients must be dense tensors");
+    }
+    const int code = code_of(t.scalar_type());
+    if (code < 0) type_error("gradients must be float32, bfloat16 or float16, got " + name_of(t.scalar_type()));
+    Tensor src = t;
+    if (outs) {
+      const Tensor& o = tensor_at(PySequence_Fast_GET_ITEM(fast_out.ptr(), i), "out", i);
+      if (!o.is_cuda() || o.device() != *device || o.layout() != at::kStrided)
+        throw std::runtime_error(kPrefix + "out must hold dense CUDA tensors on the gradients' device");
+      if (o.sizes() != t.sizes()) value_error("out[" + std::to_string(i) + "] must have its gradient's shape");
+      if (o.scalar_type() != at::kFloat && o.scalar_type() != t.scalar_type())
+        type_error("out must be float32 or the gradient's type, got " + name_of(o.scalar_type()));
+      if (!(t.is_contiguous() && o.is_contiguous()) &&
+          !(t.is_non_overlapping_and_dense() && t.strides() == o.strides())) {
+        if (!o.is_contiguous()) value_error("out[" + std::to_string(i) + "] must be contiguous");
+        src = t.contiguous();
+        g->keep.push_back(src);
+      }
+      g->out.push_back(o.data_ptr());
+      g->out_type.push_back(code_of(o.scalar_type()));
+      if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+    } else if (!t.is_contiguous() && !t.is_non_overlapping_and_dense()) {
+      src = t.contiguous();
+      g->keep.push_back(src);
+      if (clip) g->write_back.emplace_back(t, src);
+    } else if (clip && !t.is_inference()) {
+      t.unsafeGetTensorImpl()->bump_version();
+    }
+    g->in.push_back(src.data_ptr());
+    g->numel.push_back(src.numel());
+    g->in_type.push_back(code);
+  }
+  return *device;
+}
+
+int norm_kind(double norm_type) {
+  if (norm_type == 2.0) return GTK_NORM_2;
+  if (norm_type == std::numeric_limits<double>::infinity()) return GTK_NORM_INF;
+  value_error("norm_type must be 2.0 or inf, got " + std::to_string(norm_type));
+}
+
+Tensor grad_norm(const py::sequence& grads, double norm_type) {
+  const int kind = norm_kind(norm_type);
+  at::NoGradGuard no_grad;
+  Gradients g;
+  const c10::Device device = collect(grads, nullptr, false, &g);
+  c10::cuda::CUDAGuard guard(device);
+  Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+  const size_t bytes = api.grad_norm_workspace_bytes(g.in.size());
+  Tensor ws = scratch(bytes, norm);
+  check(api.grad_norm(g.in.data(), g.numel.data(), g.in_type.data(), g.in.size(), kind,
+                      static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes, stream_of(device)),
+        "gtk_grad_norm");
+  return norm;
+}
+
+Tensor clip_grad_norm(const py::sequence& grads, double max_norm, double norm_type, const py::object& out) {
+  const int kind = norm_kind(norm_type);
+  if (!(max_norm >= 0.0)) value_error("max_norm must be a number >= 0, got " + std::to_string(max_norm));
+  at::NoGradGuard no_grad;
+  Gradients g;
+  const bool in_place = out.is_none();
+  const c10::Device device = collect(grads, in_place ? nullptr : &out, true, &g);
+  c10::cuda::CUDAGuard guard(device);
+  Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+  const size_t bytes = api.grad_norm_workspace_bytes(g.in.size());
+  Tensor ws = scratch(bytes, norm);
+  check(api.clip_grad_norm(g.in.data(), in_place ? nullptr : g.out.data(), g.numel.data(), g.in_type.data(),
+                           in_place ? nullptr : g.out_type.data(), g.in.size(), kind, max_norm,
+                           static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes, stream_of(device)),
+        "gtk_clip_grad_norm");
+  for (auto& p : g.write_back) p.first.copy_(p.second);
+  return norm;
+}
+
+// ---- Embedding ----------------------------------------------------------------------------------
+
+int index_bits(const Tensor& tokens) {
+  if (tokens.scalar_type() == at::kLong) return 64;
+  if (tokens.scalar_type() == at::kInt) return 32;
+  type_error("tokens must be int32 or int64, got " + name_of(tokens.scalar_type()));
+}
+
+Tensor embedding_forward(const Tensor& tokens_in, const Tensor& weight_in, double scale, uintptr_t status) {
+  require_cuda(weight_in, "weight");
+  same_device(tokens_in, weight_in.device(), "tokens");
+  const int bits = index_bits(tokens_in);
+  const int dt = dtype_code(weight_in, "weight");
+  if (weight_in.dim() != 2 || weight_in.size(0) < 1)
+    value_error("weight must be [vocabulary, width], got " + shape_of(weight_in));
+  at::NoGradGuard no_grad;
+  c10::cuda::CUDAGuard guard(weight_in.device());
+  std::vector<int64_t> shape = tokens_in.sizes().vec();
+  shape.push_back(weight_in.size(1));
+  Tensor y = at::empty(shape, weight_in.options());
+  if (y.numel()) {
+    const Tensor tokens = contiguous(tokens_in), weight = contiguous(weight_in);
+    check(api.embedding_forward(tokens.data_ptr(), bits, weight.data_ptr(), dt, y.data_ptr(), tokens.numel(),
+                                weight.size(0), weight.size(1), static_cast<float>(scale),
+                                reinterpret_cast<uint32_t*>(status), stream_of(weight.device())),
+          "gtk_embedding_forward");
+  }
+  return y;
+}
+
+Tensor embedding_backward(const Tensor& dy_in, const Tensor& tokens_in, int64_t vocab, double scale,
+                          std::optional<int64_t> padding, std::optional<at::ScalarType> dtype, uintptr_t status) {
+  require_cuda(dy_in, "dy");
+  same_device(tokens_in, dy_in.device(), "tokens");
+  const int bits = index_bits(tokens_in);
+  const int gt = dtype_code(dy_in, "dy");
+  if (dy_in.dim() != tokens_in.dim() + 1 || dy_in.sizes().slice(0, tokens_in.dim()) != tokens_in.sizes())
+    value_error("dy must be [*tokens.shape, width], got " + shape_of(dy_in) + " for tokens " + shape_of(tokens_in));
+  if (vocab < 1) value_error("the vocabulary must have at least one token");
+  const at::ScalarType wd = dtype.value_or(dy_in.scalar_type());
+  if (wd != at::kFloat && wd != dy_in.scalar_type())
+    type_error("the table's gradient must be float32 or dy's type, got " + name_of(wd));
+  if (padding && (*padding < 0 || *padding >= vocab))
+    value_error("padding_idx must be a token of the vocabulary, got " + std::to_string(*padding));
+  at::NoGradGuard no_grad;
+  c10::cuda::CUDAGuard guard(dy_in.device());
+  const int64_t D = dy_in.size(-1), n = tokens_in.numel();
+  const auto options = dy_in.options().dtype(wd);
+  if (n == 0 || D == 0) return at::zeros({vocab, D}, options);
+  Tensor dw = at::empty({vocab, D}, options);
+  const Tensor tokens = contiguous(tokens_in), dy = contiguous(dy_in);
+  const size_t bytes = api.embedding_backward_workspace_bytes(n, vocab, D);
+  Tensor ws = scratch(bytes, dy);
+  check(api.embedding_backward(dy.data_ptr(), gt, tokens.data_ptr(), bits, dw.data_ptr(), code_of(wd), n, vocab, D,
+                               static_cast<float>(scale), padding.value_or(-1), ws.data_ptr(), bytes,
+                               reinterpret_cast<uint32_t*>(status), stream_of(dy.device())),
+        "gtk_embedding_backward");
+  return dw;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_gtk_torch, m) {
+  m.doc() = "PyTorch binding of the training operators of libgenie_tk_b200.so";
+  m.def("bind", &bind);
+  m.def("layernorm_forward", &layernorm_forward);
+  m.def("layernorm_backward", &layernorm_backward);
+  m.def("grad_norm", &grad_norm);
+  m.def("clip_grad_norm", &clip_grad_norm);
+  m.def("embedding_forward", &embedding_forward);
+  m.def("embedding_backward", &embedding_backward);
+}

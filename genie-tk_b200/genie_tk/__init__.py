@@ -18,9 +18,9 @@ from .triangle_attention import (  # noqa: F401
     TriangleAttentionEndingNode,
 )
 from .pair_transform import PairEmbedding, PairTransformLayer, PairTransformNet  # noqa: F401
-from .primitives import LayerNorm  # noqa: F401
+from .primitives import Embedding, LayerNorm  # noqa: F401
 from .stack import TrianglePairStack  # noqa: F401
-from .utils import has_cuda_kernels, get_device_info  # noqa: F401
+from .utils import clip_grad_norm_, has_cuda_kernels, get_device_info  # noqa: F401
 from . import library  # noqa: F401  (registers torch.ops.genie_tk.*)
 
 __all__ = [
@@ -35,6 +35,8 @@ __all__ = [
     "PairEmbedding",
     "TrianglePairStack",
     "LayerNorm",
+    "Embedding",
+    "clip_grad_norm_",
     "has_cuda_kernels",
     "get_device_info",
 ]

@@ -7,14 +7,20 @@ loaded, every op raises ``RuntimeError`` -- there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GENIE_TK_B200_LIB", os.path.join(_HERE, "lib", "libgenie_tk_b200.so"))
 
+# The PyTorch binding of the training operators (csrc_torch/binding.cpp)
+BINDING_PATH = os.path.join(_HERE, "lib", "_gtk_torch.so")
+
 _lock = threading.Lock()
 _lib = None
+_native = None
 _load_error = None
 
 c_i64 = ctypes.c_int64
@@ -125,6 +131,15 @@ _SIGNATURES = {
     "gtk_layernorm_backward_workspace_bytes": (c_size, [c_i64, c_i64]),
     "gtk_layernorm_backward": (c_int, [c_vp, ctypes.POINTER(Rows), c_vp, ctypes.POINTER(Rows), c_int, c_vp, c_int,
                                        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_vp]),
+    "gtk_grad_norm_workspace_bytes": (c_size, [c_i64]),
+    "gtk_grad_norm": (c_int, [c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_size, c_vp]),
+    "gtk_clip_grad_norm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, ctypes.c_double, c_vp, c_vp, c_size,
+                                   c_vp]),
+    "gtk_embedding_forward": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, ctypes.c_float, c_vp,
+                                      c_vp]),
+    "gtk_embedding_backward_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "gtk_embedding_backward": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, ctypes.c_float,
+                                       c_i64, c_vp, c_size, c_vp, c_vp]),
     "gtk_attn_core_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, ctypes.c_float,
                                       c_vp, c_vp, c_vp]),
     "gtk_attn_core_backward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_float, c_i64, c_i64,
@@ -146,6 +161,13 @@ _SIGNATURES = {
     "gtk_triatt_forward_dropout": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_int, ctypes.POINTER(Dropout), c_vp, c_size,
                                            c_i64, c_i64, c_int, c_int, c_int, ctypes.c_float, c_vp, c_vp]),
 }
+
+
+# Entry points that the binding calls
+_NATIVE_ENTRY_POINTS = ("gtk_last_error_string", "gtk_layernorm_forward", "gtk_layernorm_backward",
+                        "gtk_layernorm_backward_workspace_bytes", "gtk_grad_norm_workspace_bytes", "gtk_grad_norm",
+                        "gtk_clip_grad_norm", "gtk_embedding_forward", "gtk_embedding_backward",
+                        "gtk_embedding_backward_workspace_bytes")
 
 
 def exported_names():
@@ -171,6 +193,26 @@ def load(required: bool = True):
     if _lib is None and required:
         raise RuntimeError(_load_error or f"cannot load {LIB_PATH}")
     return _lib
+
+
+def native():
+    """Load (once) and return the PyTorch binding of the training operators, bound to the entry
+    points of the library that ``load`` returns; raise RuntimeError if it is absent."""
+    global _native
+    if _native is None:
+        lib = load()
+        with _lock:
+            if _native is None:
+                try:
+                    loader = importlib.machinery.ExtensionFileLoader("_gtk_torch", BINDING_PATH)
+                    spec = importlib.util.spec_from_file_location("_gtk_torch", BINDING_PATH, loader=loader)
+                    mod = importlib.util.module_from_spec(spec)
+                    loader.exec_module(mod)
+                except (ImportError, OSError) as e:
+                    raise RuntimeError(f"cannot load {BINDING_PATH}: {e}") from e
+                mod.bind({n: ctypes.cast(getattr(lib, n), c_vp).value for n in _NATIVE_ENTRY_POINTS})
+                _native = mod
+    return _native
 
 
 def available() -> bool:

@@ -110,7 +110,7 @@ def contract(a: Tensor, b: Tensor, outgoing: bool) -> Tensor:
 
 
 # --------------------------------------------------------------------------------------
-# LayerNorm on the library's kernels
+# LayerNorm and the embedding lookup on the library's kernels
 # --------------------------------------------------------------------------------------
 
 class LayerNormFn(torch.autograd.Function):
@@ -137,6 +137,33 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return LayerNormFn.apply(x, weight, bias, eps)
     return ops.layernorm_forward(x, weight, bias, eps)[0]
+
+
+class EmbeddingFn(torch.autograd.Function):
+    """y = scale * weight[tokens] (gtk_embedding_forward / _backward)."""
+
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding_idx):
+        ctx.save_for_backward(tokens)
+        ctx.table = (weight.shape[0], weight.dtype)
+        ctx.scale, ctx.padding_idx = scale, padding_idx
+        return ops.embedding_forward(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        tokens, = ctx.saved_tensors
+        rows, dtype = ctx.table
+        return None, ops.embedding_backward(dy.to(dtype), tokens, rows, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
+    """Differentiable scale * weight[tokens] on the library's kernels: tokens int32 or int64 [*],
+    weight [vocabulary, D]; the row ``padding_idx`` gets no gradient. Once differentiable; the
+    table's gradient is dense and the same from run to run."""
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return EmbeddingFn.apply(tokens, weight, scale, padding_idx)
+    return ops.embedding_forward(tokens, weight, scale)
 
 
 def _ln(x: Tensor, p: Dict[str, Tensor], name: str) -> Tensor:

@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
-from typing import Dict, Optional
+from typing import Dict, Optional, Sequence
 
 import torch
 
@@ -601,106 +601,20 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: flo
 
 
 # --------------------------------------------------------------------------------------
-# Training operators: shared argument handling
+# Training operators (csrc_torch/binding.cpp checks the arguments, allocates and calls the C ABI).
+# They work on the tensors' device and its current stream, whichever device is current; their
+# workspaces belong to the call. They take no part in autograd: genie_tk.autograd has the
+# differentiable forms.
 # --------------------------------------------------------------------------------------
-
-_DTYPE_CODES = {torch.float32: _lib.GTK_F32, torch.bfloat16: _lib.GTK_BF16, torch.float16: _lib.GTK_F16}
-
-
-def _dtype_code(t: torch.Tensor, name: str) -> int:
-    code = _DTYPE_CODES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"genie_tk (B200): {name} must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
-
-
-def _same_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != index):
-            raise RuntimeError(f"genie_tk (B200): {name} must be a CUDA tensor on device {index}")
-
-
-def _enqueue(what: str, index: int, fn, *args) -> None:
-    """Call the C entry point ``fn(*args, stream)`` on device ``index`` and its current stream,
-    whichever device is current."""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
-    if rc:
-        _lib.check(rc, what)
-
-
-# --------------------------------------------------------------------------------------
-# LayerNorm for training: forward with statistics, backward with the parameters' gradients
-# --------------------------------------------------------------------------------------
-
-def _row_view(x: torch.Tensor):
-    """(tensor, gtk_rows or None) of the rows of x [*, D]: None when they follow one another;
-    strided leading axes that merge into at most three are read in place, others are copied."""
-    if x.is_contiguous():
-        return x, None
-    if x.stride(-1) != 1 and x.shape[-1] != 1:
-        return x.contiguous(), None
-    levels = []  # merged (size, stride) of the leading axes, outermost first
-    for n, st in zip(x.shape[:-1], x.stride()[:-1]):
-        if n == 1:
-            continue
-        if levels and levels[-1][1] == st * n:
-            levels[-1] = (levels[-1][0] * n, st)
-        else:
-            levels.append((n, st))
-    if len(levels) > 3:
-        return x.contiguous(), None
-    levels = [(1, 0)] * (3 - len(levels)) + levels
-    return x, _lib.Rows((ctypes.c_int64 * 3)(*[n for n, _ in levels]), (ctypes.c_int64 * 3)(*[st for _, st in levels]))
-
-
-def _layernorm_params(x: torch.Tensor, index: int, **params: Optional[torch.Tensor]):
-    """(dtype code, contiguous tensors) of LayerNorm's parameters."""
-    D = x.shape[-1]
-    _same_device(index, **params)
-    dtype = None
-    out = []
-    for name, t in params.items():
-        if t is None:
-            out.append(None)
-            continue
-        if t.numel() != D:
-            raise ValueError(f"genie_tk (B200): {name} must have {D} elements, got {tuple(t.shape)}")
-        if t.dtype not in (x.dtype, torch.float32) or (dtype is not None and t.dtype != dtype):
-            raise TypeError(f"genie_tk (B200): LayerNorm parameters must both be float32 or {x.dtype}, got {t.dtype}")
-        dtype = t.dtype
-        out.append(t if t.is_contiguous() else t.contiguous())
-    return _DTYPE_CODES[dtype or x.dtype], out
-
 
 def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                       eps: float = 1e-5):
     """LayerNorm over the last axis that keeps what its backward needs: (y, mean, rstd).
 
-    x [*, D] fp32, bf16 or fp16 (strided leading axes are read in place); weight and bias [D]
-    in fp32 or x's type, or None; y is contiguous, of x's type; mean and rstd fp32 [*]."""
-    lib = _lib.load()
-    _require_cuda(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("genie_tk (B200): x must have a last axis of at least one element")
-    xt, index = _dtype_code(x, "x"), x.get_device()
-    wt, (w, b) = _layernorm_params(x, index, weight=weight, bias=bias)
-    D = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    rows = mean.numel()
-    if rows == 0:
-        return y, mean, rstd
-    x, view = _row_view(x)
-    _enqueue("gtk_layernorm_forward", index, lib.gtk_layernorm_forward, x.data_ptr(), view, xt,
-             None if w is None else w.data_ptr(), None if b is None else b.data_ptr(), wt, y.data_ptr(),
-             mean.data_ptr(), rstd.data_ptr(), rows, D, eps)
-    return y, mean, rstd
+    x [*, D] fp32, bf16 or fp16 (strided leading axes that merge into at most three are read in
+    place, others copied); weight and bias [D] in fp32 or x's type, or None; y is contiguous, of
+    x's type; mean and rstd fp32 [*]. D <= 2^20, fewer than 2^31 rows."""
+    return _lib.native().layernorm_forward(x, weight, bias, eps)
 
 
 def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
@@ -709,38 +623,56 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
 
     dy has x's shape and type; mean and rstd are the forward's. dx is contiguous. The
     parameters' gradients have ``weight``'s type (x's without a weight); one that is not
-    needed is None."""
-    lib = _lib.load()
-    _require_cuda(x, "x")
-    xt, index = _dtype_code(x, "x"), x.get_device()
-    _same_device(index, dy=dy, mean=mean, rstd=rstd)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError(f"genie_tk (B200): dy must have x's shape and type, got {tuple(dy.shape)} {dy.dtype}")
-    D = x.shape[-1]
-    rows = mean.numel()
-    if D < 1 or rows * D != x.numel() or rstd.numel() != rows:
-        raise ValueError("genie_tk (B200): mean and rstd must have one element for each row of x")
-    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
-        raise TypeError("genie_tk (B200): mean and rstd must be float32")
-    wt, (w,) = _layernorm_params(x, index, weight=weight)
-    wdtype = x.dtype if weight is None else weight.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    make = torch.empty if rows else torch.zeros
-    dw = make(D, dtype=wdtype, device=x.device) if need_weight else None
-    db = make(D, dtype=wdtype, device=x.device) if need_bias else None
-    if rows == 0:
-        return dx, dw, db
-    nbytes = lib.gtk_layernorm_backward_workspace_bytes(rows, D) if need_weight or need_bias else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    mean = mean if mean.is_contiguous() else mean.contiguous()
-    rstd = rstd if rstd.is_contiguous() else rstd.contiguous()
-    x, xv = _row_view(x)
-    dy, dv = _row_view(dy)
-    _enqueue("gtk_layernorm_backward", index, lib.gtk_layernorm_backward, dy.data_ptr(), dv, x.data_ptr(), xv, xt,
-             None if w is None else w.data_ptr(), wt, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-             None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
-             None if ws is None else ws.data_ptr(), nbytes, rows, D)
-    return dx, dw, db
+    needed is None. The same inputs give the same bits."""
+    return _lib.native().layernorm_backward(dy, x, weight, mean, rstd, need_weight, need_bias)
+
+
+def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm over all elements of ``grads`` (fp32, bf16 or fp16, on one device) as a 0-d fp32
+    tensor on that device: the 2-norm, or with ``norm_type=inf`` the largest magnitude."""
+    return _lib.native().grad_norm(grads, norm_type)
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                   out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Scale ``grads`` by min(1, max_norm / (norm + 1e-6)) in place, or into ``out`` (one tensor
+    for each gradient, of its shape, in its type or fp32), and return ``grad_norm(grads)``.
+
+    The factor comes from the norm in 64 bits (which the returned fp32 may have rounded to
+    infinity); it is NaN when a gradient is and 0 when one is infinite. The written tensors must not
+    overlap one another, nor other gradients (the same tensor twice is refused). Nothing is
+    copied to or from the host."""
+    return _lib.native().clip_grad_norm(grads, max_norm, norm_type, out)
+
+
+def _status_address(device: torch.device) -> int:
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    buf = _status_bufs.get(idx)
+    if buf is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("genie_tk (B200): the device's status word must exist before a graph is captured: run "
+                               "the operator once, or call ops.status_buffer(device), outside the capture")
+        buf = status_buffer(device)
+    return buf.data_ptr()
+
+
+def embedding_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[tokens]: tokens int32 or int64 [*], weight [vocabulary, D] fp32, bf16 or
+    fp16; returns [*, D] in weight's type. A token outside the vocabulary gives a row of zeros
+    and sets GTK_STATUS_BAD_TOKEN (0x80) in the device's status word (``check_status``)."""
+    _require_cuda(weight, "weight")
+    return _lib.native().embedding_forward(tokens, weight, scale, _status_address(weight.device))
+
+
+def embedding_backward(dy: torch.Tensor, tokens: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The table's gradient [num_embeddings, D] of ``embedding_forward`` for dy [*, D]:
+    row v is scale * the sum of the dy rows whose token is v, and zeros for ``padding_idx``
+    and for tokens that do not occur. ``dtype`` is dy's (the default) or fp32. Tokens outside the
+    vocabulary are left out and set GTK_STATUS_BAD_TOKEN. The same inputs give the same bits."""
+    _require_cuda(dy, "dy")
+    return _lib.native().embedding_backward(dy, tokens, num_embeddings, scale, padding_idx, dtype,
+                                            _status_address(dy.device))
 
 
 # --------------------------------------------------------------------------------------

@@ -70,6 +70,22 @@ class LayerNorm(nn.LayerNorm):
         return autograd.layer_norm(x.flatten(-len(shape)), w, b, self.eps).view(x.shape)
 
 
+class Embedding(nn.Embedding):
+    """nn.Embedding whose lookup and dense gradient run on the library's kernels, with the rows
+    multiplied by ``scale``: residue types to the single representation, relative positions or
+    chain relations (int [B, N, N]) to the pair representation. int32 or int64 tokens, CUDA
+    tensors only; the state dict is nn.Embedding's. A token outside the table gives zeros and
+    sets a status bit (``ops.embedding_forward``) instead of failing on the device."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None,
+                 scale: float = 1.0, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+        self.scale = float(scale)
+
+    def forward(self, tokens: Tensor) -> Tensor:
+        return autograd.embedding(tokens, self.weight, self.scale, self.padding_idx)
+
+
 def _attention_math(mod: "Attention", q_x: Tensor, k_x: Tensor, v_x: Tensor, biases: List[Tensor],
                     params: List[Tensor]) -> Tensor:
     """The reference's Attention.forward (primitives.py:114-178) in fp32 PyTorch ops; the

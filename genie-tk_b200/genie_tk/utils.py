@@ -2,12 +2,13 @@
 
 from __future__ import annotations
 
-from typing import Any, Callable, Dict
+import math
+from typing import Any, Callable, Dict, Iterable, Union
 
 import torch
 from torch import Tensor
 
-from . import _lib
+from . import _lib, ops
 
 
 def has_cuda_kernels() -> bool:
@@ -37,6 +38,25 @@ def get_device_info() -> Dict[str, Any]:
                 "multi_processor_count": props.multi_processor_count,
             })
     return info
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> Tensor:
+    """torch.nn.utils.clip_grad_norm_ on the library's kernels: scale the parameters' gradients
+    in place by min(1, max_norm / (norm + 1e-6)) and return their total norm (0-d, fp32).
+
+    ``norm_type`` is 2.0 or inf. Two launches for up to 1000 gradients, nothing copied to or from
+    the host; with ``error_if_nonfinite`` the norm is read back first, and a norm that is NaN or
+    infinite raises with the gradients left as they were."""
+    if isinstance(parameters, Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite and not math.isfinite(float(ops.grad_norm(grads, float(norm_type)))):
+        raise RuntimeError(f"genie_tk (B200): the total norm of order {norm_type} of the gradients is not finite, so it "
+                           "cannot be clipped; error_if_nonfinite=False scales by it anyway")
+    return ops.clip_grad_norm(grads, float(max_norm), float(norm_type))
 
 
 def permute_final_dims(tensor: Tensor, *dims: int) -> Tensor:

@@ -67,6 +67,9 @@ extern "C" {
  * inputs and weights of the usual 1/fan_in scale; inputs or weights large enough to leave
  * that range set this bit instead of returning a silently wrong answer. */
 #define GTK_STATUS_FP16_SATURATED 0x40u
+/* A token outside 0 .. vocab-1 reached the embedding operators: its row of the lookup is
+ * zeros, and the table's gradient leaves it out. */
+#define GTK_STATUS_BAD_TOKEN 0x80u
 
 /* Library version (major*10000 + minor*100 + patch). */
 GTK_API int gtk_version(void);
@@ -501,6 +504,47 @@ GTK_API int gtk_layernorm_backward(const void* dy, const gtk_rows* dy_rows, cons
                                    int x_dtype, const void* weight, int w_dtype, const float* mean,
                                    const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
                                    size_t workspace_bytes, int64_t rows, int64_t D, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * The global norm of many gradients, and clipping by it (torch.nn.utils.clip_grad_norm_):
+ * norm = the 2-norm (GTK_NORM_2) or the largest magnitude (GTK_NORM_INF, with NaN above all)
+ * over all tensors; outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)).
+ * grads, outs, numel, dtypes, out_dtypes are host arrays of n_tensors entries; the pointers in
+ * grads and outs are device pointers to contiguous elements, at any alignment of their type.
+ * outs NULL: in place (nothing is written when the factor is 1). out_dtypes[i] is dtypes[i] or
+ * GTK_F32; NULL: dtypes. Tensors that are written must not overlap one another, nor another
+ * gradient. norm: fp32 on the device. Sums are in 64 bits; no atomics. The host arrays are read
+ * during the call only.
+ * ------------------------------------------------------------------------------- */
+#define GTK_NORM_2 2
+#define GTK_NORM_INF 0
+
+GTK_API size_t gtk_grad_norm_workspace_bytes(int64_t n_tensors);
+GTK_API int gtk_grad_norm(const void* const* grads, const int64_t* numel, const int* dtypes, int64_t n_tensors,
+                          int norm_kind, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+GTK_API int gtk_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* numel, const int* dtypes,
+                               const int* out_dtypes, int64_t n_tensors, int norm_kind, double max_norm, float* norm,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Embedding lookup with scaling, and its gradient by sorted tokens:
+ *   y[t, :]       = scale * weight[tokens[t], :]
+ *   dweight[v, :] = scale * sum over the t with tokens[t] = v of dy[t, :]
+ * tokens int32 or int64 (index_bits) [n_tokens]; weight [vocab, D] and y [n_tokens, D] of one
+ * type (dtype); dy [n_tokens, D] (dy_dtype), dweight [vocab, D] in GTK_F32 or dy's type, all of
+ * it written. n_tokens, vocab < 2^31, D <= 2^20. The row `padding` (-1: none) of dweight is
+ * zeros; the lookup reads it like any other. Tokens out of range set GTK_STATUS_BAD_TOKEN.
+ * fp32 and 64-bit sums in a fixed order, one rounding at the end; no floating-point atomics:
+ * the same inputs give the same bits. The workspace is aligned to 256 bytes.
+ * ------------------------------------------------------------------------------- */
+GTK_API int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight, int dtype, void* y,
+                                  int64_t n_tokens, int64_t vocab, int64_t D, float scale, uint32_t* status,
+                                  void* stream);
+GTK_API size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D);
+GTK_API int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int index_bits, void* dweight,
+                                   int w_dtype, int64_t n_tokens, int64_t vocab, int64_t D, float scale,
+                                   int64_t padding, void* workspace, size_t workspace_bytes, uint32_t* status,
+                                   void* stream);
 
 /* The reference's `_C.fused_layernorm_linear(x, gamma, beta, weight, bias, eps)`
  * (kernels/bindings.cpp:97-101; layernorm.cu:46-76): out = LayerNorm(x) weight^T + bias in
