@@ -8,16 +8,16 @@
 // and of the rows behind them overlap.
 //
 // Backward: HBM bound too -- it reads dy once and writes the whole of dW once -- if the rows
-// of one token can be found together. So the tokens are sorted first (stable, least digit
-// first, in at most four passes of 8 bits; four bytes of key and four of position per token, small
-// beside dy), and the sorted list is cut into chunks of equal length, whatever the tokens'
-// frequencies: a warp sums the dy rows of its chunk in registers, in list order, and writes a
-// row of dW at each change of token. A token whose run crosses chunks gets its partial sums
-// from a scratch buffer: each chunk writes at most one for the run it continues ("head") and
-// one for the run it starts and does not finish ("tail"); a last kernel adds them in order.
-// Rows of tokens that do not occur are zeroed by further warps from a bitmap of the tokens.
+// of one token can be found together. So the tokens are sorted first (stable, least digit first,
+// up to 8 bits a pass; four bytes of key and four of position per token, small beside dy; one
+// block does it up to 8192 tokens), and the sorted list is cut into chunks of equal length,
+// whatever the tokens' frequencies: a warp sums the dy rows of its chunk in registers, in list
+// order, with the next eight rows in flight, and writes a row of dW at each change of token. Runs
+// that cross chunks are joined in the block, and those that cross blocks from a scratch buffer
+// of at most two rows a block, by a last kernel and in order. Rows of tokens that do not occur are
+// zeroed by further blocks of the same launch, which look them up in the sorted keys.
 // No atomics on floating-point values: the same inputs give the same bits. Sums are fp32 in a
-// chunk and 64-bit between chunks; dW is rounded once.
+// chunk (at most 1024 rows, by eights) and 64-bit between chunks; dW is rounded once.
 #include <vector>
 
 #include "train_common.cuh"
@@ -26,10 +26,12 @@ namespace gtk {
 namespace emb {
 
 constexpr int kSortThreads = 1024;
-constexpr int kSortPer = 8;
-constexpr int kTile = kSortThreads * kSortPer;  // tokens of one sorting block
-constexpr int kBins = 256;
+constexpr int kMaxPer = 8;                        // tokens per thread of a sorting block
+constexpr int kTile = kSortThreads * kMaxPer;     // tokens of one sorting block
+constexpr int kMaxBits = 8;                       // of a digit
+constexpr int kBins = 1 << kMaxBits;
 constexpr int kWarps = kSortThreads / 32;
+constexpr int kSlices = kSortThreads / kBins;     // threads per bin
 constexpr int kMaxWidth = 1 << 20;
 
 // The key of token t: itself, or V (sorted last and then ignored) when it is out of range or padding.
@@ -43,11 +45,9 @@ __device__ __forceinline__ uint32_t key_of(const I* tokens, int64_t t, uint32_t 
   return v == padding ? V : static_cast<uint32_t>(v);
 }
 
-// Peers of this lane with the same digit, among the active lanes.
-__device__ __forceinline__ uint32_t same_digit(uint32_t active, uint32_t d) { return __match_any_sync(active, d); }
-
 struct SortShared {
   uint16_t count[kWarps][kBins];
+  uint32_t part[kSlices][kBins];
   uint32_t base[kBins];
   uint32_t scan[kBins / 32];
 };
@@ -66,133 +66,137 @@ __device__ __forceinline__ uint32_t scan_bins(SortShared& s, uint32_t v) {
   uint32_t before = 0;
   if (threadIdx.x < kBins)
     for (int w = 0; w < warp; ++w) before += s.scan[w];
-  __syncthreads();
   return before + x - v;
 }
 
-// Stable rank of the tile's elements by digit: thread's element i (tile index
-// warp * 32 * kSortPer + i * 32 + lane) has `digit[i]`, kBins where there is no element. After
-// the call s.count[w][b] holds the number of elements of digit b in the warps before w, and
-// rank[i] the element's rank among its warp's elements of that digit; the total of digit
-// threadIdx.x is returned to the first kBins threads.
-__device__ __forceinline__ uint32_t rank_tile(SortShared& s, const uint32_t (&digit)[kSortPer],
-                                              uint32_t (&rank)[kSortPer]) {
+// Stable rank of the tile's elements by a digit of `bits` bits: the thread's element i (index
+// tile_index(i) of the tile) has digit[i], kBins where there is no element. After the call and a
+// barrier, s.count[w][b] holds the number of elements of digit b in the warps before w; rank[i]
+// is the element's rank among its warp's elements of that digit. The total of digit threadIdx.x
+// is returned to the first kBins threads. Equal digits within a warp are found with one ballot
+// per bit (__match_any_sync took 5 us where this takes 1).
+template <int kPer>
+__device__ __forceinline__ uint32_t rank_tile(SortShared& s, const uint32_t (&digit)[kPer], uint32_t (&rank)[kPer],
+                                              int bits) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int b = lane; b < kBins; b += 32) s.count[warp][b] = 0;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < kSortPer; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const uint32_t d = digit[i];
-    const uint32_t peers = same_digit(0xffffffffu, d);
-    const uint32_t before = d < kBins ? s.count[warp][d] : 0;
+    const bool valid = d < kBins;
+    uint32_t peers = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+    for (int b = 0; b < kMaxBits; ++b)
+      if (b < bits) {
+        const bool one = (d >> b) & 1u;
+        const uint32_t ones = __ballot_sync(0xffffffffu, one);
+        peers &= one ? ones : ~ones;
+      }
+    const uint32_t before = valid ? s.count[warp][d] : 0;
     __syncwarp();
     rank[i] = before + __popc(peers & ((1u << lane) - 1u));
-    if (d < kBins && (peers >> lane) == 1u) s.count[warp][d] = static_cast<uint16_t>(rank[i] + 1);
+    if (valid && (peers >> lane) == 1u) s.count[warp][d] = static_cast<uint16_t>(rank[i] + 1);
     __syncwarp();
   }
   __syncthreads();
-  uint32_t total = 0;
-  if (threadIdx.x < kBins)
-    for (int w = 0; w < kWarps; ++w) {
-      const uint32_t n = s.count[w][threadIdx.x];
-      s.count[w][threadIdx.x] = static_cast<uint16_t>(total);
-      total += n;
-    }
+  // exclusive counts over the warps: kSlices threads per bin, each for consecutive warps
+  constexpr int kRun = kWarps / kSlices;
+  const int bin = threadIdx.x & (kBins - 1), slice = threadIdx.x / kBins;
+  uint32_t n[kRun], total = 0;
+#pragma unroll
+  for (int w = 0; w < kRun; ++w) total += n[w] = s.count[slice * kRun + w][bin];
+  s.part[slice][bin] = total;
+  __syncthreads();
+  uint32_t at = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kSlices; ++i) {
+    const uint32_t t = s.part[i][bin];
+    at += i < slice ? t : 0;
+    total += t;
+  }
+#pragma unroll
+  for (int w = 0; w < kRun; ++w) {
+    s.count[slice * kRun + w][bin] = static_cast<uint16_t>(at);
+    at += n[w];
+  }
   return total;
 }
 
+// Consecutive elements belong to a warp, so that ranks by warp keep the order.
+template <int kPer>
 __device__ __forceinline__ int tile_index(int i) {
-  return (threadIdx.x >> 5) * 32 * kSortPer + i * 32 + (threadIdx.x & 31);
+  return (threadIdx.x >> 5) * 32 * kPer + i * 32 + (threadIdx.x & 31);
 }
 
-// Marks `key` in the bitmap of occurring tokens.
-__device__ __forceinline__ void mark(uint32_t* present, uint32_t key) {
-  const uint32_t bit = 1u << (key & 31);
-  if (!(__ldcg(present + (key >> 5)) & bit)) atomicOr(present + (key >> 5), bit);
-}
-
-// All of the sort in one block: T <= kTile. Keys and positions stay in registers between the
-// passes and cross through shared memory.
-template <typename I>
+// All of the sort in one block: T <= 1024 kPer. Keys and positions stay in registers during a
+// pass and cross through shared memory between two.
+template <typename I, int kPer>
 __global__ void __launch_bounds__(kSortThreads)
-    sort_small_kernel(const I* __restrict__ tokens, int T, uint32_t V, int64_t padding, int passes,
-                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* __restrict__ present,
-                      uint32_t* status) {
-  extern __shared__ uint32_t buf[];  // [2][kTile]: keys, positions
+    sort_small_kernel(const I* __restrict__ tokens, int T, uint32_t V, int64_t padding, int passes, int bits,
+                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* status) {
+  extern __shared__ uint32_t buf[];  // [2][1024 kPer]: keys, positions
   __shared__ SortShared s;
   uint32_t* bk = buf;
-  uint32_t* bp = buf + kTile;
-  for (uint32_t w = threadIdx.x; w < (V + 31) / 32; w += kSortThreads) present[w] = 0;
-  __syncthreads();
+  uint32_t* bp = buf + kSortThreads * kPer;
   bool bad = false;
-  uint32_t key[kSortPer], pos[kSortPer];
+  uint32_t key[kPer], pos[kPer];
 #pragma unroll
-  for (int i = 0; i < kSortPer; ++i) {
-    const int t = tile_index(i);
+  for (int i = 0; i < kPer; ++i) {
+    const int t = tile_index<kPer>(i);
     pos[i] = static_cast<uint32_t>(t);
-    key[i] = t < T ? key_of(tokens, t, V, padding, &bad) : 0xffffffffu;
-    if (key[i] < V) mark(present, key[i]);
+    key[i] = t < T ? key_of(tokens, t, V, padding, &bad) : 0u;
   }
   for (int p = 0; p < passes; ++p) {
-    uint32_t digit[kSortPer], rank[kSortPer];
+    uint32_t digit[kPer], rank[kPer];
 #pragma unroll
-    for (int i = 0; i < kSortPer; ++i) digit[i] = tile_index(i) < T ? (key[i] >> (8 * p)) & 255u : kBins;
-    const uint32_t total = rank_tile(s, digit, rank);
+    for (int i = 0; i < kPer; ++i)
+      digit[i] = tile_index<kPer>(i) < T ? (key[i] >> (bits * p)) & ((1u << bits) - 1u) : kBins;
+    const uint32_t total = rank_tile<kPer>(s, digit, rank, bits);
     const uint32_t base = scan_bins(s, threadIdx.x < kBins ? total : 0);
     if (threadIdx.x < kBins) s.base[threadIdx.x] = base;
     __syncthreads();
+    const bool last = p + 1 == passes;
 #pragma unroll
-    for (int i = 0; i < kSortPer; ++i)
+    for (int i = 0; i < kPer; ++i)
       if (digit[i] < kBins) {
         const uint32_t to = s.base[digit[i]] + s.count[threadIdx.x >> 5][digit[i]] + rank[i];
-        bk[to] = key[i];
-        bp[to] = pos[i];
+        (last ? keys_out : bk)[to] = key[i];
+        (last ? pos_out : bp)[to] = pos[i];
       }
+    if (last) break;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSortPer; ++i) {
-      const int t = tile_index(i);
+    for (int i = 0; i < kPer; ++i) {
+      const int t = tile_index<kPer>(i);
       if (t < T) {
         key[i] = bk[t];
         pos[i] = bp[t];
       }
     }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < kSortPer; ++i) {
-    const int t = tile_index(i);
-    if (t < T) {
-      keys_out[t] = key[i];
-      pos_out[t] = pos[i];
-    }
   }
   if (status && bad) atomicOr(status, GTK_STATUS_BAD_TOKEN);
 }
 
-// Pass `p` of the sort over many tiles, first half: the tile's digit counts. The first pass
+// Pass `pass` of the sort over many tiles, first half: the tile's digit counts. The first pass
 // reads the tokens, later ones the keys of the pass before.
 template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
     count_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys, int64_t T, uint32_t V,
-                 int64_t padding, int pass, uint32_t* __restrict__ counts, uint32_t* __restrict__ present,
-                 uint32_t* status) {
+                 int64_t padding, int pass, int bits, uint32_t* __restrict__ counts, uint32_t* status) {
   wait_previous_kernel();
   __shared__ SortShared s;
-  if (pass == 0)
-    for (int64_t w = static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x; w < (V + 31) / 32;
-         w += static_cast<int64_t>(gridDim.x) * kSortThreads)
-      present[w] = 0;
   bool bad = false;
-  uint32_t digit[kSortPer], rank[kSortPer];
+  uint32_t digit[kMaxPer], rank[kMaxPer];
 #pragma unroll
-  for (int i = 0; i < kSortPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index(i);
+  for (int i = 0; i < kMaxPer; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kMaxPer>(i);
     uint32_t k = 0;
     if (t < T) k = pass == 0 ? key_of(tokens, t, V, padding, &bad) : keys[t];
-    digit[i] = t < T ? (k >> (8 * pass)) & 255u : kBins;
+    digit[i] = t < T ? (k >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
   }
-  const uint32_t total = rank_tile(s, digit, rank);
+  const uint32_t total = rank_tile<kMaxPer>(s, digit, rank, bits);
   if (threadIdx.x < kBins) counts[static_cast<int64_t>(blockIdx.x) * kBins + threadIdx.x] = total;
   if (status && bad) atomicOr(status, GTK_STATUS_BAD_TOKEN);
 }
@@ -201,34 +205,33 @@ __global__ void __launch_bounds__(kSortThreads)
 template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
     scatter_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                   int64_t T, uint32_t V, int64_t padding, int pass, const uint32_t* __restrict__ counts, int tiles,
-                   uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* __restrict__ present) {
+                   int64_t T, uint32_t V, int64_t padding, int pass, int bits, const uint32_t* __restrict__ counts,
+                   int tiles, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
   wait_previous_kernel();
   __shared__ SortShared s;
-  __shared__ uint32_t before_part[kSortThreads / kBins][kBins], total_part[kSortThreads / kBins][kBins];
-  uint32_t key[kSortPer], p0[kSortPer], digit[kSortPer], rank[kSortPer];
+  __shared__ uint32_t before_part[kSlices][kBins], total_part[kSlices][kBins];
+  uint32_t key[kMaxPer], p0[kMaxPer], digit[kMaxPer], rank[kMaxPer];
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < kSortPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index(i);
+  for (int i = 0; i < kMaxPer; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kMaxPer>(i);
     key[i] = 0;
     p0[i] = static_cast<uint32_t>(t);
     if (t < T) {
       if (pass == 0) {
         key[i] = key_of(tokens, t, V, padding, &bad);
-        if (key[i] < V) mark(present, key[i]);
       } else {
         key[i] = keys[t];
         p0[i] = pos[t];
       }
     }
-    digit[i] = t < T ? (key[i] >> (8 * pass)) & 255u : kBins;
+    digit[i] = t < T ? (key[i] >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
   }
   // thread = (slice of the tiles, bin)
   const int bin = threadIdx.x & (kBins - 1), slice = threadIdx.x / kBins;
   uint32_t before = 0, total = 0;
 #pragma unroll 8
-  for (int t = slice; t < tiles; t += kSortThreads / kBins) {
+  for (int t = slice; t < tiles; t += kSlices) {
     const uint32_t n = counts[static_cast<int64_t>(t) * kBins + bin];
     total += n;
     before += t < static_cast<int>(blockIdx.x) ? n : 0;
@@ -238,16 +241,16 @@ __global__ void __launch_bounds__(kSortThreads)
   __syncthreads();
   before = total = 0;
   if (threadIdx.x < kBins)
-    for (int i = 0; i < kSortThreads / kBins; ++i) {
+    for (int i = 0; i < kSlices; ++i) {
       before += before_part[i][threadIdx.x];
       total += total_part[i][threadIdx.x];
     }
   const uint32_t base = scan_bins(s, total);
   if (threadIdx.x < kBins) s.base[threadIdx.x] = base + before;
-  rank_tile(s, digit, rank);
+  rank_tile<kMaxPer>(s, digit, rank, bits);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kSortPer; ++i)
+  for (int i = 0; i < kMaxPer; ++i)
     if (digit[i] < kBins) {
       const uint32_t to = s.base[digit[i]] + s.count[threadIdx.x >> 5][digit[i]] + rank[i];
       keys_out[to] = key[i];
@@ -258,7 +261,8 @@ __global__ void __launch_bounds__(kSortThreads)
 // ---- Sums over the runs of equal tokens -----------------------------------------------------
 
 constexpr int kSumThreads = 256;
-constexpr int kBatch = 8;  // dy rows in flight per warp
+constexpr int kSumWarps = kSumThreads / 32;
+constexpr int kBatch = 8;  // dy rows that a warp loads at once
 
 template <typename W, int V>
 __device__ __forceinline__ void write_row(W* dst, const float (&acc)[V], float scale) {
@@ -268,125 +272,224 @@ __device__ __forceinline__ void write_row(W* dst, const float (&acc)[V], float s
   st_vec<W, V>(dst, o);
 }
 
-// Chunk c covers the sorted entries [c L, (c + 1) L); a slab is 32 V columns. Warps
-// [0, chunks * slabs) sum, the blocks after them zero the rows of absent tokens, 32 rows and one
-// slab per warp.
+// How a warp's chunk meets its neighbours. kHead: its first run began before it; kHeadOn: and
+// that run goes on behind it (the chunk is one run). kTail: its last run begins in it and goes on.
+constexpr uint32_t kHead = 1, kHeadOn = 2, kTail = 4;
+
+// Warp c sums the sorted entries [c L, (c + 1) L) over a slab of 32 V columns; a block is one slab
+// of eight consecutive chunks (a unit), joined in shared memory, so that at most two partial
+// rows a unit go to memory: partial[2 u] for the run that began before it, partial[2 u + 1]
+// for the one that begins in it and goes on.
 template <typename T, typename W, int V>
-__global__ void __launch_bounds__(kSumThreads)
-    run_sums_kernel(const T* __restrict__ dy, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                    const uint32_t* __restrict__ present, W* __restrict__ dw, float* __restrict__ partial, int64_t n,
-                    uint32_t vocab, int D, int L, int64_t chunks, int slabs, int64_t sum_blocks, float scale) {
-  wait_previous_kernel();
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kSumThreads + threadIdx.x) >> 5;
-  if (blockIdx.x >= sum_blocks) {
-    const int64_t item = warp - sum_blocks * (kSumThreads / 32);
-    const int64_t word = item / slabs;
-    const int col = (static_cast<int>(item % slabs) * 32 + lane) * V;
-    if (word >= (static_cast<int64_t>(vocab) + 31) / 32 || col >= D) return;
-    const uint32_t bits = present[word];
-    const float zero[V] = {};
-    for (int r = 0; r < 32; ++r) {
-      const int64_t row = word * 32 + r;
-      if (row < vocab && !(bits >> r & 1u)) write_row<W, V>(dw + row * D + col, zero, 0.f);
-    }
-    return;
-  }
-  if (warp >= chunks * slabs) return;
-  const int64_t c = warp / slabs;
-  const int col = (static_cast<int>(warp % slabs) * 32 + lane) * V;
+__device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_t* __restrict__ keys,
+                                         const uint32_t* __restrict__ pos, W* __restrict__ dw,
+                                         float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
+                                         int64_t unit, int slab, float scale, float (*edge)[2][32 * V],
+                                         uint32_t* how, uint32_t* run_key) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t i0 = (unit * kSumWarps + warp) * L;
+  const int col = (slab * 32 + lane) * V;
   const bool mine = col < D;
-  const int64_t i0 = c * L, i1 = i0 + L < n ? i0 + L : n;
-  const uint32_t left = i0 > 0 ? keys[i0 - 1] : 0xffffffffu;
-  const uint32_t right = i1 < n ? keys[i1] : 0xffffffffu;
-  float acc[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  uint32_t cur = keys[i0];
-  bool continued = cur == left;  // the current run began in an earlier chunk
-  float* head = partial + (c * 2) * static_cast<int64_t>(D) + col;
-  for (int64_t b = i0; b < i1; b += 32) {
-    const int64_t e = b + lane;
-    const uint32_t my_key = e < i1 ? keys[e] : 0xffffffffu;
-    const uint32_t my_pos = e < i1 ? pos[e] : 0u;
-    const int m = static_cast<int>(i1 - b < 32 ? i1 - b : 32);
-    for (int q = 0; q < m; q += kBatch) {
-      Vec<T, V> row[kBatch];
+  if (lane == 0) how[warp] = 0;
+  if (i0 < n) {
+    const int64_t i1 = i0 + L < n ? i0 + L : n;
+    const int m = static_cast<int>(i1 - i0);
+    const uint32_t left = i0 > 0 ? keys[i0 - 1] : 0xffffffffu;
+    const uint32_t right = i1 < n ? keys[i1] : 0xffffffffu;
+    // the keys and positions of 32 entries, one per lane, and those of the next 32
+    uint32_t k_now = lane < m ? keys[i0 + lane] : 0xffffffffu;
+    uint32_t p_now = lane < m ? pos[i0 + lane] : 0u;
+    Vec<T, V> row[2][kBatch];
+    auto load = [&](Vec<T, V>(&to)[kBatch], uint32_t k32, uint32_t p32, int q) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const uint32_t k = __shfl_sync(0xffffffffu, my_key, q + u);
-        const uint32_t p = __shfl_sync(0xffffffffu, my_pos, q + u);
-        if (mine && k < vocab) row[u] = ld_vec<T, V>(dy + static_cast<int64_t>(p) * D + col);
+        const uint32_t k = __shfl_sync(0xffffffffu, k32, q + u);
+        const uint32_t p = __shfl_sync(0xffffffffu, p32, q + u);
+        if (mine && k < vocab) to[u] = ld_vec<T, V>(dy + static_cast<int64_t>(p) * D + col);
       }
+    };
+    load(row[0], k_now, p_now, 0);
+    float acc[V];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (q + u >= m) break;
-        const uint32_t k = __shfl_sync(0xffffffffu, my_key, q + u);
-        if (k >= vocab) continue;  // sorted last: nothing follows but more of them
-        if (k != cur) {
-          if (mine) {
-            if (continued)
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    uint32_t cur = __shfl_sync(0xffffffffu, k_now, 0);
+    bool continued = cur == left;  // the current run began in an earlier chunk
+    uint32_t flags = continued && cur < vocab ? kHead : 0u;
+    if (lane == 0) run_key[warp] = cur;
+    for (int b = 0; b < m; b += 32) {
+      const int e = b + 32 + lane;
+      const uint32_t k_next = e < m ? keys[i0 + e] : 0xffffffffu;
+      const uint32_t p_next = e < m ? pos[i0 + e] : 0u;
 #pragma unroll
-              for (int j = 0; j < V; ++j) head[j] = acc[j];
-            else
-              write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
-          }
-          cur = k;
-          continued = false;
+      for (int q = 0; q < 32; q += kBatch) {
+        if (b + q >= m) break;
+        Vec<T, V>(&now)[kBatch] = row[(q / kBatch) & 1];
+        // the next batch is on its way while this one is added up
+        if (q + kBatch < 32)
+          load(row[(q / kBatch + 1) & 1], k_now, p_now, q + kBatch);
+        else
+          load(row[(q / kBatch + 1) & 1], k_next, p_next, 0);
+        const uint32_t k0 = __shfl_sync(0xffffffffu, k_now, q);
+        const uint32_t k7 = __shfl_sync(0xffffffffu, k_now, q + kBatch - 1);
+        if (k0 == cur && k7 == cur && cur < vocab) {  // eight rows of the current run: a tree
+          if (mine)
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = 0.f;
+            for (int j = 0; j < V; ++j) {
+              float t[kBatch];
+#pragma unroll
+              for (int u = 0; u < kBatch; ++u) t[u] = Elem<T>::load(now[u].v[j]);
+              acc[j] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+            }
+          continue;
         }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const uint32_t k = __shfl_sync(0xffffffffu, k_now, q + u);
+          if (k >= vocab) continue;  // none, or sorted last: nothing follows but more of them
+          if (k != cur) {
+            if (mine) {
+              if (continued)
+#pragma unroll
+                for (int j = 0; j < V; ++j) edge[warp][0][lane * V + j] = acc[j];
+              else
+                write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
+            }
+            cur = k;
+            continued = false;
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = 0.f;
+          }
+          if (mine)
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += Elem<T>::load(now[u].v[j]);
+        }
+      }
+      k_now = k_next;
+      p_now = p_next;
+    }
+    if (cur < vocab) {
+      const bool goes_on = cur == right;
+      if (!goes_on && !continued) {
+        if (mine) write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
+      } else {
+        flags |= continued ? (goes_on ? kHeadOn : 0u) : kTail;
         if (mine)
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] += Elem<T>::load(row[u].v[j]);
+          for (int j = 0; j < V; ++j) edge[warp][continued ? 0 : 1][lane * V + j] = acc[j];
       }
     }
+    if (lane == 0) how[warp] = flags;
   }
-  if (!mine || cur >= vocab) return;
-  const bool goes_on = cur == right;
-  if (!goes_on && !continued) {
-    write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
-    return;
+  __syncthreads();
+  // the unit's chunks in order, one column per thread
+  for (int x = threadIdx.x; x < 32 * V; x += kSumThreads) {
+    const int c = slab * 32 * V + x;
+    if (c >= D) continue;
+    double acc = 0.0;
+    bool carrying = false, began_here = false;
+    for (int w = 0; w < kSumWarps; ++w) {
+      const uint32_t f = how[w];
+      if (f & kHead) {
+        acc += static_cast<double>(edge[w][0][x]);
+        carrying = true;
+        if (!(f & kHeadOn)) {
+          if (began_here)
+            dw[static_cast<int64_t>(run_key[w]) * D + c] = Elem<W>::store(static_cast<float>(acc * scale));
+          else
+            partial[unit * 2 * D + c] = static_cast<float>(acc);
+          acc = 0.0;
+          carrying = began_here = false;
+        }
+      }
+      if (f & kTail) {
+        acc = static_cast<double>(edge[w][1][x]);
+        carrying = began_here = true;
+      }
+    }
+    if (carrying) partial[(unit * 2 + (began_here ? 1 : 0)) * D + c] = static_cast<float>(acc);
   }
-  float* to = continued ? head : head + D;
-#pragma unroll
-  for (int j = 0; j < V; ++j) to[j] = acc[j];
 }
 
-// The runs that cross chunks: the block of the chunk in which one begins adds its tail and the
-// heads of the chunks after it.
-constexpr int kJoinThreads = 512;
-constexpr int kJoinCols = 32;
+// Blocks [0, units * slabs) sum; those behind them zero the rows of the tokens that do not occur:
+// 32 rows and zero_cols columns per warp, a binary search of the sorted keys for each row.
+template <typename T, typename W, int V>
+__global__ void __launch_bounds__(kSumThreads, 2)
+    run_sums_kernel(const T* __restrict__ dy, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+                    W* __restrict__ dw, float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
+                    int slabs, int64_t sum_blocks, int zero_cols, int zero_slabs, float scale) {
+  wait_previous_kernel();
+  __shared__ float edge[kSumWarps][2][32 * V];
+  __shared__ uint32_t how[kSumWarps], run_key[kSumWarps];
+  if (blockIdx.x < sum_blocks) {
+    const int64_t unit = blockIdx.x / static_cast<uint32_t>(slabs);
+    sum_unit<T, W, V>(dy, keys, pos, dw, partial, n, vocab, D, L, unit, static_cast<int>(blockIdx.x - unit * slabs),
+                      scale, edge, how, run_key);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (blockIdx.x - sum_blocks) * kSumWarps + (threadIdx.x >> 5);
+  const int64_t row0 = item / zero_slabs * 32;
+  if (row0 >= vocab) return;
+  const uint32_t v = static_cast<uint32_t>(row0) + lane;
+  int64_t lo = 0, hi = n;  // the first entry with keys >= v
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  uint32_t absent = __ballot_sync(0xffffffffu, v < vocab && !(lo < n && keys[lo] == v));
+  const int c0 = static_cast<int>(item % zero_slabs) * zero_cols;
+  const int c1 = c0 + zero_cols < D ? c0 + zero_cols : D;
+  const float zero[V] = {};
+  for (; absent; absent &= absent - 1) {
+    W* row = dw + (row0 + __ffs(absent) - 1) * D;
+    for (int c = c0 + lane * V; c < c1; c += 32 * V) write_row<W, V>(row + c, zero, 0.f);
+  }
+}
+
+// The runs that cross units: the block of the unit in which one begins adds its tail and the heads
+// of the units after it, 128 columns at a time.
+constexpr int kJoinCols = 128;
 
 template <typename W>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kSumThreads)
     join_runs_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, W* __restrict__ dw,
-                     int64_t n, uint32_t vocab, int D, int L, int64_t chunks, float scale) {
+                     int64_t n, uint32_t vocab, int D, int64_t unit_len, int slabs, float scale) {
   wait_previous_kernel();
-  __shared__ double part[kJoinThreads / 32][kJoinCols];
-  const int64_t c = blockIdx.x;
-  const int64_t i0 = c * L, i1 = i0 + L;
-  if (i1 >= n) return;  // the last chunk starts no run that goes on
+  __shared__ double part[kSumWarps][kJoinCols];
+  const int64_t u = blockIdx.x / static_cast<uint32_t>(slabs);
+  const int col0 = static_cast<int>(blockIdx.x - u * slabs) * kJoinCols;
+  const int64_t i0 = u * unit_len, i1 = i0 + unit_len;
+  if (i1 >= n) return;  // the last unit starts no run that goes on
   const uint32_t k = keys[i1 - 1];
   if (k >= vocab || keys[i1] != k) return;
   if (i0 > 0 && keys[i0] == k && keys[i0 - 1] == k) return;  // it began earlier
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int c0 = 0; c0 < D; c0 += kJoinCols) {
-    const int col = c0 + lane;
-    double s = 0.0;
-    if (col < D) {
-      if (warp == 0) s = partial[(c * 2 + 1) * static_cast<int64_t>(D) + col];
-      for (int64_t j = c + 1 + warp; j < chunks && keys[j * L] == k; j += kJoinThreads / 32)
-        s += partial[(j * 2) * static_cast<int64_t>(D) + col];
-    }
-    part[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0 && col < D) {
-      for (int w = 1; w < kJoinThreads / 32; ++w) s += part[w][lane];
-      dw[static_cast<int64_t>(k) * D + col] = Elem<W>::store(static_cast<float>(s * scale));
-    }
-    __syncthreads();
+  // the units behind it whose first entry belongs to the run
+  int64_t heads = 0;
+  for (int count = kSumThreads; count == kSumThreads; heads += count) {
+    const int64_t j = (u + 1 + heads + threadIdx.x) * unit_len;
+    count = __syncthreads_count(j < n && keys[j] == k);
   }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double s[kJoinCols / 32] = {};
+#pragma unroll 4
+  for (int64_t j = warp; j <= heads; j += kSumWarps) {  // 0: the tail, then the heads
+    const float* p = partial + (j == 0 ? u * 2 + 1 : (u + j) * 2) * D + col0 + lane;
+#pragma unroll
+    for (int i = 0; i < kJoinCols / 32; ++i)
+      if (col0 + lane + 32 * i < D) s[i] += static_cast<double>(p[32 * i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinCols / 32; ++i) part[warp][lane + 32 * i] = s[i];
+  __syncthreads();
+  const int c = col0 + threadIdx.x;
+  if (threadIdx.x >= kJoinCols || c >= D) return;
+  double t = part[0][threadIdx.x];
+#pragma unroll
+  for (int w = 1; w < kSumWarps; ++w) t += part[w][threadIdx.x];
+  dw[static_cast<int64_t>(k) * D + c] = Elem<W>::store(static_cast<float>(t * scale));
 }
 
 // ---- Forward ----------------------------------------------------------------------------------
@@ -448,35 +551,38 @@ int vec_width(int64_t D, size_t bytes, bool aligned) {
 
 // The backward's plan: what the workspace holds and how the sorted list is cut.
 struct Plan {
-  int passes;        // of 8 bits, for keys 0 .. vocab
+  int passes, bits;  // of the sort, for keys 0 .. vocab
   int64_t tiles;
-  int64_t L, chunks;
-  size_t keys, pos, counts, present, partial, total;  // byte offsets (keys, pos: two buffers each)
+  int64_t L, units;                            // entries of a warp's chunk; units of kSumWarps chunks
+  size_t keys, pos, counts, partial, total;    // byte offsets (keys, pos: two buffers each)
 };
 
-Plan plan_for(int64_t T, int64_t vocab, int64_t D) {
+Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype) {
   Plan p = {};
-  p.passes = 1;
-  while (p.passes < 4 && (vocab >> (8 * p.passes)) != 0) ++p.passes;
+  int bits = 1;
+  while (vocab >> bits) ++bits;
+  p.passes = (bits + kMaxBits - 1) / kMaxBits;
+  p.bits = (bits + p.passes - 1) / p.passes;
   p.tiles = (T + kTile - 1) / kTile;
-  // long enough that about 16 warps per SM have a chunk (of the narrowest slab, 32 columns: the
-  // workspace covers every type), at least 32 entries
-  const int64_t slabs = (D + 127) / 128;
-  int64_t L = (T * slabs + 148 * 16 - 1) / (148 * 16);
-  L = (L + 31) / 32 * 32;
-  p.L = L < 32 ? 32 : (L > 1024 ? 1024 : L);
-  p.chunks = (T + p.L - 1) / p.L;
+  // About 16 warps per SM get a chunk, of whole batches. Up to 512 tokens make one unit: the
+  // launch that joins units costs more than the longer chunks.
+  const int64_t slab = 32 * 16 / static_cast<int64_t>(dtype_bytes(dy_dtype));
+  const int64_t slabs = (D + slab - 1) / slab;
+  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 16 - 1) / (148 * 16);
+  L = (L + kBatch - 1) / kBatch * kBatch;
+  p.L = L > 1024 ? 1024 : L;
+  p.units = (T + p.L * kSumWarps - 1) / (p.L * kSumWarps);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
     at += round_up(bytes, 256);
     return o;
   };
-  p.keys = take(2 * round_up(4 * T, 256));
-  p.pos = take(2 * round_up(4 * T, 256));
+  const bool two = p.tiles > 1 && p.passes > 1;
+  p.keys = take((two ? 2 : 1) * round_up(4 * T, 256));
+  p.pos = take((two ? 2 : 1) * round_up(4 * T, 256));
   p.counts = take(p.tiles > 1 ? 4 * kBins * p.tiles : 0);
-  p.present = take((vocab + 31) / 32 * 4);
-  p.partial = take(p.chunks > 1 ? static_cast<size_t>(p.chunks) * 2 * D * sizeof(float) : 0);
+  p.partial = take(p.units > 1 ? static_cast<size_t>(p.units) * 2 * D * sizeof(float) : 0);
   p.total = at;
   return p;
 }
@@ -491,32 +597,42 @@ struct Args {
   cudaStream_t st;
 };
 
+template <typename I, int kPer>
+int sort_small(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
+  const int smem = p.passes > 1 ? 2 * kSortThreads * kPer * 4 : 0;
+  auto kernel = sort_small_kernel<I, kPer>;
+  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), 2 * kSortThreads * kPer * 4)) return e;
+  return launch("embedding token sort", kernel, 1, kSortThreads, smem, a.st, false, static_cast<const I*>(a.tokens),
+                static_cast<int>(a.T), static_cast<uint32_t>(a.vocab), a.padding, p.passes, p.bits, keys, pos,
+                a.status);
+}
+
 template <typename I>
 int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** pos) {
   const size_t half = round_up(4 * a.T, 256);
   uint32_t* k[2] = {reinterpret_cast<uint32_t*>(a.ws + p.keys), reinterpret_cast<uint32_t*>(a.ws + p.keys + half)};
   uint32_t* q[2] = {reinterpret_cast<uint32_t*>(a.ws + p.pos), reinterpret_cast<uint32_t*>(a.ws + p.pos + half)};
-  uint32_t* present = reinterpret_cast<uint32_t*>(a.ws + p.present);
   const I* tokens = static_cast<const I*>(a.tokens);
   const uint32_t V = static_cast<uint32_t>(a.vocab);
   if (p.tiles == 1) {
-    const int smem = 2 * kTile * 4;
-    if (int e = ensure_smem(reinterpret_cast<const void*>(sort_small_kernel<I>), smem)) return e;
     *keys = k[0];
     *pos = q[0];
-    return launch("embedding token sort", sort_small_kernel<I>, 1, kSortThreads, smem, a.st, false, tokens,
-                  static_cast<int>(a.T), V, a.padding, p.passes, k[0], q[0], present, a.status);
+    // one token per thread as far as that goes: the ranks of a thread's tokens are one after another
+    if (a.T <= kSortThreads) return sort_small<I, 1>(a, p, k[0], q[0]);
+    if (a.T <= 2 * kSortThreads) return sort_small<I, 2>(a, p, k[0], q[0]);
+    if (a.T <= 4 * kSortThreads) return sort_small<I, 4>(a, p, k[0], q[0]);
+    return sort_small<I, kMaxPer>(a, p, k[0], q[0]);
   }
   uint32_t* counts = reinterpret_cast<uint32_t*>(a.ws + p.counts);
   const uint32_t *ki = nullptr, *qi = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {
     uint32_t *ko = k[pass & 1], *qo = q[pass & 1];
     if (int e = launch("embedding token count", count_kernel<I>, p.tiles, kSortThreads, 0, a.st, pass > 0, tokens, ki,
-                       a.T, V, a.padding, pass, counts, present, a.status))
+                       a.T, V, a.padding, pass, p.bits, counts, a.status))
       return e;
     if (int e = launch("embedding token scatter", scatter_kernel<I>, p.tiles, kSortThreads, 0, a.st, true, tokens, ki,
-                       qi, a.T, V, a.padding, pass, static_cast<const uint32_t*>(counts), static_cast<int>(p.tiles),
-                       ko, qo, present))
+                       qi, a.T, V, a.padding, pass, p.bits, static_cast<const uint32_t*>(counts),
+                       static_cast<int>(p.tiles), ko, qo))
       return e;
     ki = ko;
     qi = qo;
@@ -529,22 +645,23 @@ int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** p
 template <typename T, typename W, int V>
 int sums(const Args& a, const Plan& p, const uint32_t* keys, const uint32_t* pos) {
   const int slabs = static_cast<int>((a.D + 32 * V - 1) / (32 * V));
-  constexpr int kPerBlock = kSumThreads / 32;
-  const int64_t sum_blocks = (p.chunks * slabs + kPerBlock - 1) / kPerBlock;
-  const int64_t zero_blocks = ((a.vocab + 31) / 32 * slabs + kPerBlock - 1) / kPerBlock;
-  if (sum_blocks + zero_blocks > (int64_t(1) << 31) - 1)
-    return fail(GTK_ERR_UNSUPPORTED, "embedding: vocabulary times width is too large");
+  const int64_t sum_blocks = p.units * slabs;
+  const int zero_cols = 8 * 32 * V;
+  const int zero_slabs = static_cast<int>((a.D + zero_cols - 1) / zero_cols);
+  const int64_t zero_blocks = ((a.vocab + 31) / 32 * zero_slabs + kSumWarps - 1) / kSumWarps;
+  const int join_slabs = static_cast<int>((a.D + kJoinCols - 1) / kJoinCols);
+  if (sum_blocks + zero_blocks > (int64_t(1) << 31) - 1 || p.units * join_slabs > (int64_t(1) << 31) - 1)
+    return fail(GTK_ERR_UNSUPPORTED, "embedding: tokens or vocabulary times width too large");
   float* partial = reinterpret_cast<float*>(a.ws + p.partial);
   const uint32_t V32 = static_cast<uint32_t>(a.vocab);
   if (int e = launch("embedding run sums", run_sums_kernel<T, W, V>, sum_blocks + zero_blocks, kSumThreads, 0, a.st,
-                     true, static_cast<const T*>(a.dy), keys, pos,
-                     reinterpret_cast<const uint32_t*>(a.ws + p.present), static_cast<W*>(a.dw), partial, a.T, V32,
-                     static_cast<int>(a.D), static_cast<int>(p.L), p.chunks, slabs, sum_blocks, a.scale))
+                     true, static_cast<const T*>(a.dy), keys, pos, static_cast<W*>(a.dw), partial, a.T, V32,
+                     static_cast<int>(a.D), static_cast<int>(p.L), slabs, sum_blocks, zero_cols, zero_slabs, a.scale))
     return e;
-  if (p.chunks == 1) return GTK_OK;
-  return launch("embedding run join", join_runs_kernel<W>, p.chunks, kJoinThreads, 0, a.st, true, keys,
-                static_cast<const float*>(partial), static_cast<W*>(a.dw), a.T, V32, static_cast<int>(a.D),
-                static_cast<int>(p.L), p.chunks, a.scale);
+  if (p.units == 1) return GTK_OK;
+  return launch("embedding run join", join_runs_kernel<W>, (p.units - 1) * join_slabs, kSumThreads, 0, a.st, true,
+                keys, static_cast<const float*>(partial), static_cast<W*>(a.dw), a.T, V32, static_cast<int>(a.D),
+                p.L * kSumWarps, join_slabs, a.scale);
 }
 
 template <typename T, typename W>
@@ -602,9 +719,9 @@ int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight
                           : emb::forward_by_type<int32_t>(a, weight, y, dtype);
 }
 
-size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D) {
-  if (!dims_ok(n_tokens) || !dims_ok(vocab) || !dims_ok(D, emb::kMaxWidth)) return 0;
-  return emb::plan_for(n_tokens, vocab, D).total;
+size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D, int dy_dtype) {
+  if (!dims_ok(n_tokens) || !dims_ok(vocab) || !dims_ok(D, emb::kMaxWidth) || !dtype_ok(dy_dtype)) return 0;
+  return emb::plan_for(n_tokens, vocab, D, dy_dtype).total;
 }
 
 int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int index_bits, void* dweight,
@@ -614,7 +731,7 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
   if (!dtype_ok(dy_dtype) || !(w_dtype == dy_dtype || w_dtype == GTK_F32))
     return fail(GTK_ERR_UNSUPPORTED, "embedding: dy is fp32, bf16 or fp16, the table's gradient fp32 or dy's type");
   if (padding >= vocab) return fail(GTK_ERR_INVALID_ARG, "embedding: the padding token must be below the vocabulary");
-  const emb::Plan p = emb::plan_for(n_tokens, vocab, D);
+  const emb::Plan p = emb::plan_for(n_tokens, vocab, D, dy_dtype);
   if (workspace_bytes < p.total) return fail(GTK_ERR_WORKSPACE, "embedding: workspace too small");
   if (int e = emb::check_tokens(tokens, index_bits)) return e;
   if (int e = check_ptr(dy, "dy", dtype_bytes(dy_dtype))) return e;

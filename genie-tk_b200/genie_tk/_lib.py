@@ -137,7 +137,7 @@ _SIGNATURES = {
                                    c_vp]),
     "gtk_embedding_forward": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, ctypes.c_float, c_vp,
                                       c_vp]),
-    "gtk_embedding_backward_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "gtk_embedding_backward_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int]),
     "gtk_embedding_backward": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, ctypes.c_float,
                                        c_i64, c_vp, c_size, c_vp, c_vp]),
     "gtk_attn_core_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, ctypes.c_float,

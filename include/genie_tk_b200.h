@@ -540,7 +540,7 @@ GTK_API int gtk_clip_grad_norm(const void* const* grads, void* const* outs, cons
 GTK_API int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight, int dtype, void* y,
                                   int64_t n_tokens, int64_t vocab, int64_t D, float scale, uint32_t* status,
                                   void* stream);
-GTK_API size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D);
+GTK_API size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D, int dy_dtype);
 GTK_API int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int index_bits, void* dweight,
                                    int w_dtype, int64_t n_tokens, int64_t vocab, int64_t D, float scale,
                                    int64_t padding, void* workspace, size_t workspace_bytes, uint32_t* status,

@@ -97,8 +97,9 @@ def test_gradient_norm_entry_points(lib):
 def test_embedding_entry_points(lib):
     p, q = P(1 << 20), P((1 << 20) + 2)
     size = lib.gtk_embedding_backward_workspace_bytes
-    assert size(1, 10, 8) > 0 and size(0, 10, 8) == 0 and size(5, 0, 8) == 0 and size(5, 5, (1 << 20) + 1) == 0
-    assert size(1000, 10, 8) % 256 == 0 and size(20000, 32000, 128) > size(5000, 32000, 128) > 16 * 5000
+    assert size(1, 10, 8, 0) > 0 and size(0, 10, 8, 0) == 0 and size(5, 0, 8, 0) == 0
+    assert size(5, 5, (1 << 20) + 1, 0) == 0 and size(5, 5, 5, 3) == 0
+    assert size(1000, 10, 8, 1) % 256 == 0 and size(20000, 32000, 128, 0) > size(5000, 32000, 128, 0) > 8 * 5000
 
     def fwd(tok=p, bits=64, w=p, dt=0, y=p, n=4, v=10, d=8):
         return lib.gtk_embedding_forward(tok, bits, w, dt, y, n, v, d, 1.0, None, None)
