@@ -10,15 +10,15 @@
 // Backward: HBM bound too -- it reads dy once and writes the whole of dW once -- if the rows
 // of one token can be found together. So the tokens are sorted first (stable, least digit first,
 // up to 8 bits a pass; four bytes of key and four of position per token, small beside dy; one
-// block does it up to 8192 tokens), and the sorted list is cut into chunks of equal length,
+// cluster of blocks does it up to 32,768 tokens), and the sorted list is cut into chunks of equal length,
 // whatever the tokens' frequencies: a warp sums the dy rows of its chunk in registers, in list
-// order, with the next eight rows in flight, and writes a row of dW at each change of token. Runs
+// order, with the next twelve rows in flight, and writes a row of dW at each change of token. Runs
 // that cross chunks are joined in the block, and those that cross blocks from a scratch buffer
 // of at most two rows a block, by a last kernel and in order. Rows of tokens that do not occur are
 // zeroed by further blocks of the same launch, which look them up in the sorted keys.
 // No atomics on floating-point values: the same inputs give the same bits. Sums are fp32 in a
-// chunk (at most 1024 rows, by eights) and 64-bit between chunks; dW is rounded once.
-#include <vector>
+// chunk (at most 1024 rows, by fours) and 64-bit between chunks; dW is rounded once.
+#include <cooperative_groups.h>
 
 #include "train_common.cuh"
 
@@ -26,18 +26,19 @@ namespace gtk {
 namespace emb {
 
 constexpr int kSortThreads = 1024;
-constexpr int kMaxPer = 8;                        // tokens per thread of a sorting block
-constexpr int kTile = kSortThreads * kMaxPer;     // tokens of one sorting block
+constexpr int kMaxCluster = 8;                    // sorting blocks that exchange through their shared memory
+constexpr int kClusterPer = 4;                    // most tokens per thread of such a block
+constexpr int64_t kClusterTokens = static_cast<int64_t>(kSortThreads) * kClusterPer * kMaxCluster;
+constexpr int kPer = 8;                           // tokens per thread of the sort over many tiles
+constexpr int kTile = kSortThreads * kPer;
 constexpr int kMaxBits = 8;                       // of a digit
 constexpr int kBins = 1 << kMaxBits;
 constexpr int kWarps = kSortThreads / 32;
 constexpr int kSlices = kSortThreads / kBins;     // threads per bin
 constexpr int kMaxWidth = 1 << 20;
 
-// The key of token t: itself, or V (sorted last and then ignored) when it is out of range or padding.
-template <typename I>
-__device__ __forceinline__ uint32_t key_of(const I* tokens, int64_t t, uint32_t V, int64_t padding, bool* bad) {
-  const int64_t v = static_cast<int64_t>(tokens[t]);
+// The key of token v: itself, or V (sorted last and then ignored) when it is out of range or padding.
+__device__ __forceinline__ uint32_t key_of(int64_t v, uint32_t V, int64_t padding, bool* bad) {
   if (v < 0 || v >= static_cast<int64_t>(V)) {
     *bad = true;
     return V;
@@ -75,14 +76,14 @@ __device__ __forceinline__ uint32_t scan_bins(SortShared& s, uint32_t v) {
 // is the element's rank among its warp's elements of that digit. The total of digit threadIdx.x
 // is returned to the first kBins threads. Equal digits within a warp are found with one ballot
 // per bit (__match_any_sync took 5 us where this takes 1).
-template <int kPer>
-__device__ __forceinline__ uint32_t rank_tile(SortShared& s, const uint32_t (&digit)[kPer], uint32_t (&rank)[kPer],
+template <int N>
+__device__ __forceinline__ uint32_t rank_tile(SortShared& s, const uint32_t (&digit)[N], uint32_t (&rank)[N],
                                               int bits) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int b = lane; b < kBins; b += 32) s.count[warp][b] = 0;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < N; ++i) {
     const uint32_t d = digit[i];
     const bool valid = d < kBins;
     uint32_t peers = __ballot_sync(0xffffffffu, valid);
@@ -125,79 +126,128 @@ __device__ __forceinline__ uint32_t rank_tile(SortShared& s, const uint32_t (&di
 }
 
 // Consecutive elements belong to a warp, so that ranks by warp keep the order.
-template <int kPer>
+template <int N>
 __device__ __forceinline__ int tile_index(int i) {
-  return (threadIdx.x >> 5) * 32 * kPer + i * 32 + (threadIdx.x & 31);
+  return (threadIdx.x >> 5) * 32 * N + i * 32 + (threadIdx.x & 31);
 }
 
-// All of the sort in one block: T <= 1024 kPer. Keys and positions stay in registers during a
-// pass and cross through shared memory between two.
-template <typename I, int kPer>
+// The whole sort in one launch of one cluster: up to eight blocks of 1024 N tokens each, which
+// read one another's digit counts and send every token to the block of its next place
+// through distributed shared memory. Four launches over tiles took 14 us for 8192 tokens where
+// this takes 7.
+// Further clusters, where `zero` is given, zero `zero_bytes` there meanwhile (16-byte multiples).
+template <typename I, int N>
 __global__ void __launch_bounds__(kSortThreads)
-    sort_small_kernel(const I* __restrict__ tokens, int T, uint32_t V, int64_t padding, int passes, int bits,
-                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* status) {
-  extern __shared__ uint32_t buf[];  // [2][1024 kPer]: keys, positions
+    sort_cluster_kernel(const I* __restrict__ tokens, int T, uint32_t V, int64_t padding, int passes, int bits,
+                        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint4* __restrict__ zero,
+                        int64_t zero_bytes, uint32_t* status) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (blockIdx.x >= cluster.num_blocks()) {
+    const int64_t step = static_cast<int64_t>(gridDim.x - cluster.num_blocks()) * kSortThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - cluster.num_blocks()) * kSortThreads + threadIdx.x;
+         i < zero_bytes / 16; i += step)
+      zero[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  extern __shared__ uint32_t buf[];  // [2][1024 N]: keys, positions
   __shared__ SortShared s;
-  uint32_t* bk = buf;
-  uint32_t* bp = buf + kSortThreads * kPer;
+  __shared__ uint32_t totals[kBins];
+  constexpr int kHere = kSortThreads * N;
+  const int blocks = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
   bool bad = false;
-  uint32_t key[kPer], pos[kPer];
+  uint32_t key[N], pos[N];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int t = tile_index<kPer>(i);
+  for (int i = 0; i < N; ++i) {
+    const int t = me * kHere + tile_index<N>(i);
     pos[i] = static_cast<uint32_t>(t);
-    key[i] = t < T ? key_of(tokens, t, V, padding, &bad) : 0u;
+    key[i] = t < T ? key_of(static_cast<int64_t>(tokens[t]), V, padding, &bad) : 0u;
   }
   for (int p = 0; p < passes; ++p) {
-    uint32_t digit[kPer], rank[kPer];
+    uint32_t digit[N], rank[N];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      digit[i] = tile_index<kPer>(i) < T ? (key[i] >> (bits * p)) & ((1u << bits) - 1u) : kBins;
-    const uint32_t total = rank_tile<kPer>(s, digit, rank, bits);
-    const uint32_t base = scan_bins(s, threadIdx.x < kBins ? total : 0);
-    if (threadIdx.x < kBins) s.base[threadIdx.x] = base;
+    for (int i = 0; i < N; ++i)
+      digit[i] = me * kHere + tile_index<N>(i) < T ? (key[i] >> (bits * p)) & ((1u << bits) - 1u) : kBins;
+    const uint32_t total = rank_tile<N>(s, digit, rank, bits);
+    if (threadIdx.x < kBins) totals[threadIdx.x] = total;
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < kBins) {
+      uint32_t n[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) n[r] = r < blocks ? cluster.map_shared_rank(totals, r)[threadIdx.x] : 0u;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        before += r < me ? n[r] : 0;
+        all += n[r];
+      }
+    }
+    const uint32_t base = scan_bins(s, all);
+    if (threadIdx.x < kBins) s.base[threadIdx.x] = base + before;
     __syncthreads();
-    const bool last = p + 1 == passes;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < N; ++i)
       if (digit[i] < kBins) {
         const uint32_t to = s.base[digit[i]] + s.count[threadIdx.x >> 5][digit[i]] + rank[i];
-        (last ? keys_out : bk)[to] = key[i];
-        (last ? pos_out : bp)[to] = pos[i];
+        uint32_t* there = cluster.map_shared_rank(buf, to / kHere);
+        there[to % kHere] = key[i];
+        there[kHere + to % kHere] = pos[i];
       }
-    if (last) break;
-    __syncthreads();
+    cluster.sync();  // the tokens have arrived, and nobody reads `totals` of this pass any more
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int t = tile_index<kPer>(i);
-      if (t < T) {
-        key[i] = bk[t];
-        pos[i] = bp[t];
+    for (int i = 0; i < N; ++i) {
+      const int t = tile_index<N>(i);
+      if (me * kHere + t < T) {
+        key[i] = buf[t];
+        pos[i] = buf[kHere + t];
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int t = me * kHere + tile_index<N>(i);
+    if (t < T) {
+      keys_out[t] = key[i];
+      pos_out[t] = pos[i];
     }
   }
   if (status && bad) atomicOr(status, GTK_STATUS_BAD_TOKEN);
 }
 
 // Pass `pass` of the sort over many tiles, first half: the tile's digit counts. The first pass
-// reads the tokens, later ones the keys of the pass before.
+// reads the tokens, later ones the keys of the pass before. Warps count in four histograms; 32
+// equal digits (frequent tokens, sorted data) are one addition.
 template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
     count_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys, int64_t T, uint32_t V,
                  int64_t padding, int pass, int bits, uint32_t* __restrict__ counts, uint32_t* status) {
   wait_previous_kernel();
-  __shared__ SortShared s;
+  __shared__ uint32_t hist[4][kBins];
+  (&hist[0][0])[threadIdx.x] = 0;
+  __syncthreads();
   bool bad = false;
-  uint32_t digit[kMaxPer], rank[kMaxPer];
+  uint32_t digit[kPer];
 #pragma unroll
-  for (int i = 0; i < kMaxPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kMaxPer>(i);
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
     uint32_t k = 0;
-    if (t < T) k = pass == 0 ? key_of(tokens, t, V, padding, &bad) : keys[t];
+    if (t < T) k = pass == 0 ? key_of(static_cast<int64_t>(tokens[t]), V, padding, &bad) : keys[t];
     digit[i] = t < T ? (k >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
   }
-  const uint32_t total = rank_tile<kMaxPer>(s, digit, rank, bits);
-  if (threadIdx.x < kBins) counts[static_cast<int64_t>(blockIdx.x) * kBins + threadIdx.x] = total;
+  uint32_t* h = hist[(threadIdx.x >> 5) & 3];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t first = __shfl_sync(0xffffffffu, digit[i], 0);
+    if (__all_sync(0xffffffffu, digit[i] == first)) {
+      if ((threadIdx.x & 31) == 0 && first < kBins) atomicAdd(h + first, 32u);
+    } else if (digit[i] < kBins) {
+      atomicAdd(h + digit[i], 1u);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kBins)
+    counts[static_cast<int64_t>(blockIdx.x) * kBins + threadIdx.x] =
+        hist[0][threadIdx.x] + hist[1][threadIdx.x] + hist[2][threadIdx.x] + hist[3][threadIdx.x];
   if (status && bad) atomicOr(status, GTK_STATUS_BAD_TOKEN);
 }
 
@@ -209,48 +259,48 @@ __global__ void __launch_bounds__(kSortThreads)
                    int tiles, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
   wait_previous_kernel();
   __shared__ SortShared s;
-  __shared__ uint32_t before_part[kSlices][kBins], total_part[kSlices][kBins];
-  uint32_t key[kMaxPer], p0[kMaxPer], digit[kMaxPer], rank[kMaxPer];
-  bool bad = false;
+  __shared__ uint32_t before_part[kSortThreads], total_part[kSortThreads];
+  uint32_t key[kPer], p0[kPer], digit[kPer], rank[kPer];
+  int64_t token[kPer];  // requested here, looked at after the counts, which are on their way meanwhile
 #pragma unroll
-  for (int i = 0; i < kMaxPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kMaxPer>(i);
-    key[i] = 0;
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
     p0[i] = static_cast<uint32_t>(t);
-    if (t < T) {
-      if (pass == 0) {
-        key[i] = key_of(tokens, t, V, padding, &bad);
-      } else {
-        key[i] = keys[t];
-        p0[i] = pos[t];
-      }
-    }
-    digit[i] = t < T ? (key[i] >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
+    token[i] = t >= T ? 0 : pass == 0 ? static_cast<int64_t>(tokens[t]) : static_cast<int64_t>(keys[t]);
+    if (pass && t < T) p0[i] = pos[t];
   }
   // thread = (slice of the tiles, bin)
-  const int bin = threadIdx.x & (kBins - 1), slice = threadIdx.x / kBins;
+  const int bins = 1 << bits, slices = kSortThreads >> bits;
+  const int bin = threadIdx.x & (bins - 1), slice = threadIdx.x >> bits;
   uint32_t before = 0, total = 0;
 #pragma unroll 8
-  for (int t = slice; t < tiles; t += kSlices) {
+  for (int t = slice; t < tiles; t += slices) {
     const uint32_t n = counts[static_cast<int64_t>(t) * kBins + bin];
     total += n;
     before += t < static_cast<int>(blockIdx.x) ? n : 0;
   }
-  before_part[slice][bin] = before;
-  total_part[slice][bin] = total;
+  before_part[threadIdx.x] = before;
+  total_part[threadIdx.x] = total;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
+    key[i] = pass == 0 ? key_of(token[i], V, padding, &bad) : static_cast<uint32_t>(token[i]);
+    digit[i] = t < T ? (key[i] >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
+  }
   __syncthreads();
   before = total = 0;
-  if (threadIdx.x < kBins)
-    for (int i = 0; i < kSlices; ++i) {
-      before += before_part[i][threadIdx.x];
-      total += total_part[i][threadIdx.x];
+  if (threadIdx.x < bins)
+    for (int i = 0; i < slices; ++i) {
+      before += before_part[(i << bits) + threadIdx.x];
+      total += total_part[(i << bits) + threadIdx.x];
     }
   const uint32_t base = scan_bins(s, total);
   if (threadIdx.x < kBins) s.base[threadIdx.x] = base + before;
-  rank_tile<kMaxPer>(s, digit, rank, bits);
+  rank_tile<kPer>(s, digit, rank, bits);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kMaxPer; ++i)
+  for (int i = 0; i < kPer; ++i)
     if (digit[i] < kBins) {
       const uint32_t to = s.base[digit[i]] + s.count[threadIdx.x >> 5][digit[i]] + rank[i];
       keys_out[to] = key[i];
@@ -262,15 +312,75 @@ __global__ void __launch_bounds__(kSortThreads)
 
 constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
-constexpr int kBatch = 8;  // dy rows that a warp loads at once
+constexpr int kBatch = 4;  // dy rows that a warp requests and adds at once
 
 template <typename W, int V>
 __device__ __forceinline__ void write_row(W* dst, const float (&acc)[V], float scale) {
-  Vec<W, V> o;
+  float f[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) o.v[j] = Elem<W>::store(acc[j] * scale);
-  st_vec<W, V>(dst, o);
+  for (int j = 0; j < V; ++j) f[j] = acc[j] * scale;
+  constexpr int kMost = 16 / static_cast<int>(sizeof(W));  // elements of a store
+  constexpr int kEach = V < kMost ? V : kMost;
+#pragma unroll
+  for (int j = 0; j < V; j += kEach)
+    st_vec<W, kEach>(dst + j, Vec<W, kEach>::of(reinterpret_cast<const float(&)[kEach]>(f[j])));
 }
+
+// The dy rows of a warp's chunk, requested some batches ahead of their use. 16-byte vectors go to
+// a ring in shared memory with cp.async, sixteen rows (8 KB) a warp, which takes no registers: a
+// lane reads only what it requested itself, so the lane's own wait is enough. Single elements
+// (odd widths) are too small for that and are loaded into registers, one batch ahead.
+template <typename T, int V>
+struct Rows {
+  static constexpr bool kAsync = V > 1;
+  static constexpr int kSlots = kAsync ? 4 : 2;  // batches
+  static constexpr int kAhead = kSlots - 1;
+  static constexpr int kRingBytes = kAsync ? kSlots * kBatch * 32 * 16 : 0;  // of a warp
+  const T* base;
+  const int D;
+  const bool mine;
+  const uint32_t vocab;
+  char* ring;
+  Vec<T, V> held[kAsync ? 1 : kSlots][kBatch];
+
+  __device__ __forceinline__ Rows(const T* b, int d, bool m, uint32_t v, char* r)
+      : base(b), D(d), mine(m), vocab(v), ring(r + (threadIdx.x & 31) * 16) {}
+
+  // Batch g: entries q .. q + 3 of the 32 whose keys and positions the lanes hold.
+  __device__ __forceinline__ void request(int g, uint32_t k32, uint32_t p32, int q) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const uint32_t k = __shfl_sync(0xffffffffu, k32, q + u);
+      const uint32_t p = __shfl_sync(0xffffffffu, p32, q + u);
+      if (!mine || k >= vocab) continue;
+      const T* src = base + static_cast<int64_t>(p) * D;
+      if constexpr (kAsync)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
+                         __cvta_generic_to_shared(ring + ((g % kSlots) * kBatch + u) * 512))),
+                     "l"(src)
+                     : "memory");
+      else
+        held[g % kSlots][u] = ld_vec<T, V>(src);
+    }
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  __device__ __forceinline__ void take(int g, Vec<T, V> (&to)[kBatch]) {
+    if constexpr (kAsync) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        to[u] = ld_vec<T, V>(reinterpret_cast<const T*>(ring + ((g % kSlots) * kBatch + u) * 512));
+    } else {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) to[u] = held[g % kSlots][u];
+    }
+  }
+
+  __device__ __forceinline__ void drain() {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+};
 
 // How a warp's chunk meets its neighbours. kHead: its first run began before it; kHeadOn: and
 // that run goes on behind it (the chunk is one run). kTail: its last run begins in it and goes on.
@@ -285,7 +395,7 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
                                          const uint32_t* __restrict__ pos, W* __restrict__ dw,
                                          float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
                                          int64_t unit, int slab, float scale, float (*edge)[2][32 * V],
-                                         uint32_t* how, uint32_t* run_key) {
+                                         uint32_t* how, uint32_t* run_key, char* ring) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t i0 = (unit * kSumWarps + warp) * L;
   const int col = (slab * 32 + lane) * V;
@@ -299,16 +409,9 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
     // the keys and positions of 32 entries, one per lane, and those of the next 32
     uint32_t k_now = lane < m ? keys[i0 + lane] : 0xffffffffu;
     uint32_t p_now = lane < m ? pos[i0 + lane] : 0u;
-    Vec<T, V> row[2][kBatch];
-    auto load = [&](Vec<T, V>(&to)[kBatch], uint32_t k32, uint32_t p32, int q) {
+    Rows<T, V> rows(dy + col, D, mine, vocab, ring);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const uint32_t k = __shfl_sync(0xffffffffu, k32, q + u);
-        const uint32_t p = __shfl_sync(0xffffffffu, p32, q + u);
-        if (mine && k < vocab) to[u] = ld_vec<T, V>(dy + static_cast<int64_t>(p) * D + col);
-      }
-    };
-    load(row[0], k_now, p_now, 0);
+    for (int g = 0; g < Rows<T, V>::kAhead; ++g) rows.request(g, k_now, p_now, g * kBatch);
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
@@ -321,30 +424,29 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
       const uint32_t k_next = e < m ? keys[i0 + e] : 0xffffffffu;
       const uint32_t p_next = e < m ? pos[i0 + e] : 0u;
 #pragma unroll
-      for (int q = 0; q < 32; q += kBatch) {
-        if (b + q >= m) break;
-        Vec<T, V>(&now)[kBatch] = row[(q / kBatch) & 1];
-        // the next batch is on its way while this one is added up
-        if (q + kBatch < 32)
-          load(row[(q / kBatch + 1) & 1], k_now, p_now, q + kBatch);
+      for (int g = 0; g < 32 / kBatch; ++g) {
+        if (b + g * kBatch >= m) break;
+        // a later batch is on its way while this one is added up
+        const int ahead = g + Rows<T, V>::kAhead;
+        if (ahead < 32 / kBatch)
+          rows.request(ahead, k_now, p_now, ahead * kBatch);
         else
-          load(row[(q / kBatch + 1) & 1], k_next, p_next, 0);
-        const uint32_t k0 = __shfl_sync(0xffffffffu, k_now, q);
-        const uint32_t k7 = __shfl_sync(0xffffffffu, k_now, q + kBatch - 1);
-        if (k0 == cur && k7 == cur && cur < vocab) {  // eight rows of the current run: a tree
+          rows.request(ahead, k_next, p_next, (ahead - 32 / kBatch) * kBatch);
+        Vec<T, V> now[kBatch];
+        rows.take(g, now);
+        const uint32_t k0 = __shfl_sync(0xffffffffu, k_now, g * kBatch);
+        const uint32_t k3 = __shfl_sync(0xffffffffu, k_now, g * kBatch + kBatch - 1);
+        if (k0 == cur && k3 == cur && cur < vocab) {  // all of the current run: a tree
           if (mine)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              float t[kBatch];
-#pragma unroll
-              for (int u = 0; u < kBatch; ++u) t[u] = Elem<T>::load(now[u].v[j]);
-              acc[j] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-            }
+            for (int j = 0; j < V; ++j)
+              acc[j] += (now[0].get(j) + now[1].get(j)) +
+                        (now[2].get(j) + now[3].get(j));
           continue;
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const uint32_t k = __shfl_sync(0xffffffffu, k_now, q + u);
+          const uint32_t k = __shfl_sync(0xffffffffu, k_now, g * kBatch + u);
           if (k >= vocab) continue;  // none, or sorted last: nothing follows but more of them
           if (k != cur) {
             if (mine) {
@@ -361,12 +463,13 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
           }
           if (mine)
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += Elem<T>::load(now[u].v[j]);
+            for (int j = 0; j < V; ++j) acc[j] += now[u].get(j);
         }
       }
       k_now = k_next;
       p_now = p_next;
     }
+    rows.drain();
     if (cur < vocab) {
       const bool goes_on = cur == right;
       if (!goes_on && !continued) {
@@ -413,17 +516,18 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
 // Blocks [0, units * slabs) sum; those behind them zero the rows of the tokens that do not occur:
 // 32 rows and zero_cols columns per warp, a binary search of the sorted keys for each row.
 template <typename T, typename W, int V>
-__global__ void __launch_bounds__(kSumThreads, 2)
+__global__ void __launch_bounds__(kSumThreads, 3)
     run_sums_kernel(const T* __restrict__ dy, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                     W* __restrict__ dw, float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
                     int slabs, int64_t sum_blocks, int zero_cols, int zero_slabs, float scale) {
   wait_previous_kernel();
+  extern __shared__ __align__(16) char rings[];
   __shared__ float edge[kSumWarps][2][32 * V];
   __shared__ uint32_t how[kSumWarps], run_key[kSumWarps];
   if (blockIdx.x < sum_blocks) {
     const int64_t unit = blockIdx.x / static_cast<uint32_t>(slabs);
     sum_unit<T, W, V>(dy, keys, pos, dw, partial, n, vocab, D, L, unit, static_cast<int>(blockIdx.x - unit * slabs),
-                      scale, edge, how, run_key);
+                      scale, edge, how, run_key, rings + (threadIdx.x >> 5) * Rows<T, V>::kRingBytes);
     return;
   }
   const int lane = threadIdx.x & 31;
@@ -452,13 +556,15 @@ __global__ void __launch_bounds__(kSumThreads, 2)
 // The runs that cross units: the block of the unit in which one begins adds its tail and the heads
 // of the units after it, 128 columns at a time.
 constexpr int kJoinCols = 128;
+constexpr int kJoinThreads = 512;
+constexpr int kJoinWarps = kJoinThreads / 32;
 
 template <typename W>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kJoinThreads)
     join_runs_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, W* __restrict__ dw,
                      int64_t n, uint32_t vocab, int D, int64_t unit_len, int slabs, float scale) {
   wait_previous_kernel();
-  __shared__ double part[kSumWarps][kJoinCols];
+  __shared__ double part[kJoinWarps][kJoinCols];
   const int64_t u = blockIdx.x / static_cast<uint32_t>(slabs);
   const int col0 = static_cast<int>(blockIdx.x - u * slabs) * kJoinCols;
   const int64_t i0 = u * unit_len, i1 = i0 + unit_len;
@@ -468,14 +574,14 @@ __global__ void __launch_bounds__(kSumThreads)
   if (i0 > 0 && keys[i0] == k && keys[i0 - 1] == k) return;  // it began earlier
   // the units behind it whose first entry belongs to the run
   int64_t heads = 0;
-  for (int count = kSumThreads; count == kSumThreads; heads += count) {
+  for (int count = kJoinThreads; count == kJoinThreads; heads += count) {
     const int64_t j = (u + 1 + heads + threadIdx.x) * unit_len;
     count = __syncthreads_count(j < n && keys[j] == k);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double s[kJoinCols / 32] = {};
-#pragma unroll 4
-  for (int64_t j = warp; j <= heads; j += kSumWarps) {  // 0: the tail, then the heads
+#pragma unroll 8
+  for (int64_t j = warp; j <= heads; j += kJoinWarps) {  // 0: the tail, then the heads
     const float* p = partial + (j == 0 ? u * 2 + 1 : (u + j) * 2) * D + col0 + lane;
 #pragma unroll
     for (int i = 0; i < kJoinCols / 32; ++i)
@@ -488,7 +594,7 @@ __global__ void __launch_bounds__(kSumThreads)
   if (threadIdx.x >= kJoinCols || c >= D) return;
   double t = part[0][threadIdx.x];
 #pragma unroll
-  for (int w = 1; w < kSumWarps; ++w) t += part[w][threadIdx.x];
+  for (int w = 1; w < kJoinWarps; ++w) t += part[w][threadIdx.x];
   dw[static_cast<int64_t>(k) * D + c] = Elem<W>::store(static_cast<float>(t * scale));
 }
 
@@ -519,17 +625,16 @@ __global__ void __launch_bounds__(256)
           e[q] = ld_vec<T, V>(w + tok[q] * D + static_cast<int64_t>(i) * V);
         else {
           bad = true;
-#pragma unroll
-          for (int j = 0; j < V; ++j) e[q].v[j] = Elem<T>::store(0.f);
+          e[q] = Vec<T, V>::zero();
         }
       }
 #pragma unroll
       for (int q = 0; q < kRowsAtOnce; ++q) {
         if (r + q >= n) continue;
-        Vec<T, V> o;
+        float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = Elem<T>::store(Elem<T>::load(e[q].v[j]) * scale);
-        st_vec<T, V>(y + (r + q) * D + static_cast<int64_t>(i) * V, o);
+        for (int j = 0; j < V; ++j) o[j] = e[q].get(j) * scale;
+        st_vec<T, V>(y + (r + q) * D + static_cast<int64_t>(i) * V, Vec<T, V>::of(o));
       }
     }
   }
@@ -553,22 +658,29 @@ int vec_width(int64_t D, size_t bytes, bool aligned) {
 struct Plan {
   int passes, bits;  // of the sort, for keys 0 .. vocab
   int64_t tiles;
+  bool zero_first;   // all of dW is zeroed beside the sort
   int64_t L, units;                            // entries of a warp's chunk; units of kSumWarps chunks
   size_t keys, pos, counts, partial, total;    // byte offsets (keys, pos: two buffers each)
 };
 
-Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype) {
+Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype, int w_dtype) {
   Plan p = {};
   int bits = 1;
   while (vocab >> bits) ++bits;
   p.passes = (bits + kMaxBits - 1) / kMaxBits;
   p.bits = (bits + p.passes - 1) / p.passes;
   p.tiles = (T + kTile - 1) / kTile;
-  // About 16 warps per SM get a chunk, of whole batches. Up to 512 tokens make one unit: the
+  // The sort of a short list leaves most of the device idle for some 8 us, in which it can zero
+  // all of dW. The rows that do occur are then written twice, which costs less than that time
+  // as long as they are at most 32 MB (8192 tokens, 32000 x 1024 bf16: the whole gradient takes
+  // 26 us, against 37 us when the absent rows are looked up and zeroed after the sort).
+  p.zero_first = T <= kClusterTokens &&
+                 (T < vocab ? T : vocab) * D * static_cast<int64_t>(dtype_bytes(w_dtype)) <= (32 << 20);
+  // About 24 warps per SM get a chunk, of whole batches. Up to 512 tokens make one unit: the
   // launch that joins units costs more than the longer chunks.
   const int64_t slab = 32 * 16 / static_cast<int64_t>(dtype_bytes(dy_dtype));
   const int64_t slabs = (D + slab - 1) / slab;
-  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 16 - 1) / (148 * 16);
+  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 24 - 1) / (148 * 24);
   L = (L + kBatch - 1) / kBatch * kBatch;
   p.L = L > 1024 ? 1024 : L;
   p.units = (T + p.L * kSumWarps - 1) / (p.L * kSumWarps);
@@ -578,10 +690,10 @@ Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype) {
     at += round_up(bytes, 256);
     return o;
   };
-  const bool two = p.tiles > 1 && p.passes > 1;
+  const bool tiled = T > kClusterTokens, two = tiled && p.passes > 1;
   p.keys = take((two ? 2 : 1) * round_up(4 * T, 256));
   p.pos = take((two ? 2 : 1) * round_up(4 * T, 256));
-  p.counts = take(p.tiles > 1 ? 4 * kBins * p.tiles : 0);
+  p.counts = take(tiled ? 4 * kBins * p.tiles : 0);
   p.partial = take(p.units > 1 ? static_cast<size_t>(p.units) * 2 * D * sizeof(float) : 0);
   p.total = at;
   return p;
@@ -591,20 +703,41 @@ struct Args {
   const void *tokens, *dy;
   void* dw;
   char* ws;
-  int64_t T, vocab, D, padding;
+  int64_t T, vocab, D, padding, dw_bytes;
   float scale;
   uint32_t* status;
   cudaStream_t st;
 };
 
-template <typename I, int kPer>
-int sort_small(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
-  const int smem = p.passes > 1 ? 2 * kSortThreads * kPer * 4 : 0;
-  auto kernel = sort_small_kernel<I, kPer>;
-  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), 2 * kSortThreads * kPer * 4)) return e;
-  return launch("embedding token sort", kernel, 1, kSortThreads, smem, a.st, false, static_cast<const I*>(a.tokens),
-                static_cast<int>(a.T), static_cast<uint32_t>(a.vocab), a.padding, p.passes, p.bits, keys, pos,
-                a.status);
+template <typename I, int N>
+int sort_cluster(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
+  auto kernel = sort_cluster_kernel<I, N>;
+  const int smem = 2 * kSortThreads * N * 4;
+  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), smem)) return e;
+  int blocks = 1;
+  while (static_cast<int64_t>(blocks) * kSortThreads * N < a.T) blocks <<= 1;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t zero_bytes = p.zero_first ? a.dw_bytes : 0;
+  // two blocks per SM, in whole clusters, but no more than there are 64 KB pieces
+  int64_t zero_blocks = (zero_bytes + 65535) / 65536;
+  if (zero_blocks > 2 * num_sms()) zero_blocks = 2 * num_sms();
+  zero_blocks = (zero_blocks + blocks - 1) / blocks * blocks;
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks + zero_blocks));
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = a.st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(a.tokens), static_cast<int>(a.T),
+                                           static_cast<uint32_t>(a.vocab), a.padding, p.passes, p.bits, keys, pos,
+                                           static_cast<uint4*>(a.dw), zero_bytes, a.status);
+  if (e == cudaSuccess) return GTK_OK;
+  cudaGetLastError();
+  return fail(GTK_ERR_CUDA, std::string("embedding token sort: ") + cudaGetErrorString(e));
 }
 
 template <typename I>
@@ -614,14 +747,13 @@ int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** p
   uint32_t* q[2] = {reinterpret_cast<uint32_t*>(a.ws + p.pos), reinterpret_cast<uint32_t*>(a.ws + p.pos + half)};
   const I* tokens = static_cast<const I*>(a.tokens);
   const uint32_t V = static_cast<uint32_t>(a.vocab);
-  if (p.tiles == 1) {
+  if (a.T <= kClusterTokens) {
     *keys = k[0];
     *pos = q[0];
-    // one token per thread as far as that goes: the ranks of a thread's tokens are one after another
-    if (a.T <= kSortThreads) return sort_small<I, 1>(a, p, k[0], q[0]);
-    if (a.T <= 2 * kSortThreads) return sort_small<I, 2>(a, p, k[0], q[0]);
-    if (a.T <= 4 * kSortThreads) return sort_small<I, 4>(a, p, k[0], q[0]);
-    return sort_small<I, kMaxPer>(a, p, k[0], q[0]);
+    // as few tokens per thread as the cluster allows: their ranks are found one after another
+    if (a.T <= kSortThreads * kMaxCluster) return sort_cluster<I, 1>(a, p, k[0], q[0]);
+    if (a.T <= 2 * kSortThreads * kMaxCluster) return sort_cluster<I, 2>(a, p, k[0], q[0]);
+    return sort_cluster<I, kClusterPer>(a, p, k[0], q[0]);
   }
   uint32_t* counts = reinterpret_cast<uint32_t*>(a.ws + p.counts);
   const uint32_t *ki = nullptr, *qi = nullptr;
@@ -646,20 +778,24 @@ template <typename T, typename W, int V>
 int sums(const Args& a, const Plan& p, const uint32_t* keys, const uint32_t* pos) {
   const int slabs = static_cast<int>((a.D + 32 * V - 1) / (32 * V));
   const int64_t sum_blocks = p.units * slabs;
-  const int zero_cols = 8 * 32 * V;
+  const int zero_cols = 2 * 32 * V;
   const int zero_slabs = static_cast<int>((a.D + zero_cols - 1) / zero_cols);
-  const int64_t zero_blocks = ((a.vocab + 31) / 32 * zero_slabs + kSumWarps - 1) / kSumWarps;
+  const int64_t zero_blocks =
+      p.zero_first ? 0 : ((a.vocab + 31) / 32 * zero_slabs + kSumWarps - 1) / kSumWarps;
   const int join_slabs = static_cast<int>((a.D + kJoinCols - 1) / kJoinCols);
   if (sum_blocks + zero_blocks > (int64_t(1) << 31) - 1 || p.units * join_slabs > (int64_t(1) << 31) - 1)
     return fail(GTK_ERR_UNSUPPORTED, "embedding: tokens or vocabulary times width too large");
   float* partial = reinterpret_cast<float*>(a.ws + p.partial);
   const uint32_t V32 = static_cast<uint32_t>(a.vocab);
-  if (int e = launch("embedding run sums", run_sums_kernel<T, W, V>, sum_blocks + zero_blocks, kSumThreads, 0, a.st,
-                     true, static_cast<const T*>(a.dy), keys, pos, static_cast<W*>(a.dw), partial, a.T, V32,
+  auto kernel = run_sums_kernel<T, W, V>;
+  constexpr int kSmem = kSumWarps * Rows<T, V>::kRingBytes;
+  if (kSmem)
+    if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
+  if (int e = launch("embedding run sums", kernel, sum_blocks + zero_blocks, kSumThreads, kSmem, a.st, true, static_cast<const T*>(a.dy), keys, pos, static_cast<W*>(a.dw), partial, a.T, V32,
                      static_cast<int>(a.D), static_cast<int>(p.L), slabs, sum_blocks, zero_cols, zero_slabs, a.scale))
     return e;
   if (p.units == 1) return GTK_OK;
-  return launch("embedding run join", join_runs_kernel<W>, (p.units - 1) * join_slabs, kSumThreads, 0, a.st, true,
+  return launch("embedding run join", join_runs_kernel<W>, (p.units - 1) * join_slabs, kJoinThreads, 0, a.st, true,
                 keys, static_cast<const float*>(partial), static_cast<W*>(a.dw), a.T, V32, static_cast<int>(a.D),
                 p.L * kSumWarps, join_slabs, a.scale);
 }
@@ -721,7 +857,7 @@ int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight
 
 size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D, int dy_dtype) {
   if (!dims_ok(n_tokens) || !dims_ok(vocab) || !dims_ok(D, emb::kMaxWidth) || !dtype_ok(dy_dtype)) return 0;
-  return emb::plan_for(n_tokens, vocab, D, dy_dtype).total;
+  return emb::plan_for(n_tokens, vocab, D, dy_dtype, dy_dtype).total;
 }
 
 int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int index_bits, void* dweight,
@@ -731,7 +867,7 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
   if (!dtype_ok(dy_dtype) || !(w_dtype == dy_dtype || w_dtype == GTK_F32))
     return fail(GTK_ERR_UNSUPPORTED, "embedding: dy is fp32, bf16 or fp16, the table's gradient fp32 or dy's type");
   if (padding >= vocab) return fail(GTK_ERR_INVALID_ARG, "embedding: the padding token must be below the vocabulary");
-  const emb::Plan p = emb::plan_for(n_tokens, vocab, D, dy_dtype);
+  emb::Plan p = emb::plan_for(n_tokens, vocab, D, dy_dtype, w_dtype);
   if (workspace_bytes < p.total) return fail(GTK_ERR_WORKSPACE, "embedding: workspace too small");
   if (int e = emb::check_tokens(tokens, index_bits)) return e;
   if (int e = check_ptr(dy, "dy", dtype_bytes(dy_dtype))) return e;
@@ -741,6 +877,8 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
   emb::Args a = {};
   a.tokens = tokens, a.dy = dy, a.dw = dweight, a.ws = static_cast<char*>(workspace), a.T = n_tokens;
   a.vocab = vocab, a.D = D, a.padding = padding, a.scale = scale, a.status = status;
+  a.dw_bytes = vocab * D * static_cast<int64_t>(dtype_bytes(w_dtype));
+  p.zero_first = p.zero_first && aligned16(dweight) && a.dw_bytes % 16 == 0;
   a.st = static_cast<cudaStream_t>(stream);
   const uint32_t *keys = nullptr, *pos = nullptr;
   if (int e = index_bits == 64 ? emb::sort<int64_t>(a, p, &keys, &pos) : emb::sort<int32_t>(a, p, &keys, &pos))

@@ -7,15 +7,16 @@
 // k is NaN when the norm is (every output becomes NaN) and 0 when the norm is infinite, the
 // same as torch.nn.utils.clip_grad_norm_.
 //
-// What bounds it: HBM, and for the gradients of a small model the launches. Two launches:
-// clip_norm_kernel reads the gradients once and leaves one partial per block; clip_scale_kernel
-// adds the partials (every block the same sum, in the same order) and scales. The tensors
-// reach the kernels as a table in the kernel's own parameters (up to 1000 tensors a launch), so
-// there is no table to copy to the device and nothing to keep alive behind the call.
+// What bounds it: HBM, and for the gradients of a small model the host and the launches. Two
+// launches: clip_norm_kernel reads the gradients once and leaves one partial per block;
+// clip_scale_kernel adds the partials (every block the same sum, in the same order) and scales.
+// The list of tensors travels in the first kernel's parameters (24 bytes a tensor, up to 1000
+// tensors a launch), which writes it to the workspace for the second: there is no table to copy
+// to the device and nothing to keep alive behind the call.
 //
-// The tensors are cut into chunks of 8192 elements, and every block owns a run of consecutive
-// chunks. The second kernel walks its run backwards: what the first one read last is still in
-// the L2 cache then. In place and with k = 1 it has nothing to do and returns.
+// The tensors are cut into chunks, and every block owns a run of consecutive ones (one search of
+// the table per block; taking chunks in turn, with a search for each, was 20% slower). The second
+// kernel walks its run backwards: what the first one read last is still in the L2 cache then. In place and with k = 1 it has nothing to do and returns.
 //
 // Squares are summed 16 at a time in fp32 and from there on in 64 bits. Where such a sum is not
 // a plain number (it overflowed, or is so small that its squares may have underflowed) the 16
@@ -28,21 +29,43 @@
 namespace gtk {
 namespace clip {
 
-constexpr int kThreads = 512;
-constexpr int kPer = 16;                      // elements per thread and chunk
-constexpr int kChunk = kThreads * kPer;       // 8192
-constexpr int kBlocksPerSm = 2;
+constexpr int kThreads = 256;
+// Elements per thread and chunk. Few elements in all are cut finely, to spread them over the
+// device; many coarsely, so that a thread has 128 bytes in flight (see `coarse` below).
+constexpr int kFine = 16, kCoarse = 64;
+constexpr int kFineBlocks = 8, kCoarseBlocks = 4;  // per SM
+constexpr int kBlocksPerSm = kFineBlocks;
 constexpr int kMaxBlocks = 148 * kBlocksPerSm;  // partials per launch
-constexpr int kMaxTensors = 1000;             // of one launch (32,000 of the 32,764 parameter bytes)
+constexpr int kMaxTensors = 1000;             // of one launch (24,000 of the 32,764 parameter bytes)
 constexpr float kEps = 1e-6f;
 
 struct Tensor {
   const void* in;
   void* out;
-  int64_t numel;
-  uint32_t first_chunk;
+  uint32_t first_chunk;  // of the tensor, counted over the launch
+  uint16_t last_len;     // elements of its last chunk, from 1 on
   uint8_t in_type, out_type;
 };
+static_assert(sizeof(Tensor) == 24, "the parameter table's size");
+
+// Chunks begin on 16-byte boundaries of the gradient: they are counted from the boundary at or
+// before its first element, `lead` elements earlier, and the first chunk is that much shorter.
+__host__ __device__ __forceinline__ int lead_of(const void* in, int type) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(in) & 15u) / (type == GTK_F32 ? 4 : 2));
+}
+
+struct Span {
+  int64_t off;  // of the chunk's first element in the tensor
+  int n;
+};
+// Chunk i (of `size` elements) of a tensor; `last`: its last one.
+__device__ __forceinline__ Span span_of(const Tensor& e, uint32_t i, bool last, int size) {
+  const int lead = lead_of(e.in, e.in_type);
+  Span s;
+  s.off = i ? static_cast<int64_t>(i) * size - lead : 0;
+  s.n = last ? e.last_len : i ? size : size - lead;
+  return s;
+}
 
 template <int N>
 struct Table {
@@ -52,13 +75,18 @@ struct Table {
   uint32_t per;     // chunks of one block
 };
 
-// The tensor that holds chunk c (t.first_chunk is ascending).
-template <int N>
-__device__ __forceinline__ int find(const Table<N>& tab, uint32_t c) {
-  int lo = 0, hi = tab.n - 1;
+// What the second kernel needs of a launch's table, in the workspace.
+struct Shadow {
+  Tensor t[kMaxTensors];
+};
+
+// The tensor that holds chunk c: first(i) is ascending in i < n.
+template <typename F>
+__device__ __forceinline__ int find(F first, int n, uint32_t c) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab.t[mid].first_chunk <= c)
+    if (first(mid) <= c)
       lo = mid;
     else
       hi = mid - 1;
@@ -66,64 +94,90 @@ __device__ __forceinline__ int find(const Table<N>& tab, uint32_t c) {
   return lo;
 }
 
-__device__ __forceinline__ float square_or_max(float acc, float v, bool inf_norm) {
-  // |v| as an ordered integer, in which NaN is above infinity
-  if (inf_norm) return __uint_as_float(max(__float_as_uint(acc), __float_as_uint(v) & 0x7fffffffu));
-  return fmaf(v, v, acc);
-}
-
-// acc += the squares of n values whose fp32 sum is s (or the maximum, as ordered bits).
-template <int n>
-__device__ __forceinline__ void add_sum(double& acc, float s, const float (&v)[n], bool inf_norm) {
-  if (inf_norm) {
-    acc = __longlong_as_double(max(__double_as_longlong(acc), static_cast<long long>(__float_as_uint(s))));
-    return;
-  }
-  if (s > 1e-20f && s < 1e37f) {
-    acc += static_cast<double>(s);
-    return;
-  }
-  for (int i = 0; i < n; ++i) acc = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), acc);
-}
-
-template <typename T>
-__device__ __forceinline__ void norm_chunk(const T* p, int n, bool inf_norm, double& acc) {
-  constexpr int V = 16 / sizeof(T);
-  constexpr int K = kPer / V;
-  // elements before the first 16-byte boundary, then vectors, then the rest
-  int head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / sizeof(T));
-  head = head < n ? head : n;
-  const int nv = (n - head) / V;
-  Vec<T, V> e[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    if (i < nv)
-      e[k] = ld_vec<T, V>(p + head + i * V);
-    else
-#pragma unroll
-      for (int j = 0; j < V; ++j) e[k].v[j] = Elem<T>::store(0.f);
-  }
-  float v[kPer], s = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[k * V + j] = Elem<T>::load(e[k].v[j]);
-      s = square_or_max(s, v[k * V + j], inf_norm);
-    }
-  if (s != 0.f || threadIdx.x < nv) add_sum(acc, s, v, inf_norm);
-  const int loose = n - nv * V;
-  if (threadIdx.x < loose) {
-    const int i = threadIdx.x < head ? threadIdx.x : threadIdx.x + nv * V;
-    float w[1] = {Elem<T>::load(p[i])};
-    add_sum(acc, square_or_max(0.f, w[0], inf_norm), w, inf_norm);
-  }
-}
+// |v| as an ordered integer, in which NaN is above infinity.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 __device__ __forceinline__ double join(double a, double b, bool inf_norm) {
   if (!inf_norm) return a + b;
   return __longlong_as_double(max(__double_as_longlong(a), __double_as_longlong(b)));
+}
+
+// The sum of squares of n loaded vectors, or the largest magnitude (as ordered bits in a double).
+template <typename T, int V, int K>
+__device__ __forceinline__ double reduce(const Vec<T, V> (&e)[K], bool inf_norm) {
+  if (inf_norm) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = max(m, magnitude(e[k].get(j)));
+    return __longlong_as_double(static_cast<long long>(m));
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float v = e[k].get(j);
+      s = fmaf(v, v, s);
+    }
+  if (s > 1e-20f && s < 1e37f) return static_cast<double>(s);
+  double d = 0.0;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double v = static_cast<double>(e[k].get(j));
+      d = fma(v, v, d);
+    }
+  return d;
+}
+
+// Elements before the first 16-byte boundary (of `bytes` each), at most n.
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int n) {
+  const int head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / sizeof(T));
+  return head < n ? head : n;
+}
+
+// Vectors of V elements that a thread loads at once: 128 bytes, or the fine chunk's share.
+template <typename T, int V, int kPer>
+constexpr int vectors() {
+  const int all = kPer / V, most = 128 / (V * static_cast<int>(sizeof(T)));
+  return all < most ? all : most;
+}
+
+template <typename T, int kPer>
+__device__ __forceinline__ void norm_chunk(const T* p, int n, bool inf_norm, double& acc) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int K = vectors<T, V, kPer>();
+  // elements before the first 16-byte boundary, then vectors, then the rest
+  const int head = head_of(p, n), nv = (n - head) / V;
+  const T* src = p + head + threadIdx.x * V;
+  constexpr int kStep = 16 / V;  // sixteen squares to a sum
+  int left = nv - static_cast<int>(threadIdx.x);
+#pragma unroll 1
+  for (; left > (K - 1) * kThreads; left -= K * kThreads, src += K * kThreads * V) {
+    Vec<T, V> e[K / kStep][kStep];
+#pragma unroll
+    for (int k = 0; k < K; ++k) e[k / kStep][k % kStep] = ld_vec<T, V>(src + k * kThreads * V);
+#pragma unroll
+    for (int k = 0; k < K / kStep; ++k) acc = join(acc, reduce(e[k], inf_norm), inf_norm);
+  }
+  constexpr int R = kStep;  // what is left, a sum at once
+#pragma unroll 1
+  for (; left > 0; left -= R * kThreads, src += R * kThreads * V) {
+    Vec<T, V> e[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      e[k] = left > k * kThreads ? ld_vec<T, V>(src + k * kThreads * V) : Vec<T, V>::zero();
+    acc = join(acc, reduce(e, inf_norm), inf_norm);
+  }
+  const int loose = n - nv * V, x = threadIdx.x;
+  if (x < loose) {
+    const Vec<T, 1> w[1] = {ld_vec<T, 1>(p + (x < head ? x : x + nv * V))};
+    acc = join(acc, reduce(w, inf_norm), inf_norm);
+  }
 }
 
 // The block's total in every thread.
@@ -139,24 +193,30 @@ __device__ __forceinline__ double block_total(double v, bool inf_norm) {
   return t;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads)
-    clip_norm_kernel(const __grid_constant__ Table<N> tab, double* __restrict__ partial, bool inf_norm) {
+template <int N, int kPer>
+__global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoarseBlocks)
+    clip_norm_kernel(const __grid_constant__ Table<N> tab, double* __restrict__ partial, Shadow* __restrict__ shadow,
+                     bool inf_norm) {
+  if (shadow)
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < tab.n; i += gridDim.x * kThreads) shadow->t[i] = tab.t[i];
+  constexpr int kChunk = kThreads * kPer;
   double acc = 0.0;
   const uint32_t c0 = blockIdx.x * tab.per;
   const uint32_t c1 = min(c0 + tab.per, tab.chunks);
-  int t = c0 < c1 ? find(tab, c0) : 0;
+  int t = c0 < c1 ? find([&](int i) { return tab.t[i].first_chunk; }, tab.n, c0) : 0;
   for (uint32_t c = c0; c < c1; ++c) {
-    while (t + 1 < tab.n && tab.t[t + 1].first_chunk <= c) ++t;
+    uint32_t next = t + 1 < tab.n ? tab.t[t + 1].first_chunk : tab.chunks;
+    if (next <= c) next = ++t + 1 < tab.n ? tab.t[t + 1].first_chunk : tab.chunks;  // every tensor has a chunk
     const Tensor& e = tab.t[t];
-    const int64_t off = static_cast<int64_t>(c - e.first_chunk) * kChunk;
-    const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), e.numel - off));
+    const Span sp = span_of(e, c - e.first_chunk, c + 1 == next, kChunk);
+    const int64_t off = sp.off;
+    const int n = sp.n;
     if (e.in_type == GTK_F32)
-      norm_chunk(static_cast<const float*>(e.in) + off, n, inf_norm, acc);
+      norm_chunk<float, kPer>(static_cast<const float*>(e.in) + off, n, inf_norm, acc);
     else if (e.in_type == GTK_BF16)
-      norm_chunk(static_cast<const __nv_bfloat16*>(e.in) + off, n, inf_norm, acc);
+      norm_chunk<__nv_bfloat16, kPer>(static_cast<const __nv_bfloat16*>(e.in) + off, n, inf_norm, acc);
     else
-      norm_chunk(static_cast<const __half*>(e.in) + off, n, inf_norm, acc);
+      norm_chunk<__half, kPer>(static_cast<const __half*>(e.in) + off, n, inf_norm, acc);
   }
   const double total = block_total(acc, inf_norm);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
@@ -165,80 +225,99 @@ __global__ void __launch_bounds__(kThreads)
 // The norm from all blocks' partials, the same in every block.
 __device__ __forceinline__ double total_norm(const double* partial, int n, bool inf_norm) {
   double v = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += kThreads) v = join(v, partial[i], inf_norm);
   v = block_total(v, inf_norm);
   return inf_norm ? static_cast<double>(__uint_as_float(static_cast<uint32_t>(__double_as_longlong(v)))) : sqrt(v);
 }
 
-template <typename T, typename O>
-__device__ __forceinline__ void scale_chunk(const T* p, O* o, int n, float k) {
-  constexpr int V = 16 / sizeof(T);
-  constexpr int K = kPer / V;
-  int head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / sizeof(T));
-  head = head < n ? head : n;
-  const int nv = (n - head) / V;
-  constexpr int kOutAlign = sizeof(O) * V < 16 ? sizeof(O) * V : 16;
-  const bool vec = (reinterpret_cast<uintptr_t>(o + head) % kOutAlign) == 0;
-  Vec<T, V> e[K];
+template <typename T, typename O, int V>
+__device__ __forceinline__ Vec<O, V> scaled(const Vec<T, V>& e, float k) {
+  float f[V];
 #pragma unroll
-  for (int q = 0; q < K; ++q) {
-    const int i = threadIdx.x + q * kThreads;
-    if (i < nv) e[q] = ld_vec<T, V>(p + head + i * V);
+  for (int j = 0; j < V; ++j) f[j] = e.get(j) * k;
+  return Vec<O, V>::of(f);
+}
+
+// o = k p over one chunk. Vectors of V elements: 16 bytes of the output each, so that a warp's
+// stores are contiguous (16-bit gradients to fp32: 8-byte loads, 16-byte stores).
+template <typename T, typename O, int kPer>
+__device__ __forceinline__ void scale_chunk(const void* in, void* out, int64_t off, int n, float k) {
+  const T* p = static_cast<const T*>(in) + off;
+  O* o = static_cast<O*>(out) + off;
+  constexpr int V = 16 / sizeof(O);
+  constexpr int K = vectors<T, V, kPer>();
+  const int head = head_of(p, n), nv = (n - head) / V;
+  if ((reinterpret_cast<uintptr_t>(o + head) & 15u) != 0) {  // gradient and output lie differently
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kThreads) o[i] = Elem<O>::store(Elem<T>::load(p[i]) * k);
+    return;
   }
+  const T* src = p + head + threadIdx.x * V;
+  O* dst = o + head + threadIdx.x * V;
+  int left = nv - static_cast<int>(threadIdx.x);
+#pragma unroll 1
+  for (; left > (K - 1) * kThreads; left -= K * kThreads, src += K * kThreads * V, dst += K * kThreads * V) {
+    Vec<T, V> e[K];
 #pragma unroll
-  for (int q = 0; q < K; ++q) {
-    const int i = threadIdx.x + q * kThreads;
-    if (i >= nv) continue;
-    O* d = o + head + i * V;
-    constexpr int VO = kOutAlign / sizeof(O);
+    for (int q = 0; q < K; ++q) e[q] = ld_vec<T, V>(src + q * kThreads * V);
 #pragma unroll
-    for (int a = 0; a < V; a += VO) {
-      Vec<O, VO> w;
-#pragma unroll
-      for (int j = 0; j < VO; ++j) w.v[j] = Elem<O>::store(Elem<T>::load(e[q].v[a + j]) * k);
-      if (vec)
-        st_vec<O, VO>(d + a, w);
-      else
-#pragma unroll
-        for (int j = 0; j < VO; ++j) d[a + j] = w.v[j];
-    }
+    for (int q = 0; q < K; ++q) st_vec<O, V>(dst + q * kThreads * V, scaled<T, O, V>(e[q], k));
   }
-  const int loose = n - nv * V;
-  if (threadIdx.x < loose) {
-    const int i = threadIdx.x < head ? threadIdx.x : threadIdx.x + nv * V;
+  constexpr int R = K < 4 ? K : 4;  // what is left, a few vectors at once
+#pragma unroll 1
+  for (; left > 0; left -= R * kThreads, src += R * kThreads * V, dst += R * kThreads * V) {
+    Vec<T, V> e[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      e[q] = left > q * kThreads ? ld_vec<T, V>(src + q * kThreads * V) : Vec<T, V>::zero();
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (left > q * kThreads) st_vec<O, V>(dst + q * kThreads * V, scaled<T, O, V>(e[q], k));
+  }
+  const int loose = n - nv * V, x = threadIdx.x;
+  if (x < loose) {
+    const int i = x < head ? x : x + nv * V;
     o[i] = Elem<O>::store(Elem<T>::load(p[i]) * k);
   }
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads)
-    clip_scale_kernel(const __grid_constant__ Table<N> tab, const double* __restrict__ partial, int partials,
-                      bool inf_norm, double max_norm, bool in_place, float* __restrict__ norm_out) {
+template <int kPer>
+__global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoarseBlocks)
+    clip_scale_kernel(const Shadow* __restrict__ shadow, int tensors, uint32_t chunks, uint32_t per,
+                      const double* __restrict__ partial, int partials, bool inf_norm, double max_norm, bool in_place,
+                      float* __restrict__ norm_out) {
   wait_previous_kernel();
-  const double norm = total_norm(partial, partials, inf_norm);
+  __shared__ uint32_t first[kMaxTensors + 1];
+  for (int i = threadIdx.x; i < tensors; i += kThreads) first[i] = shadow->t[i].first_chunk;
+  if (threadIdx.x == 0) first[tensors] = chunks;
+  const double norm = total_norm(partial, partials, inf_norm);  // its barrier covers `first` too
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(norm);
   const double q = max_norm / (norm + static_cast<double>(kEps));
   const float k = static_cast<float>(q < 1.0 || isnan(q) ? q : 1.0);
   if (in_place && k == 1.f) return;
-  const uint32_t c0 = blockIdx.x * tab.per;
-  const uint32_t c1 = min(c0 + tab.per, tab.chunks);
+  constexpr int kChunk = kThreads * kPer;
+  const uint32_t c0 = blockIdx.x * per;
+  const uint32_t c1 = min(c0 + per, chunks);
   if (c0 >= c1) return;
-  int t = find(tab, c1 - 1);
+  int t = find([&](int i) { return first[i]; }, tensors, c1 - 1);
+  Tensor e = shadow->t[t];
+#pragma unroll 1
   for (uint32_t c = c1; c-- > c0;) {
-    while (tab.t[t].first_chunk > c) --t;
-    const Tensor& e = tab.t[t];
-    const int64_t off = static_cast<int64_t>(c - e.first_chunk) * kChunk;
-    const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), e.numel - off));
+    if (first[t] > c) e = shadow->t[--t];
+    const Span sp = span_of(e, c - first[t], c + 1 == first[t + 1], kChunk);
+    const int64_t off = sp.off;
+    const int n = sp.n;
     if (e.in_type == GTK_F32)
-      scale_chunk(static_cast<const float*>(e.in) + off, static_cast<float*>(e.out) + off, n, k);
+      scale_chunk<float, float, kPer>(e.in, e.out, off, n, k);
     else if (e.in_type == GTK_BF16 && e.out_type == GTK_BF16)
-      scale_chunk(static_cast<const __nv_bfloat16*>(e.in) + off, static_cast<__nv_bfloat16*>(e.out) + off, n, k);
+      scale_chunk<__nv_bfloat16, __nv_bfloat16, kPer>(e.in, e.out, off, n, k);
     else if (e.in_type == GTK_BF16)
-      scale_chunk(static_cast<const __nv_bfloat16*>(e.in) + off, static_cast<float*>(e.out) + off, n, k);
+      scale_chunk<__nv_bfloat16, float, kPer>(e.in, e.out, off, n, k);
     else if (e.out_type == GTK_F16)
-      scale_chunk(static_cast<const __half*>(e.in) + off, static_cast<__half*>(e.out) + off, n, k);
+      scale_chunk<__half, __half, kPer>(e.in, e.out, off, n, k);
     else
-      scale_chunk(static_cast<const __half*>(e.in) + off, static_cast<float*>(e.out) + off, n, k);
+      scale_chunk<__half, float, kPer>(e.in, e.out, off, n, k);
   }
 }
 
@@ -250,64 +329,89 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 struct Request {
-  std::vector<Tensor> t;  // without the empty ones
+  std::vector<Tensor> t;       // without the empty ones; first_chunk and last_len not set
+  std::vector<int64_t> numel;
+  int64_t elements;
   bool inf_norm, in_place, scale;
   double max_norm;
   float* norm;
-  double* partial;
+  char* ws;
   cudaStream_t st;
 };
 
-int blocks_for(uint32_t chunks) {
-  const int cap = num_sms() * kBlocksPerSm < kMaxBlocks ? num_sms() * kBlocksPerSm : kMaxBlocks;
-  return static_cast<int>(chunks < static_cast<uint32_t>(cap) ? chunks : static_cast<uint32_t>(cap));
+// The workspace: kMaxBlocks partials and one shadow table per launch.
+size_t launches_for(int64_t n) { return static_cast<size_t>(n <= kMaxTensors ? 1 : (n + kMaxTensors - 1) / kMaxTensors); }
+size_t partial_bytes(int64_t n) { return round_up(sizeof(double) * kMaxBlocks * launches_for(n), 256); }
+size_t workspace_bytes(int64_t n) {
+  const size_t launches = launches_for(n);
+  const size_t last = sizeof(Tensor) * static_cast<size_t>(n - (launches - 1) * kMaxTensors);
+  return partial_bytes(n) + (launches - 1) * sizeof(Shadow) + round_up(last, 256);
 }
 
+struct Part {
+  int tensors, blocks;
+  uint32_t chunks, per;
+  Shadow* shadow;
+};
+
+// Coarse chunks from 40 M elements on, where they still give every block of the device four
+// (2^27 bf16 elements into fp32: 205 us, against 330 us in fine chunks; 8 M fp32 elements: no gain).
+bool coarse(int64_t elements) { return elements >= int64_t(40) * 1000 * 1000; }
+
+// The first kernel over the tensors [first, first + n).
 template <int N>
-void fill(Table<N>* tab, const Request& r, size_t first, size_t n) {
+int norm_part(const Request& r, size_t first, size_t n, int partials, Part* part) {
+  Table<N> tab;
+  const bool big = coarse(r.elements);
+  const int64_t chunk = kThreads * (big ? kCoarse : kFine);
   uint32_t chunks = 0;
   for (size_t i = 0; i < n; ++i) {
-    tab->t[i] = r.t[first + i];
-    tab->t[i].first_chunk = chunks;
-    chunks += static_cast<uint32_t>((r.t[first + i].numel + kChunk - 1) / kChunk);
+    tab.t[i] = r.t[first + i];
+    const int64_t lead = lead_of(tab.t[i].in, tab.t[i].in_type), numel = r.numel[first + i];
+    const int64_t m = (numel + lead + chunk - 1) / chunk;
+    tab.t[i].first_chunk = chunks;
+    tab.t[i].last_len = static_cast<uint16_t>(m == 1 ? numel : numel + lead - (m - 1) * chunk);
+    chunks += static_cast<uint32_t>(m);
   }
-  tab->n = static_cast<int>(n);
-  tab->chunks = chunks;
-  const uint32_t blocks = static_cast<uint32_t>(blocks_for(chunks));
-  tab->per = (chunks + blocks - 1) / blocks;
+  const int64_t cap = std::min<int64_t>(static_cast<int64_t>(num_sms()) * (big ? kCoarseBlocks : kFineBlocks),
+                                        kMaxBlocks);
+  const uint32_t blocks = chunks < cap ? chunks : static_cast<uint32_t>(cap);
+  tab.n = part->tensors = static_cast<int>(n);
+  tab.chunks = part->chunks = chunks;
+  tab.per = part->per = (chunks + blocks - 1) / blocks;
+  part->blocks = static_cast<int>((chunks + tab.per - 1) / tab.per);
+  return launch("gradient norm", big ? clip_norm_kernel<N, kCoarse> : clip_norm_kernel<N, kFine>, part->blocks,
+                kThreads, 0, r.st, false, tab, reinterpret_cast<double*>(r.ws) + partials,
+                r.scale ? part->shadow : nullptr, r.inf_norm);
 }
 
-// One launch over the tensors [first, first + n). `scale`: the second kernel, else the first.
-template <int N>
-int run_part(const Request& r, size_t first, size_t n, bool scale, bool write_norm, int* partials) {
-  Table<N> tab;
-  fill(&tab, r, first, n);
-  const int blocks = static_cast<int>((tab.chunks + tab.per - 1) / tab.per);
-  if (!scale) {
-    const int e = launch("gradient norm", clip_norm_kernel<N>, blocks, kThreads, 0, r.st, false, tab,
-                         r.partial + *partials, r.inf_norm);
-    *partials += blocks;
-    return e;
-  }
-  return launch("gradient clipping", clip_scale_kernel<N>, blocks, kThreads, 0, r.st, write_norm, tab,
-                static_cast<const double*>(r.partial), *partials, r.inf_norm, r.max_norm, r.in_place,
-                write_norm ? r.norm : static_cast<float*>(nullptr));
-}
-
-int run(const Request& r) {
+int run(const Request& r, int64_t n_given) {
+  const double* partial = reinterpret_cast<const double*>(r.ws);
+  Shadow* shadow = reinterpret_cast<Shadow*>(r.ws + partial_bytes(n_given));
+  const size_t launches = (r.t.size() + kMaxTensors - 1) / kMaxTensors;
+  std::vector<Part> parts(launches);
   int partials = 0;
-  for (int phase = 0; phase < (r.scale ? 2 : 1); ++phase)
-    for (size_t first = 0; first < r.t.size(); first += kMaxTensors) {
-      const size_t n = std::min<size_t>(kMaxTensors, r.t.size() - first);
-      // the table travels with every launch: 2, 8 or 32 KB of parameters, by the number of tensors
-      const int e = n <= 64    ? run_part<64>(r, first, n, phase, first == 0, &partials)
-                    : n <= 256 ? run_part<256>(r, first, n, phase, first == 0, &partials)
-                               : run_part<kMaxTensors>(r, first, n, phase, first == 0, &partials);
-      if (e) return e;
-    }
-  if (r.scale && !r.t.empty()) return GTK_OK;
-  return launch("gradient norm", norm_only_kernel, 1, kThreads, 0, r.st, !r.t.empty(),
-                static_cast<const double*>(r.partial), partials, r.inf_norm, r.norm);
+  for (size_t i = 0; i < launches; ++i) {
+    const size_t first = i * kMaxTensors, n = std::min<size_t>(kMaxTensors, r.t.size() - first);
+    parts[i].shadow = shadow + i;
+    // the launch copies its whole table, 1.5 to 24 KB: it takes the smallest that holds the tensors
+    const int e = n <= 64    ? norm_part<64>(r, first, n, partials, &parts[i])
+                  : n <= 256 ? norm_part<256>(r, first, n, partials, &parts[i])
+                  : n <= 512 ? norm_part<512>(r, first, n, partials, &parts[i])
+                             : norm_part<kMaxTensors>(r, first, n, partials, &parts[i]);
+    if (e) return e;
+    partials += parts[i].blocks;
+  }
+  if (!r.scale || r.t.empty())
+    return launch("gradient norm", norm_only_kernel, 1, kThreads, 0, r.st, !r.t.empty(), partial, partials,
+                  r.inf_norm, r.norm);
+  for (size_t i = 0; i < launches; ++i)
+    if (int e = launch("gradient clipping", coarse(r.elements) ? clip_scale_kernel<kCoarse> : clip_scale_kernel<kFine>, parts[i].blocks, kThreads, 0, r.st, i == 0,
+                       static_cast<const Shadow*>(parts[i].shadow), parts[i].tensors, parts[i].chunks, parts[i].per,
+                       partial, partials, r.inf_norm, r.max_norm, r.in_place,
+                       i == 0 ? r.norm : static_cast<float*>(nullptr)))
+      return e;
+  return GTK_OK;
 }
 
 struct Range {
@@ -349,8 +453,9 @@ int gather(const void* const* grads, void* const* outs, const int64_t* numel, co
     return fail(GTK_ERR_INVALID_ARG, "gradient norm: bad tensor list");
   std::vector<Range> in, out;
   r->t.reserve(n);
-  out.reserve(n);
-  if (outs) in.reserve(n);
+  r->numel.reserve(n);
+  if (r->scale) out.reserve(n);
+  if (r->scale && outs) in.reserve(n);
   for (int64_t i = 0; i < n; ++i) {
     if (numel[i] < 0 || numel[i] > (int64_t(1) << 40))
       return fail(GTK_ERR_INVALID_ARG, "gradient norm: bad size of tensor " + std::to_string(i));
@@ -364,24 +469,19 @@ int gather(const void* const* grads, void* const* outs, const int64_t* numel, co
     const uintptr_t a = reinterpret_cast<uintptr_t>(grads[i]), b = reinterpret_cast<uintptr_t>(o);
     if (a % dtype_bytes(dtypes[i]) || b % dtype_bytes(ot))
       return fail(GTK_ERR_ALIGNMENT, "gradient norm: tensor " + std::to_string(i) + " is misaligned");
-    r->t.push_back(Tensor{grads[i], o, numel[i], 0, static_cast<uint8_t>(dtypes[i]), static_cast<uint8_t>(ot)});
+    r->t.push_back(Tensor{grads[i], o, 0, 0, static_cast<uint8_t>(dtypes[i]), static_cast<uint8_t>(ot)});
+    r->numel.push_back(numel[i]);
+    r->elements += numel[i];
     if (!r->scale) continue;
     out.push_back(Range{b, b + numel[i] * dtype_bytes(ot), i});
     if (outs) in.push_back(Range{a, a + numel[i] * dtype_bytes(dtypes[i]), i});
   }
-  int64_t chunks = 0;
-  for (const Tensor& t : r->t) chunks += (t.numel + kChunk - 1) / kChunk;
-  if (chunks > (int64_t(1) << 31)) return fail(GTK_ERR_UNSUPPORTED, "gradient norm: too many elements");
+  if (r->elements > (int64_t(1) << 42)) return fail(GTK_ERR_UNSUPPORTED, "gradient norm: too many elements");
   if (r->scale && outputs_clash(std::move(in), std::move(out), !outs))
     return fail(GTK_ERR_INVALID_ARG,
                 outs ? "gradient clipping: outputs overlap one another or other gradients"
                      : "gradient clipping: the gradients overlap one another (the same tensor twice?)");
   return GTK_OK;
-}
-
-size_t workspace_bytes(int64_t n) {
-  const int64_t launches = (n + kMaxTensors - 1) / kMaxTensors;
-  return sizeof(double) * static_cast<size_t>(kMaxBlocks) * static_cast<size_t>(launches < 1 ? 1 : launches);
 }
 
 int start(const void* const* grads, void* const* outs, const int64_t* numel, const int* dtypes, const int* out_dtypes,
@@ -392,14 +492,14 @@ int start(const void* const* grads, void* const* outs, const int64_t* numel, con
   if (int e = gather(grads, outs, numel, dtypes, out_dtypes, n, r)) return e;
   if (int e = check_ptr(norm, "norm", 4)) return e;
   if (workspace_bytes_given < workspace_bytes(n)) return fail(GTK_ERR_WORKSPACE, "gradient norm: workspace too small");
-  if (int e = check_ptr(workspace, "workspace")) return e;
+  if (int e = check_ptr(workspace, "workspace", 256)) return e;
   if (int e = check_device()) return e;
   r->inf_norm = norm_kind == GTK_NORM_INF;
   r->in_place = !outs;
   r->norm = norm;
-  r->partial = static_cast<double*>(workspace);
+  r->ws = static_cast<char*>(workspace);
   r->st = static_cast<cudaStream_t>(stream);
-  return run(*r);
+  return run(*r, n);
 }
 
 }  // namespace clip

@@ -90,8 +90,7 @@ struct Row {
       if (valid && i < nv)
         e[k] = ld_vec<T, V>(p + static_cast<int64_t>(i) * V);
       else
-#pragma unroll
-        for (int j = 0; j < V; ++j) e[k].v[j] = Elem<T>::store(0.f);
+        e[k] = Vec<T, V>::zero();
     }
   }
 };
@@ -138,7 +137,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += Elem<T>::load(cur.e[k].v[j]);
+      for (int j = 0; j < V; ++j) s += cur.e[k].get(j);
     const float mean = (kBlock ? block_sum2(s, 0.f, red, half).x : group_sum(s, G)) * inv_d;
     float q = 0.f;
 #pragma unroll
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
       if (lane + G * k < nv)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float d = Elem<T>::load(cur.e[k].v[j]) - mean;
+          const float d = cur.e[k].get(j) - mean;
           q = fmaf(d, d, q);
         }
     const float var = (kBlock ? block_sum2(q, 0.f, red, half).x : group_sum(q, G)) * inv_d;
@@ -157,12 +156,10 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     for (int k = 0; k < K; ++k) {
       const int i = lane + G * k;
       if (i >= nv) continue;
-      Vec<T, V> o;
+      float o[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        o.v[j] = Elem<T>::store(
-            fmaf((Elem<T>::load(cur.e[k].v[j]) - mean) * rstd, wf[k * V + j], bf[k * V + j]));
-      st_vec<T, V>(yr + static_cast<int64_t>(i) * V, o);
+      for (int j = 0; j < V; ++j) o[j] = fmaf((cur.e[k].get(j) - mean) * rstd, wf[k * V + j], bf[k * V + j]);
+      st_vec<T, V>(yr + static_cast<int64_t>(i) * V, Vec<T, V>::of(o));
     }
     if (lane == 0) {
       mean_out[r64] = mean;
@@ -205,8 +202,8 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
       if (valid && lane + G * k < nv)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float d = Elem<T>::load(gr.e[k].v[j]);
-          const float xh = (Elem<T>::load(xr.e[k].v[j]) - mean) * rstd;
+          const float d = gr.e[k].get(j);
+          const float xh = (xr.e[k].get(j) - mean) * rstd;
           const float g = __fmul_rn(d, wf[k * V + j]);
           aw[k * V + j] = fmaf(d, xh, aw[k * V + j]);
           ab[k * V + j] += d;
@@ -227,14 +224,14 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     for (int k = 0; k < K; ++k) {
       const int i = lane + G * k;
       if (i >= nv) continue;
-      Vec<T, V> o;
+      float o[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = (Elem<T>::load(xr.e[k].v[j]) - mean) * rstd;
-        const float g = __fmul_rn(Elem<T>::load(gr.e[k].v[j]), wf[k * V + j]);
-        o.v[j] = Elem<T>::store(rstd * ((g - c1) - xh * c2));
+        const float xh = (xr.e[k].get(j) - mean) * rstd;
+        const float g = __fmul_rn(gr.e[k].get(j), wf[k * V + j]);
+        o[j] = rstd * ((g - c1) - xh * c2);
       }
-      st_vec<T, V>(dr + static_cast<int64_t>(i) * V, o);
+      st_vec<T, V>(dr + static_cast<int64_t>(i) * V, Vec<T, V>::of(o));
     }
   }
   if (!partial) return;

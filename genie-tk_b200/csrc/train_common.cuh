@@ -31,27 +31,111 @@ struct Elem<__half> {
   static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
 };
 
+// V elements of a vector load or store, kept as the words they come in (arrays of 16-bit classes
+// under predicates end up in local memory).
+template <int kBytes>
+struct Words;
+template <>
+struct Words<16> {
+  using type = uint4;
+  static __device__ __forceinline__ uint32_t get(const uint4& r, int i) {
+    return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+  }
+  static __device__ __forceinline__ uint4 make(const uint32_t (&w)[4]) { return make_uint4(w[0], w[1], w[2], w[3]); }
+};
+template <>
+struct Words<8> {
+  using type = uint2;
+  static __device__ __forceinline__ uint32_t get(const uint2& r, int i) { return i == 0 ? r.x : r.y; }
+  static __device__ __forceinline__ uint2 make(const uint32_t (&w)[2]) { return make_uint2(w[0], w[1]); }
+};
+template <>
+struct Words<4> {
+  using type = uint32_t;
+  static __device__ __forceinline__ uint32_t get(uint32_t r, int) { return r; }
+  static __device__ __forceinline__ uint32_t make(const uint32_t (&w)[1]) { return w[0]; }
+};
+template <>
+struct Words<2> {
+  using type = unsigned short;
+  static __device__ __forceinline__ uint32_t get(unsigned short r, int) { return r; }
+  static __device__ __forceinline__ unsigned short make(const uint32_t (&w)[1]) {
+    return static_cast<unsigned short>(w[0]);
+  }
+};
+
+// Two 16-bit elements of a word.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  static __device__ __forceinline__ uint32_t make(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float lo(uint32_t w) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xffffu)));
+  }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
+  }
+  static __device__ __forceinline__ uint32_t make(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T v[V];
+struct Vec {
+  using W = Words<static_cast<int>(sizeof(T)) * V>;
+  typename W::type r;
+  // Element j as fp32 (j is a constant wherever loops are unrolled).
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(W::get(r, j));
+    else
+      return (j & 1) ? Pair<T>::hi(W::get(r, j >> 1)) : Pair<T>::lo(W::get(r, j >> 1));
+  }
+  // Rounded from fp32.
+  static __device__ __forceinline__ Vec of(const float (&f)[V]) {
+    constexpr int kWords = (static_cast<int>(sizeof(T)) * V + 3) / 4;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4)
+        w[i] = __float_as_uint(f[i]);
+      else
+        w[i] = Pair<T>::make(f[(2 * i) % V], V > 1 ? f[(2 * i + 1) % V] : 0.f);
+    }
+    Vec v;
+    v.r = W::make(w);
+    return v;
+  }
+  static __device__ __forceinline__ Vec zero() {
+    const float f[V] = {};
+    return of(f);
+  }
 };
 
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> ld_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, V>*>(p);
+  Vec<T, V> v;
+  v.r = *reinterpret_cast<const typename Vec<T, V>::W::type*>(p);
+  return v;
 }
 template <typename T, int V>
 __device__ __forceinline__ void st_vec(T* p, const Vec<T, V>& v) {
-  *reinterpret_cast<Vec<T, V>*>(p) = v;
+  *reinterpret_cast<typename Vec<T, V>::W::type*>(p) = v.r;
 }
 
 // Waits until the kernel before this one on the stream has finished and its writes are
 // visible; at once when the launch carried no programmatic dependency.
 __device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next kernel of the stream be scheduled; it still waits for this one's end in
-// wait_previous_kernel().
-__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Launch on `st`; `after_previous`: the kernel may be set up while its predecessor on the
 // stream still runs. It must call wait_previous_kernel() before it touches memory.
 template <typename... KArgs, typename... Args>

@@ -247,9 +247,24 @@ struct Gradients {
   std::vector<std::pair<Tensor, Tensor>> write_back;  // (gradient, its clipped copy)
 };
 
-const Tensor& tensor_at(PyObject* o, const char* name, Py_ssize_t i) {
+// Element i of a list or tuple of tensors. (Reads the TensorImpl directly from here on: a list may
+// hold hundreds of gradients, and every call on a Tensor counts.)
+c10::TensorImpl* tensor_at(PyObject* seq, const char* name, Py_ssize_t i) {
+  PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
   if (!THPVariable_Check(o)) type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined()) type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
+  return t.unsafeGetTensorImpl();
+}
+
+Tensor handle(c10::TensorImpl* t) {
+  return Tensor(c10::intrusive_ptr<c10::TensorImpl, c10::UndefinedTensorImpl>::reclaim_copy(t));
+}
+
+bool dense(c10::TensorImpl* t) { return t->is_contiguous() || t->is_non_overlapping_and_dense(); }
+
+void written(c10::TensorImpl* t) {
+  if (!t->is_inference()) t->bump_version();
 }
 
 // Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
@@ -264,55 +279,52 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     if (!fast_out) throw py::error_already_set();
     if (PySequence_Fast_GET_SIZE(fast_out.ptr()) != n) value_error("out must have one tensor for each gradient");
   }
-  g->in.reserve(n);
-  g->numel.reserve(n);
-  g->in_type.reserve(n);
+  g->in.resize(n);
+  g->numel.resize(n);
+  g->in_type.resize(n);
   if (outs) {
-    g->out.reserve(n);
-    g->out_type.reserve(n);
+    g->out.resize(n);
+    g->out_type.resize(n);
   }
-  std::optional<c10::Device> device;
+  require_cuda(handle(tensor_at(fast.ptr(), "grads", 0)), "grads[0]");
+  const c10::Device device = tensor_at(fast.ptr(), "grads", 0)->device();
   for (Py_ssize_t i = 0; i < n; ++i) {
-    const Tensor& t = tensor_at(PySequence_Fast_GET_ITEM(fast.ptr(), i), "grads", i);
-    if (!device) {
-      require_cuda(t, "grads[0]");
-      device = t.device();
-    } else {
-      if (!t.is_cuda() || t.device() != *device)
-        throw std::runtime_error(kPrefix + "all gradients must be CUDA tensors on one device");
-      if (t.layout() != at::kStrided) type_error("gradients must be dense tensors");
-    }
-    const int code = code_of(t.scalar_type());
-    if (code < 0) type_error("gradients must be float32, bfloat16 or float16, got " + name_of(t.scalar_type()));
-    Tensor src = t;
+    c10::TensorImpl* t = tensor_at(fast.ptr(), "grads", i);
+    if (t->device() != device)
+      throw std::runtime_error(kPrefix + "all gradients must be CUDA tensors on one device");
+    if (t->layout() != at::kStrided) type_error("gradients must be dense tensors");
+    const at::ScalarType st = c10::typeMetaToScalarType(t->dtype());
+    const int code = code_of(st);
+    if (code < 0) type_error("gradients must be float32, bfloat16 or float16, got " + name_of(st));
     if (outs) {
-      const Tensor& o = tensor_at(PySequence_Fast_GET_ITEM(fast_out.ptr(), i), "out", i);
-      if (!o.is_cuda() || o.device() != *device || o.layout() != at::kStrided)
+      c10::TensorImpl* o = tensor_at(fast_out.ptr(), "out", i);
+      if (o->device() != device || o->layout() != at::kStrided)
         throw std::runtime_error(kPrefix + "out must hold dense CUDA tensors on the gradients' device");
-      if (o.sizes() != t.sizes()) value_error("out[" + std::to_string(i) + "] must have its gradient's shape");
-      if (o.scalar_type() != at::kFloat && o.scalar_type() != t.scalar_type())
-        type_error("out must be float32 or the gradient's type, got " + name_of(o.scalar_type()));
-      if (!(t.is_contiguous() && o.is_contiguous()) &&
-          !(t.is_non_overlapping_and_dense() && t.strides() == o.strides())) {
-        if (!o.is_contiguous()) value_error("out[" + std::to_string(i) + "] must be contiguous");
-        src = t.contiguous();
-        g->keep.push_back(src);
+      if (o->sizes() != t->sizes()) value_error("out[" + std::to_string(i) + "] must have its gradient's shape");
+      const at::ScalarType ot = c10::typeMetaToScalarType(o->dtype());
+      if (ot != at::kFloat && ot != st)
+        type_error("out must be float32 or the gradient's type, got " + name_of(ot));
+      const bool alike = (t->is_contiguous() && o->is_contiguous()) ||
+                         (t->is_non_overlapping_and_dense() && t->strides() == o->strides());
+      if (!alike) {
+        if (!o->is_contiguous()) value_error("out[" + std::to_string(i) + "] must be contiguous");
+        g->keep.push_back(handle(t).contiguous());
+        t = g->keep.back().unsafeGetTensorImpl();
       }
-      g->out.push_back(o.data_ptr());
-      g->out_type.push_back(code_of(o.scalar_type()));
-      if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
-    } else if (!t.is_contiguous() && !t.is_non_overlapping_and_dense()) {
-      src = t.contiguous();
-      g->keep.push_back(src);
-      if (clip) g->write_back.emplace_back(t, src);
-    } else if (clip && !t.is_inference()) {
-      t.unsafeGetTensorImpl()->bump_version();
+      g->out[i] = o->mutable_data();
+      g->out_type[i] = code_of(ot);
+    } else if (!dense(t)) {
+      g->keep.push_back(handle(t).contiguous());
+      if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
+      t = g->keep.back().unsafeGetTensorImpl();
     }
-    g->in.push_back(src.data_ptr());
-    g->numel.push_back(src.numel());
-    g->in_type.push_back(code);
+    g->in[i] = t->data();
+    g->numel[i] = t->numel();
+    g->in_type[i] = code;
   }
-  return *device;
+  // only now, when nothing is refused any more: what is written counts as written
+  for (Py_ssize_t i = 0; clip && i < n; ++i) written(tensor_at(outs ? fast_out.ptr() : fast.ptr(), "grads", i));
+  return device;
 }
 
 int norm_kind(double norm_type) {
