@@ -11,16 +11,29 @@
 // once, at its store. The variance is the sum of squared deviations from the finished mean
 // (not E[x^2] - mean^2, which cancels), so a row is held in registers and reduced twice.
 //
-// g is rounded to fp32 before it enters dx as it is before it enters its mean (__fmul_rn keeps
-// the compiler from fusing the product into g - mean(g)), so that what cancels in the formula
-// cancels here: rows of one element have dx = 0.
+// g is rounded to fp32 before it enters dx as it is before it enters its mean (a product fused
+// into g - mean(g) is not), so that what cancels in the formula cancels here: rows of one
+// element have dx = 0.
 //
-// What bounds it: HBM. The forward reads x and writes y once, the backward reads x and dy and
-// writes dx once. A group of G threads owns a row and keeps 16 (D <= 8192) or 32 (D <= 16384)
-// of its elements per thread in registers: up to 32 threads the reductions are shuffles,
-// beyond that the group is the block and they go through shared memory. 16 elements per
-// thread make few shuffle steps per element (D = 128: 8 threads, 3 steps). Wider rows take
-// the loop kernels, which read a row again for each reduction.
+// What bounds it: HBM, and for 16-bit rows nearly as much the instructions per element, which are
+// therefore done for pairs of elements where fp32 allows (add2, mul2, fma2). The forward reads x and
+// writes y once, the backward reads x and dy and writes dx once. A group of G threads owns a row,
+// 16 of its elements per thread (32 from D = 8193 on, up to 16384): up to 32 threads the reductions
+// are shuffles, beyond that the group is the block, they go through shared memory, and two rows
+// share each barrier. 16 elements per thread make few shuffle steps per element (D = 128: 8 threads,
+// 3 steps). The rows that follow are on their way meanwhile: every thread copies its own elements
+// of the next rows to a ring in shared memory (cp.async), which takes no registers and, as nobody
+// else reads them, no barriers. Wider rows take the loop kernels, which read a row again for
+// each reduction.
+//
+// Widths that no 16-byte vector divides: rows then begin at different places of a vector, but all
+// rows of one group at the same place, because the groups step by a multiple of eight rows. The
+// group's vectors are laid over its rows from the boundary before them (`lead` elements earlier),
+// and only the first and the last vector of a row are looked at by element.
+//
+// Rows of a transposed pair tensor lie far apart in one axis and next to one another in the other.
+// They are visited in tiles of 8 x 4, which reads runs of eight rows and writes runs of four
+// (in plain order, the backward of 512 x 512 x 128 fp32 took 82 us instead of 70).
 //
 // dw and db: a thread meets the same columns in every row of its group, so it sums them in
 // registers over all the group's rows; the block's groups are then joined in shared memory,
@@ -36,8 +49,9 @@ namespace ln {
 constexpr int kMaxWidth = 1 << 20;
 constexpr int kGroupThreads = 256;  // block of the kernels whose groups are at most a warp
 constexpr int kMaxBlockGroup = 512;
-constexpr int kJoinCols = 32;
 constexpr int kJoinThreads = 1024;
+constexpr int kMaxStages = 4;             // rows of the ring
+constexpr int kRingBytes = 200 * 1024;    // of an SM
 
 // Where row r of a tensor with up to three leading axes begins: r = (a n1 + b) n2 + c lies
 // at a s0 + b s1 + c s2 (element strides); n1 = n2 = 0: rows follow one another, s2 apart.
@@ -53,185 +67,445 @@ __device__ __forceinline__ int64_t row_offset(const RowMap& m, uint32_t r) {
   return a * m.s0 + b * m.s1 + c * m.s2;
 }
 
-// Sum over the group: G <= 32 lanes of a warp.
-__device__ __forceinline__ float group_sum(float v, int G) {
-  for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// The order in which rows are visited: as they come (n1 = 0), or the n1 x n2 planes of rows in
+// tiles of 8 x 4, t1 x t2 of them (the last ones in part outside). `visits` counts places.
+struct Order {
+  uint32_t n1, n2, t1, t2;
+  uint64_t visits;
+};
+constexpr uint32_t kNoRow = 0xffffffffu;
+
+__device__ __forceinline__ uint32_t row_at(const Order& o, uint64_t v) {
+  if (v >= o.visits) return kNoRow;
+  if (o.n1 == 0) return static_cast<uint32_t>(v);
+  const uint32_t tile = static_cast<uint32_t>(v >> 5), t = tile / o.t2, a = t / o.t1;
+  const uint32_t b = (t - a * o.t1) * 8 + (static_cast<uint32_t>(v) & 7u);
+  const uint32_t c = (tile - t * o.t2) * 4 + (static_cast<uint32_t>(v >> 3) & 3u);
+  return b < o.n1 && c < o.n2 ? (a * o.n1 + b) * o.n2 + c : kNoRow;
 }
 
-// Sums of two values over the block (at most 16 warps); `buf` alternates between two halves,
-// so that one barrier per reduction is enough.
-__device__ __forceinline__ float2 block_sum2(float a, float b, float2* buf, int& half) {
+// Sums over a group of G <= 32 lanes of a warp.
+template <int n>
+__device__ __forceinline__ void group_sum(float (&v)[n], int G) {
+  for (int o = G >> 1; o > 0; o >>= 1)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
+    for (int i = 0; i < n; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+}
+
+// Sums of n = 1, 2 or 4 values over the block (at most 16 warps). The values are spread over the
+// lanes as they are added up, 5 or 6 shuffles for all of them. `buf` alternates between two
+// halves, so that one barrier per reduction is enough.
+template <int n>
+__device__ __forceinline__ void block_sum(float (&v)[n], float* buf, int& half) {
+  const int lane = threadIdx.x & 31;
+  float x;
+  if constexpr (n == 4) {
+    const bool hi = lane & 16;
+    const float a = (hi ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16);
+    const float b = (hi ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16);
+    const bool up = lane & 8;
+    x = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
+  } else if constexpr (n == 2) {
+    const bool hi = lane & 16;
+    x = (hi ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[1], 16);
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+  } else {
+    x = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
   }
-  float2* s = buf + 16 * half;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  float* s = buf + 64 * half;
   half ^= 1;
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = make_float2(a, b);
+  constexpr int kEach = 32 / n;  // lanes that hold one value
+  if (lane % kEach == 0) s[(threadIdx.x >> 5) * n + lane / kEach] = x;
   __syncthreads();
   const int nw = blockDim.x >> 5;
-  float2 t = s[0];
-  for (int i = 1; i < nw; ++i) {
-    t.x += s[i].x;
-    t.y += s[i].y;
+#pragma unroll
+  for (int i = 0; i < n; ++i) v[i] = 0.f;
+#pragma unroll 4
+  for (int w = 0; w < nw; ++w) {
+    if constexpr (n == 4) {
+      const float4 t = reinterpret_cast<const float4*>(s)[w];
+      v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+    } else if constexpr (n == 2) {
+      const float2 t = reinterpret_cast<const float2*>(s)[w];
+      v[0] += t.x, v[1] += t.y;
+    } else {
+      v[0] += s[w];
+    }
   }
-  return t;
 }
 
+// How a group's vectors lie over its rows: vector i covers the columns i V - lead .. + V - 1.
+struct Lay {
+  int lane, G, nv, lead, D;
+};
+
+// A thread's elements of a row: K vectors of V at vector indices lane + G k < nv. Vectors come
+// through a ring slot in shared memory ([k][thread], 16 bytes each; slots of vectors that do not
+// exist hold zeros from the start); single elements (V = 1: rows that begin anywhere) through
+// registers, without a row ahead.
 template <typename T, int V, int K>
 struct Row {
-  Vec<T, V> e[K];
-  __device__ __forceinline__ void load(const T* p, int lane, int G, int nv, bool valid) {
+  static constexpr bool kAsync = V > 1;
+  static constexpr int kBytes = 16;
+  Vec<T, V> e[kAsync ? 1 : K];
+  const char* slot;
+  int pitch;
+
+  // `p`: the row's first element. The last vector reads no further than the row; the first one
+  // begins with up to V - 1 elements of the row before.
+  static __device__ __forceinline__ void request(char* slot, int pitch, const T* p, const Lay& l) {
+    if constexpr (kAsync) {
+      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
+      const T* from = p - l.lead + l.lane * V;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = lane + G * k;
-      if (valid && i < nv)
-        e[k] = ld_vec<T, V>(p + static_cast<int64_t>(i) * V);
-      else
-        e[k] = Vec<T, V>::zero();
+      for (int k = 0; k < K; ++k) {
+        const int i = l.lane + l.G * k;
+        if (i >= l.nv) continue;
+        const int left = (l.lead + l.D - i * V) * static_cast<int>(sizeof(T));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * pitch),
+                     "l"(from + static_cast<int64_t>(l.G) * k * V), "r"(left < 16 ? left : 16)
+                     : "memory");
+      }
+    }
+  }
+  // What was requested (kAsync), or now.
+  __device__ __forceinline__ void open(const char* s, int pt, const T* p, const Lay& l) {
+    if constexpr (kAsync) {
+      slot = s;
+      pitch = pt;
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int i = l.lane + l.G * k;
+        e[k] = i < l.nv ? ld_vec<T, V>(p + i) : Vec<T, V>::zero();
+      }
+    }
+  }
+  // Vector k; elements before the row are zeros.
+  __device__ __forceinline__ Vec<T, V> vec(int k, const Lay& l) const {
+    if constexpr (!kAsync) return e[k];
+    Vec<T, V> v = ld_vec<T, V>(reinterpret_cast<const T*>(slot + k * pitch));
+    if (k == 0 && l.lead > l.lane * V) {
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = j < l.lead ? 0.f : v.get(j);
+      v = Vec<T, V>::of(f);
+    }
+    return v;
+  }
+  // The thread's elements in pairs: 2 p and 2 p + 1.
+  __device__ __forceinline__ void pairs(float2 (&out)[K * V / 2], const Lay& l) const {
+    if constexpr (V == 1) {
+#pragma unroll
+      for (int p = 0; p < K / 2; ++p) out[p] = make_float2(e[2 * p].get(0), e[2 * p + 1].get(0));
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const Vec<T, V> v = vec(k, l);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) out[k * (V / 2) + j] = make_float2(v.get(2 * j), v.get(2 * j + 1));
+      }
     }
   }
 };
 
-// Parameters of the thread's columns as floats; `other` where there is none.
-template <typename W, int V, int K>
-__device__ __forceinline__ void load_columns(float (&out)[K * V], const W* w, int lane, int G, int D, float other) {
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (lane + G * k) * V + j;
-      out[k * V + j] = (w && c < D) ? Elem<W>::load(w[c]) : other;
-    }
-}
-
-// Forward. kBlock: the block is one group of blockDim.x threads; else groups of G <= 32.
-template <typename T, typename W, int V, int K, bool kBlock>
-__global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
-    forward_kernel(const T* __restrict__ x, RowMap xm, const W* __restrict__ w, const W* __restrict__ b,
-                   T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, uint32_t rows,
-                   int D, int G, float eps) {
-  __shared__ float2 red[32];
-  int half = 0;
-  const int lane = kBlock ? threadIdx.x : (threadIdx.x & (G - 1));
-  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
-  const uint32_t first = kBlock ? blockIdx.x : blockIdx.x * per_block + threadIdx.x / G;
-  const uint32_t step = gridDim.x * per_block;
-  const int nv = D / V;
-  const float inv_d = 1.0f / static_cast<float>(D);
-  float wf[K * V], bf[K * V];
-  load_columns<W, V, K>(wf, w, lane, G, D, 1.f);
-  load_columns<W, V, K>(bf, b, lane, G, D, 0.f);
-  Row<T, V, K> next;
-  next.load(x + (first < rows ? row_offset(xm, first) : 0), lane, G, nv, first < rows);
-  // every group of the block makes the same number of turns, so that shuffles and barriers meet
-  const uint32_t block_first = kBlock ? first : blockIdx.x * per_block;
-  for (uint64_t base = block_first, r64 = first; base < rows; base += step, r64 += step) {
-    const bool valid = r64 < rows;
-    Row<T, V, K> cur = next;
-    const bool more = r64 + step < rows;
-    next.load(x + (more ? row_offset(xm, static_cast<uint32_t>(r64 + step)) : 0), lane, G, nv, more);
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) s += cur.e[k].get(j);
-    const float mean = (kBlock ? block_sum2(s, 0.f, red, half).x : group_sum(s, G)) * inv_d;
-    float q = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (lane + G * k < nv)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = cur.e[k].get(j) - mean;
-          q = fmaf(d, d, q);
-        }
-    const float var = (kBlock ? block_sum2(q, 0.f, red, half).x : group_sum(q, G)) * inv_d;
-    const float rstd = 1.0f / sqrtf(var + eps);
-    if (!valid) continue;
-    T* yr = y + static_cast<int64_t>(r64) * D;
+// Stores the thread's elements of a row; the first and last vector by element where the row
+// begins or ends inside.
+template <typename T, int V, int K>
+__device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], const Lay& l) {
+  if constexpr (V == 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int i = lane + G * k;
-      if (i >= nv) continue;
+      const int c = l.lane + l.G * k;
+      if (c < l.D) p[c] = Elem<T>::store(k & 1 ? f[k / 2].y : f[k / 2].x);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = l.lane + l.G * k, c = i * V - l.lead;
+      if (i >= l.nv) continue;
       float o[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = fmaf((cur.e[k].get(j) - mean) * rstd, wf[k * V + j], bf[k * V + j]);
-      st_vec<T, V>(yr + static_cast<int64_t>(i) * V, Vec<T, V>::of(o));
-    }
-    if (lane == 0) {
-      mean_out[r64] = mean;
-      rstd_out[r64] = rstd;
+      for (int j = 0; j < V / 2; ++j) o[2 * j] = f[k * (V / 2) + j].x, o[2 * j + 1] = f[k * (V / 2) + j].y;
+      if (c >= 0 && c + V <= l.D) {
+        st_vec<T, V>(p + c, Vec<T, V>::of(o));
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j >= 0 && c + j < l.D) p[c + j] = Elem<T>::store(o[j]);
+      }
     }
   }
 }
 
-// Backward: dx and, per block, one partial row [dw | db] of 2 D floats.
-template <typename T, typename W, int V, int K, bool kBlock>
-__global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
-    backward_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm,
-                    const W* __restrict__ w, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-                    T* __restrict__ dx, float* __restrict__ partial, uint32_t rows, int D, int G) {
-  extern __shared__ float cols[];  // groups of a warp or less: [2][D]
-  __shared__ float2 red[32];
-  int half = 0;
-  const int lane = kBlock ? threadIdx.x : (threadIdx.x & (G - 1));
-  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
-  const uint32_t first = kBlock ? blockIdx.x : blockIdx.x * per_block + threadIdx.x / G;
-  const uint32_t step = gridDim.x * per_block;
-  const int nv = D / V;
-  const float inv_d = 1.0f / static_cast<float>(D);
-  float wf[K * V], aw[K * V], ab[K * V];
-  load_columns<W, V, K>(wf, w, lane, G, D, 1.f);
+// The column of the thread's element e (0 .. K V - 1); negative or >= D where there is none.
+template <int V>
+__device__ __forceinline__ int column_of(int e, const Lay& l) {
+  return (l.lane + l.G * (e / V)) * V - l.lead + e % V;
+}
+
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the newest `stages` - 1 groups of this thread's copies have arrived.
+__device__ __forceinline__ void wait_copies(int stages) {
+  if (stages >= 4)
+    asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (stages == 3)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (stages == 2)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// The thread's columns of a parameter in pairs: kept in registers with 16 elements per thread,
+// read again for every row (from the L1 cache) with 32.
+template <typename W, int V, int K>
+struct Columns {
+  static constexpr bool kKeep = V * K <= 16;
+  float2 f[kKeep ? V * K / 2 : 1];
+  const W* w;
+  float other;
+  __device__ __forceinline__ float element(int e, const Lay& l) const {
+    const int c = column_of<V>(e, l);
+    return w && c >= 0 && c < l.D ? Elem<W>::load(w[c]) : other;
+  }
+  __device__ __forceinline__ Columns(const W* p, float absent, const Lay& l) : w(p), other(absent) {
+    if constexpr (kKeep) {
 #pragma unroll
-  for (int i = 0; i < K * V; ++i) aw[i] = ab[i] = 0.f;
-  const uint32_t block_first = kBlock ? first : blockIdx.x * per_block;
-  for (uint64_t base = block_first, r64 = first; base < rows; base += step, r64 += step) {
-    const bool valid = r64 < rows;
-    const uint32_t r = valid ? static_cast<uint32_t>(r64) : 0u;
-    Row<T, V, K> xr, gr;
-    xr.load(x + row_offset(xm, r), lane, G, nv, valid);
-    gr.load(dy + row_offset(dm, r), lane, G, nv, valid);
-    const float mean = valid ? __ldg(mean_in + r) : 0.f;
-    const float rstd = valid ? __ldg(rstd_in + r) : 0.f;
-    float c1 = 0.f, c2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (valid && lane + G * k < nv)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = gr.e[k].get(j);
-          const float xh = (xr.e[k].get(j) - mean) * rstd;
-          const float g = __fmul_rn(d, wf[k * V + j]);
-          aw[k * V + j] = fmaf(d, xh, aw[k * V + j]);
-          ab[k * V + j] += d;
-          c1 += g;
-          c2 = fmaf(g, xh, c2);
-        }
-    if (kBlock) {
-      const float2 t = block_sum2(c1, c2, red, half);
-      c1 = t.x * inv_d;
-      c2 = t.y * inv_d;
-    } else {
-      c1 = group_sum(c1, G) * inv_d;
-      c2 = group_sum(c2, G) * inv_d;
+      for (int i = 0; i < V * K / 2; ++i) f[i] = make_float2(element(2 * i, l), element(2 * i + 1, l));
     }
-    if (!valid) continue;
-    T* dr = dx + static_cast<int64_t>(r64) * D;
+  }
+  __device__ __forceinline__ float2 get(int i, const Lay& l) const {
+    if constexpr (kKeep) return f[i];
+    return make_float2(element(2 * i, l), element(2 * i + 1, l));
+  }
+};
+
+__device__ __forceinline__ void zero_ring(char* ring, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+    *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+
+// Forward. kBlock: the block is one group of blockDim.x threads; else groups of G <= 32. A turn of
+// the loop takes N rows of each group.
+template <typename T, typename W, int V, int K, bool kBlock, int N>
+__global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
+    forward_kernel(const T* __restrict__ x, RowMap xm, Order order, const W* __restrict__ w,
+                   const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean_out,
+                   float* __restrict__ rstd_out, int D, int G, int stages, float eps) {
+  extern __shared__ __align__(16) char ring[];
+  __shared__ __align__(16) float red[128];
+  using R = Row<T, V, K>;
+  constexpr int P = K * V / 2;
+  int half = 0;
+  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
+  const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
+  const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
+  const int lead = static_cast<int>(first * D & (V - 1));
+  const Lay l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+                 (lead + D + V - 1) / V, lead, D};
+  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch;
+  char* mine = ring + threadIdx.x * R::kBytes;
+  const float inv_d = 1.0f / static_cast<float>(D);
+  if constexpr (R::kAsync) zero_ring(ring, stages * N * row_bytes);
+  const Columns<W, V, K> wc(w, 1.f, l), bc(b, 0.f, l);
+  auto request = [&](int s, uint64_t v) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = lane + G * k;
-      if (i >= nv) continue;
-      float o[V];
+    for (int q = 0; q < N; ++q) {
+      const uint32_t r = row_at(order, v + q * step);
+      if (r != kNoRow) R::request(mine + (s * N + q) * row_bytes, pitch, x + row_offset(xm, r), l);
+    }
+    commit_copies();
+  };
+  if constexpr (R::kAsync)
+    for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+  int now = 0;
+  // every group of the block makes the same number of turns, so that shuffles and barriers meet
+  for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
+    if constexpr (R::kAsync) {
+      request(now ? now - 1 : stages - 1, v0 + (stages - 1) * (N * step));
+      wait_copies(stages);
+    }
+    uint32_t r[N];
+    float2 v[N][P];
+    float s[N], sq[N];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xh = (xr.e[k].get(j) - mean) * rstd;
-        const float g = __fmul_rn(gr.e[k].get(j), wf[k * V + j]);
-        o[j] = rstd * ((g - c1) - xh * c2);
+    for (int q = 0; q < N; ++q) {
+      r[q] = row_at(order, v0 + q * step);
+      Lay lq = l;
+      if (r[q] == kNoRow) lq.nv = 0;
+      R row;
+      row.open(mine + (now * N + q) * row_bytes, pitch, x + row_offset(xm, r[q] == kNoRow ? 0u : r[q]), lq);
+      row.pairs(v[q], l);
+      float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < P; ++p) t = add2(t, v[q][p]);
+      s[q] = t.x + t.y;
+    }
+    now = now + 1 < stages ? now + 1 : 0;
+    if constexpr (kBlock)
+      block_sum<N>(s, red, half);
+    else
+      group_sum<N>(s, G);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      s[q] *= inv_d;
+      float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        v[q][p] = add2(v[q][p], both(-s[q]));
+        if constexpr (V == 1) {  // elements that do not exist have no deviation
+          if (column_of<V>(2 * p, l) >= D) v[q][p].x = 0.f;
+          if (column_of<V>(2 * p + 1, l) >= D) v[q][p].y = 0.f;
+        } else {
+          const int c = column_of<V>(2 * p / V * V, l);
+          if (c < 0 || c + V > D) {
+            const int c2 = column_of<V>(2 * p, l);
+            if (c2 < 0 || c2 >= D) v[q][p].x = 0.f;
+            if (c2 + 1 < 0 || c2 + 1 >= D) v[q][p].y = 0.f;
+          }
+        }
+        t = fma2(v[q][p], v[q][p], t);
       }
-      st_vec<T, V>(dr + static_cast<int64_t>(i) * V, Vec<T, V>::of(o));
+      sq[q] = t.x + t.y;
+    }
+    if constexpr (kBlock)
+      block_sum<N>(sq, red, half);
+    else
+      group_sum<N>(sq, G);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      if (r[q] == kNoRow) continue;
+      const float rstd = 1.0f / sqrtf(sq[q] * inv_d + eps);
+#pragma unroll
+      for (int p = 0; p < P; ++p) v[q][p] = fma2(mul2(v[q][p], both(rstd)), wc.get(p, l), bc.get(p, l));
+      store_row<T, V, K>(y + static_cast<int64_t>(r[q]) * D, v[q], l);
+      if (l.lane == 0) {
+        mean_out[r[q]] = s[q];
+        rstd_out[r[q]] = rstd;
+      }
+    }
+  }
+}
+
+// Backward: dx and, per block, one partial row [dw | db] of 2 D floats. The ring's stage holds N
+// x rows, N dy rows and, for each warp (group, where that is smaller), their mean and rstd.
+template <typename T, typename W, int V, int K, bool kBlock, int N>
+__global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBlock ? 1 : 2)
+    backward_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm, Order order,
+                    const W* __restrict__ w, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                    T* __restrict__ dx, float* __restrict__ partial, int D, int G, int stages) {
+  extern __shared__ __align__(16) char ring[];
+  __shared__ __align__(16) float red[128];
+  using R = Row<T, V, K>;
+  constexpr int P = K * V / 2;
+  int half = 0;
+  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
+  const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
+  const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
+  const int lead = static_cast<int>(first * D & (V - 1));
+  const Lay l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+                 (lead + D + V - 1) / V, lead, D};
+  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch, stage_bytes = 2 * N * row_bytes;
+  const int share = kBlock ? 32 : G;  // threads that share a copy of the statistics
+  char* mine = ring + threadIdx.x * R::kBytes;
+  float* stats = reinterpret_cast<float*>(ring + stages * stage_bytes) + threadIdx.x / share * 2 * N;
+  const int stats_stage = blockDim.x / share * 2 * N;
+  const float inv_d = 1.0f / static_cast<float>(D);
+  if constexpr (R::kAsync) zero_ring(ring, stages * stage_bytes);
+  const Columns<W, V, K> wc(w, 1.f, l);
+  float2 aw[P], ab[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) aw[p] = ab[p] = make_float2(0.f, 0.f);
+  auto request = [&](int s, uint64_t v) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const uint32_t r = row_at(order, v + q * step);
+      if (r == kNoRow) continue;
+      char* to = mine + s * stage_bytes + 2 * q * row_bytes;
+      R::request(to, pitch, x + row_offset(xm, r), l);
+      R::request(to + row_bytes, pitch, dy + row_offset(dm, r), l);
+      if (threadIdx.x % share == 0) {
+        const uint32_t st = static_cast<uint32_t>(__cvta_generic_to_shared(stats + s * stats_stage + 2 * q));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st), "l"(mean_in + r) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + 4), "l"(rstd_in + r) : "memory");
+      }
+    }
+    commit_copies();
+  };
+  if constexpr (R::kAsync)
+    for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+  int now = 0;
+  for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
+    if constexpr (R::kAsync) {
+      request(now ? now - 1 : stages - 1, v0 + (stages - 1) * (N * step));
+      wait_copies(stages);
+      __syncwarp();  // the statistics come from the first lane's copies
+    }
+    uint32_t r[N];
+    R xr[N], gr[N];
+    float mean[N], rstd[N], c[2 * N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      r[q] = row_at(order, v0 + q * step);
+      const bool valid = r[q] != kNoRow;
+      Lay lq = l;
+      if (!valid) lq.nv = 0;
+      mean[q] = rstd[q] = 0.f;
+      if constexpr (R::kAsync) {
+        if (valid) {
+          mean[q] = stats[now * stats_stage + 2 * q];
+          rstd[q] = stats[now * stats_stage + 2 * q + 1];
+        }
+      } else if (valid) {
+        mean[q] = __ldg(mean_in + r[q]);
+        rstd[q] = __ldg(rstd_in + r[q]);
+      }
+      const char* slot = mine + now * stage_bytes + 2 * q * row_bytes;
+      xr[q].open(slot, pitch, x + row_offset(xm, valid ? r[q] : 0u), lq);
+      gr[q].open(slot + row_bytes, pitch, dy + row_offset(dm, valid ? r[q] : 0u), lq);
+      c[2 * q] = c[2 * q + 1] = 0.f;
+      if (!valid) continue;
+      float2 xp[P], gp[P], c1 = make_float2(0.f, 0.f), c2 = c1;
+      xr[q].pairs(xp, l);
+      gr[q].pairs(gp, l);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const float2 xh = mul2(add2(xp[p], both(-mean[q])), both(rstd[q]));
+        const float2 g = mul2(gp[p], wc.get(p, l));
+        aw[p] = fma2(gp[p], xh, aw[p]);
+        ab[p] = add2(ab[p], gp[p]);
+        c1 = add2(c1, g);
+        c2 = fma2(g, xh, c2);
+      }
+      c[2 * q] = c1.x + c1.y;
+      c[2 * q + 1] = c2.x + c2.y;
+    }
+    now = now + 1 < stages ? now + 1 : 0;
+    if constexpr (kBlock)
+      block_sum<2 * N>(c, red, half);
+    else
+      group_sum<2 * N>(c, G);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      if (r[q] == kNoRow) continue;
+      const float c1 = c[2 * q] * inv_d, c2 = c[2 * q + 1] * inv_d;
+      float2 xp[P], gp[P];
+      xr[q].pairs(xp, l);
+      gr[q].pairs(gp, l);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const float2 xh = mul2(add2(xp[p], both(-mean[q])), both(rstd[q]));
+        const float2 g = rounded_mul2(gp[p], wc.get(p, l));
+        xp[p] = mul2(both(rstd[q]), fma2(xh, both(-c2), add2(g, both(-c1))));
+      }
+      store_row<T, V, K>(dx + static_cast<int64_t>(r[q]) * D, xp, l);
     }
   }
   if (!partial) return;
@@ -239,86 +513,104 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
   float* pb = pw + D;
   if (kBlock) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (lane + G * k < nv)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = (lane + G * k) * V + j;
-          pw[c] = aw[k * V + j];
-          pb[c] = ab[k * V + j];
-        }
+    for (int e = 0; e < K * V; ++e) {
+      const int col = column_of<V>(e, l);
+      if (col < 0 || col >= D) continue;
+      pw[col] = e & 1 ? aw[e / 2].y : aw[e / 2].x;
+      pb[col] = e & 1 ? ab[e / 2].y : ab[e / 2].x;
+    }
     return;
   }
-  // the warp's groups by shuffles, then the warps one after another in shared memory
+  // the groups one after another in the ring's memory; groups that lie alike are added in the
+  // warp first (with a lead, the groups of a warp lie differently)
+  wait_copies(1);
+  const bool alike = D % V == 0;
+  if (alike)
 #pragma unroll
-  for (int i = 0; i < K * V; ++i)
-    for (int o = G; o < 32; o <<= 1) {
-      aw[i] += __shfl_xor_sync(0xffffffffu, aw[i], o);
-      ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], o);
-    }
-  const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  for (int t = 0; t < nw; ++t) {
-    if (warp == t && (threadIdx.x & 31) < G)
+    for (int p = 0; p < P; ++p)
+      for (int o = G; o < 32; o <<= 1) {
+        aw[p].x += __shfl_xor_sync(0xffffffffu, aw[p].x, o);
+        aw[p].y += __shfl_xor_sync(0xffffffffu, aw[p].y, o);
+        ab[p].x += __shfl_xor_sync(0xffffffffu, ab[p].x, o);
+        ab[p].y += __shfl_xor_sync(0xffffffffu, ab[p].y, o);
+      }
+  __syncthreads();
+  float* cols = reinterpret_cast<float*>(ring);  // [2][D]
+  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) cols[i] = 0.f;
+  __syncthreads();
+  const int unit = alike ? 32 : G;  // threads that add at once
+  for (int t = 0; t < static_cast<int>(blockDim.x) / unit; ++t) {
+    if (static_cast<int>(threadIdx.x) / unit == t && static_cast<int>(threadIdx.x) % unit < G)
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (lane + G * k < nv)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int c = (lane + G * k) * V + j;
-            cols[c] = (t ? cols[c] : 0.f) + aw[k * V + j];
-            cols[D + c] = (t ? cols[D + c] : 0.f) + ab[k * V + j];
-          }
+      for (int e = 0; e < K * V; ++e) {
+        const int col = column_of<V>(e, l);
+        if (col < 0 || col >= D) continue;
+        cols[col] += e & 1 ? aw[e / 2].y : aw[e / 2].x;
+        cols[D + col] += e & 1 ? ab[e / 2].y : ab[e / 2].x;
+      }
     __syncthreads();
   }
-  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) pw[c] = cols[c];
+  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) pw[i] = cols[i];
 }
 
-// dw, db: the sum of `n` partial rows of 2 D floats, in a fixed order (64 bits across warps).
-template <typename W>
+// dw, db: the sum of `n` partial rows of 2 D floats, in a fixed order and 64 bits. A warp covers
+// kCols columns of 32 / kCols rows at a time.
+template <typename W, int kCols>
 __global__ void __launch_bounds__(kJoinThreads)
     join_kernel(const float* __restrict__ partial, int n, int D, W* __restrict__ dw, W* __restrict__ db) {
   wait_previous_kernel();
-  __shared__ double part[kJoinThreads / 32][kJoinCols + 1];
+  constexpr int kWarps = kJoinThreads / 32, kRows = 32 / kCols;
+  __shared__ double part[kWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * kJoinCols + lane;
+  const int c = blockIdx.x * kCols + (lane & (kCols - 1));
   double s = 0.0;
   if (c < 2 * D) {
     const float* p = partial + c;
     const int64_t ld = 2 * static_cast<int64_t>(D);
 #pragma unroll 8
-    for (int i = warp; i < n; i += kJoinThreads / 32) s += static_cast<double>(p[i * ld]);
+    for (int i = warp * kRows + lane / kCols; i < n; i += kWarps * kRows) s += static_cast<double>(p[i * ld]);
   }
-  part[warp][lane] = s;
+#pragma unroll
+  for (int o = kCols; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane < kCols) part[warp][lane] = s;
   __syncthreads();
-  if (warp) return;
-  for (int i = 1; i < kJoinThreads / 32; ++i) s += part[i][lane];
-  if (c < D) {
-    if (dw) dw[c] = Elem<W>::store(static_cast<float>(s));
-  } else if (c < 2 * D) {
-    if (db) db[c - D] = Elem<W>::store(static_cast<float>(s));
+  // warp k adds column k over the warps
+  for (int k = warp; k < kCols; k += kWarps) {
+    double t = part[lane][k];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    const int col = blockIdx.x * kCols + k;
+    if (lane) continue;
+    if (col < D) {
+      if (dw) dw[col] = Elem<W>::store(static_cast<float>(t));
+    } else if (col < 2 * D) {
+      if (db) db[col - D] = Elem<W>::store(static_cast<float>(t));
+    }
   }
 }
 
-// ---- Rows of more than 16384 elements -----------------------------------------------------
+// ---- Rows of more than 16384 elements (a vector less where none divides the width) -----------------------------------------------------
 
 template <typename T, typename W>
 __global__ void __launch_bounds__(kMaxBlockGroup)
     forward_wide_kernel(const T* __restrict__ x, RowMap xm, const W* __restrict__ w, const W* __restrict__ b,
                         T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, uint32_t rows,
                         int D, float eps) {
-  __shared__ float2 red[32];
+  __shared__ __align__(16) float red[128];
   int half = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + row_offset(xm, static_cast<uint32_t>(r));
-    float s = 0.f, q = 0.f;
-    for (int c = threadIdx.x; c < D; c += blockDim.x) s += Elem<T>::load(xr[c]);
-    const float mean = block_sum2(s, 0.f, red, half).x * inv_d;
+    float s[1] = {0.f}, q[1] = {0.f};
+    for (int c = threadIdx.x; c < D; c += blockDim.x) s[0] += Elem<T>::load(xr[c]);
+    block_sum<1>(s, red, half);
+    const float mean = s[0] * inv_d;
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
       const float d = Elem<T>::load(xr[c]) - mean;
-      q = fmaf(d, d, q);
+      q[0] = fmaf(d, d, q[0]);
     }
-    const float rstd = 1.0f / sqrtf(block_sum2(q, 0.f, red, half).x * inv_d + eps);
+    block_sum<1>(q, red, half);
+    const float rstd = 1.0f / sqrtf(q[0] * inv_d + eps);
     T* yr = y + static_cast<int64_t>(r) * D;
     for (int c = threadIdx.x; c < D; c += blockDim.x)
       yr[c] = Elem<T>::store(fmaf((Elem<T>::load(xr[c]) - mean) * rstd, w ? Elem<W>::load(w[c]) : 1.f,
@@ -335,25 +627,25 @@ __global__ void __launch_bounds__(kMaxBlockGroup)
     backward_wide_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm,
                          const W* __restrict__ w, const float* __restrict__ mean_in,
                          const float* __restrict__ rstd_in, T* __restrict__ dx, uint32_t rows, int D) {
-  __shared__ float2 red[32];
+  __shared__ __align__(16) float red[128];
   int half = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + row_offset(xm, static_cast<uint32_t>(r));
     const T* gr = dy + row_offset(dm, static_cast<uint32_t>(r));
     const float mean = mean_in[r], rstd = rstd_in[r];
-    float c1 = 0.f, c2 = 0.f;
+    float t[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
       const float g = __fmul_rn(Elem<T>::load(gr[c]), w ? Elem<W>::load(w[c]) : 1.f);
-      c1 += g;
-      c2 = fmaf(g, (Elem<T>::load(xr[c]) - mean) * rstd, c2);
+      t[0] += g;
+      t[1] = fmaf(g, (Elem<T>::load(xr[c]) - mean) * rstd, t[1]);
     }
-    const float2 t = block_sum2(c1, c2, red, half);
+    block_sum<2>(t, red, half);
     T* dr = dx + static_cast<int64_t>(r) * D;
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
       const float g = __fmul_rn(Elem<T>::load(gr[c]), w ? Elem<W>::load(w[c]) : 1.f);
       const float xh = (Elem<T>::load(xr[c]) - mean) * rstd;
-      dr[c] = Elem<T>::store(rstd * ((g - t.x * inv_d) - xh * (t.y * inv_d)));
+      dr[c] = Elem<T>::store(rstd * ((g - t[0] * inv_d) - xh * (t[1] * inv_d)));
     }
   }
 }
@@ -386,31 +678,32 @@ __global__ void __launch_bounds__(256)
 constexpr int64_t kWideSlabs = 64;
 
 struct Shape {
-  int V, G;
+  int G;
   bool block, thirty_two, wide;
 };
 
-// Elements per thread and threads per row (see the file comment). 16-byte vectors when every
-// row of every tensor begins on a 16-byte boundary, else single elements.
-Shape choose(int64_t D, bool vec, int elem_bytes) {
+// Threads per row and elements per thread (see the file comment). A row whose width no vector
+// divides takes up to a vector more.
+Shape choose(int64_t D) {
   Shape s = {};
-  s.V = vec ? 16 / elem_bytes : 1;
-  s.wide = D > 16384;
-  s.thirty_two = D > 8192;
+  const int64_t cover = D + (D % 8 ? 7 : 0);
+  s.wide = cover > 16384;
+  s.thirty_two = cover > 8192;
   const int64_t per = s.thirty_two ? 32 : 16;
-  int G = 1;
-  while (static_cast<int64_t>(G) * per < D) G <<= 1;
-  if (s.thirty_two && G < 64) G = 64;
-  s.G = G;
-  s.block = G > 32;
+  const int64_t need = (cover + per - 1) / per;  // threads
+  s.block = need > 32;
+  if (s.block)
+    s.G = static_cast<int>((need + 31) / 32 * 32);
+  else
+    for (s.G = 1; s.G < need;) s.G <<= 1;
   return s;
 }
 
 // Partial rows that the workspace holds: as many as the backward has blocks, which are at most
 // 1024 threads' worth per SM (16 blocks) on the 148 SMs of this family, and no more than rows.
 int64_t max_partials(int64_t rows, int64_t D) {
-  if (D > 16384) return rows < kWideSlabs ? rows : kWideSlabs;
-  const Shape s = choose(D, false, 4);
+  const Shape s = choose(D);
+  if (s.wide) return rows < kWideSlabs ? rows : kWideSlabs;
   const int threads = s.block ? s.G : kGroupThreads;
   int64_t cap = 1024 / threads;
   cap = 148 * (cap > 16 ? 16 : cap);
@@ -420,6 +713,7 @@ int64_t max_partials(int64_t rows, int64_t D) {
 struct Args {
   const void *x, *dy, *w, *b;
   RowMap xm, dm;
+  Order order;
   void *y, *dx, *dw, *db;
   float *mean, *rstd, *partial;
   int64_t rows;
@@ -428,53 +722,84 @@ struct Args {
   cudaStream_t st;
 };
 
-// Resident blocks of a kernel by block size (64, 128, 256, 512 threads), asked for once.
-constexpr int kBlockSizes = 4;
+// Stages of the ring and its bytes: as many as fit `sharing` blocks of an SM, four at most.
+struct Ring {
+  int stages, bytes;
+};
+template <typename R>
+Ring ring_for(int threads, int K, int tensors, int sharing, int extra) {
+  Ring r = {1, 0};
+  const int stage = tensors * K * threads * R::kBytes + extra;
+  if (R::kAsync) {
+    r.stages = kRingBytes / (sharing < 1 ? 1 : sharing) / stage;
+    r.stages = r.stages < 1 ? 1 : r.stages > kMaxStages ? kMaxStages : r.stages;
+    r.bytes = r.stages * stage;
+  }
+  return r;
+}
+
+// Resident blocks of a kernel by block size (multiples of 32), asked for once.
+constexpr int kBlockSizes = kMaxBlockGroup / 32 + 1;
 template <typename F>
 int64_t cached_residency(std::atomic<int64_t>* cache, F kernel, int threads, int smem) {
-  std::atomic<int64_t>& c = cache[threads >= 512 ? 3 : threads >= 256 ? 2 : threads >= 128 ? 1 : 0];
+  std::atomic<int64_t>& c = cache[threads / 32];
   int64_t v = c.load(std::memory_order_relaxed);
   if (!v) c.store(v = resident_blocks(kernel, threads, smem), std::memory_order_relaxed);
   return v;
 }
 
-template <typename T, typename W, int V, int K, bool kBlock>
+// Blocks for `visits` rows in turns of N per group: all that fit the device at once; with a lead,
+// a multiple of eight rows apart (see the file comment).
+int64_t grid_for(uint64_t visits, int64_t per, int N, int64_t cap, int D) {
+  const int64_t need = static_cast<int64_t>((visits + static_cast<uint64_t>(per) * N - 1) / (per * N));
+  if (need <= cap && N == 1) return need;
+  int64_t blocks = need < cap ? need : cap;
+  if (per % 8 && D % 8 && blocks > 8) blocks &= ~int64_t(7);
+  return blocks;
+}
+
+template <typename T, typename W, int V, int K, bool kBlock, int N>
 int run_forward(const Args& a, const Shape& s) {
-  auto kernel = forward_kernel<T, W, V, K, kBlock>;
+  auto kernel = forward_kernel<T, W, V, K, kBlock, N>;
   const int threads = kBlock ? s.G : kGroupThreads;
+  const Ring ring = ring_for<Row<T, V, K>>(threads, K, N, 512 / threads, 0);
+  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
-  const int64_t cap = cached_residency(cache, kernel, threads, 0);
-  const int64_t per = kBlock ? 1 : kGroupThreads / s.G;
-  int64_t blocks = (a.rows + per - 1) / per;
-  if (blocks > cap) blocks = cap;
-  return launch("layernorm forward", kernel, blocks, threads, 0, a.st, false, static_cast<const T*>(a.x), a.xm,
-                static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean, a.rstd,
-                static_cast<uint32_t>(a.rows), a.D, s.G, a.eps);
+  const int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
+  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, a.D);
+  return launch("layernorm forward", kernel, blocks, threads, ring.bytes, a.st, false, static_cast<const T*>(a.x),
+                a.xm, a.order, static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean,
+                a.rstd, a.D, s.G, ring.stages, a.eps);
 }
 
 template <typename W>
 int run_join(const Args& a, int64_t n) {
-  return launch("layernorm gradient join", join_kernel<W>, (2 * static_cast<int64_t>(a.D) + kJoinCols - 1) / kJoinCols,
-                kJoinThreads, 0, a.st, true, static_cast<const float*>(a.partial), static_cast<int>(n), a.D,
-                static_cast<W*>(a.dw), static_cast<W*>(a.db));
+  // eight columns a block until that makes more blocks than the device takes at once
+  const int64_t cols = 2 * static_cast<int64_t>(a.D);
+  const bool narrow = cols <= 8 * 296;
+  return launch("layernorm gradient join", narrow ? join_kernel<W, 8> : join_kernel<W, 32>,
+                narrow ? (cols + 7) / 8 : (cols + 31) / 32, kJoinThreads, 0, a.st, true,
+                static_cast<const float*>(a.partial), static_cast<int>(n), a.D, static_cast<W*>(a.dw),
+                static_cast<W*>(a.db));
 }
 
-template <typename T, typename W, int V, int K, bool kBlock>
+template <typename T, typename W, int V, int K, bool kBlock, int N>
 int run_backward(const Args& a, const Shape& s) {
-  auto kernel = backward_kernel<T, W, V, K, kBlock>;
+  auto kernel = backward_kernel<T, W, V, K, kBlock, N>;
   const int threads = kBlock ? s.G : kGroupThreads;
-  const int smem = kBlock ? 0 : 2 * a.D * static_cast<int>(sizeof(float));
+  // a stage's statistics: 8 bytes a row for each warp or smaller group; the ring also joins the groups
+  Ring ring = ring_for<Row<T, V, K>>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N);
+  if (!kBlock && ring.bytes < 2 * a.D * 4) ring.bytes = 2 * a.D * 4;
+  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
-  const int64_t cap = cached_residency(cache, kernel, threads, kBlock ? 0 : 4096);
-  const int64_t per = kBlock ? 1 : kGroupThreads / s.G;
-  int64_t blocks = (a.rows + per - 1) / per;
-  if (blocks > cap) blocks = cap;
+  int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
   const int64_t most = max_partials(a.rows, a.D);
-  if (blocks > most) blocks = most;
-  if (int e = launch("layernorm backward", kernel, blocks, threads, smem, a.st, false, static_cast<const T*>(a.dy),
-                     a.dm, static_cast<const T*>(a.x), a.xm, static_cast<const W*>(a.w),
-                     static_cast<const float*>(a.mean), static_cast<const float*>(a.rstd), static_cast<T*>(a.dx),
-                     a.partial, static_cast<uint32_t>(a.rows), a.D, s.G))
+  if (cap > most) cap = most;
+  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, a.D);
+  if (int e = launch("layernorm backward", kernel, blocks, threads, ring.bytes, a.st, false,
+                     static_cast<const T*>(a.dy), a.dm, static_cast<const T*>(a.x), a.xm, a.order,
+                     static_cast<const W*>(a.w), static_cast<const float*>(a.mean),
+                     static_cast<const float*>(a.rstd), static_cast<T*>(a.dx), a.partial, a.D, s.G, ring.stages))
     return e;
   return a.partial ? run_join<W>(a, blocks) : GTK_OK;
 }
@@ -506,24 +831,26 @@ int run_wide(const Args& a, bool backward) {
   return run_join<W>(a, slabs);
 }
 
-template <typename T, typename W, int V, int K, bool kBlock>
+template <typename T, typename W, int V, int K, bool kBlock, int N>
 int run_one(const Args& a, const Shape& s, bool backward) {
-  return backward ? run_backward<T, W, V, K, kBlock>(a, s) : run_forward<T, W, V, K, kBlock>(a, s);
+  return backward ? run_backward<T, W, V, K, kBlock, N>(a, s) : run_forward<T, W, V, K, kBlock, N>(a, s);
 }
 
 template <typename T, typename W>
 int run_typed(const Args& a, bool vec, bool backward) {
   constexpr int VX = 16 / static_cast<int>(sizeof(T));
-  const Shape s = choose(a.D, vec, sizeof(T));
+  const Shape s = choose(a.D);
   if (s.wide) return run_wide<T, W>(a, backward);
-  if (s.V > 1) {
-    if (s.thirty_two) return run_one<T, W, VX, 32 / VX, true>(a, s, backward);
-    if (s.block) return run_one<T, W, VX, 16 / VX, true>(a, s, backward);
-    return run_one<T, W, VX, 16 / VX, false>(a, s, backward);
+  if (vec) {
+    if (s.thirty_two) return run_one<T, W, VX, 32 / VX, true, 1>(a, s, backward);
+    if (!s.block) return run_one<T, W, VX, 16 / VX, false, 1>(a, s, backward);
+    // two rows a turn, once there are more rows than blocks
+    if (a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G)) return run_one<T, W, VX, 16 / VX, true, 1>(a, s, backward);
+    return run_one<T, W, VX, 16 / VX, true, 2>(a, s, backward);
   }
-  if (s.thirty_two) return run_one<T, W, 1, 32, true>(a, s, backward);
-  if (s.block) return run_one<T, W, 1, 16, true>(a, s, backward);
-  return run_one<T, W, 1, 16, false>(a, s, backward);
+  if (s.thirty_two) return run_one<T, W, 1, 32, true, 1>(a, s, backward);
+  if (s.block) return run_one<T, W, 1, 16, true, 1>(a, s, backward);
+  return run_one<T, W, 1, 16, false, 1>(a, s, backward);
 }
 
 int run(const Args& a, int xt, int wt, bool vec, bool backward) {
@@ -534,15 +861,17 @@ int run(const Args& a, int xt, int wt, bool vec, bool backward) {
   return wt == GTK_F32 ? run_typed<__half, float>(a, vec, backward) : run_typed<__half, __half>(a, vec, backward);
 }
 
-// Checks a tensor's leading axes and fills its RowMap; `vec` is cleared when some row does not
-// begin on a 16-byte boundary.
+// Checks a tensor's leading axes and fills its RowMap; `vec` is cleared when its rows cannot be
+// read in aligned 16-byte vectors: they begin anywhere, or strided rows do not all begin on a
+// boundary.
 int row_map(const gtk_rows* v, const void* base, int64_t rows, int64_t D, size_t bytes, const char* what, RowMap* out,
             bool* vec) {
-  if ((D * bytes) % 16 || !aligned16(base)) *vec = false;
+  if (!aligned16(base)) *vec = false;
   if (!v) {
     *out = RowMap{0, 0, D, 0, 0};
     return GTK_OK;
   }
+  if ((D * bytes) % 16) *vec = false;
   for (int i = 0; i < 3; ++i) {
     if (v->size[i] < 1 || v->size[i] > rows)
       return fail(GTK_ERR_INVALID_ARG, std::string("layernorm: bad leading sizes of ") + what);
@@ -554,6 +883,19 @@ int row_map(const gtk_rows* v, const void* base, int64_t rows, int64_t D, size_t
   *out = RowMap{v->stride[0], v->stride[1], v->stride[2], static_cast<uint32_t>(v->size[1]),
                 static_cast<uint32_t>(v->size[2])};
   return GTK_OK;
+}
+
+// Tiles where a tensor's rows lie closer along its second axis than along its third.
+Order order_for(int64_t rows, const RowMap& a, const RowMap* b) {
+  Order o = {0, 0, 0, 0, static_cast<uint64_t>(rows)};
+  for (const RowMap* m : {&a, b}) {
+    if (!m || m->n2 < 4 || m->n1 < 8 || m->s1 >= m->s2) continue;
+    const uint64_t t1 = (m->n1 + 7) / 8, t2 = (m->n2 + 3) / 4, planes = rows / (static_cast<uint64_t>(m->n1) * m->n2);
+    if (planes * t1 * t2 > (uint64_t(1) << 31)) continue;
+    o = Order{m->n1, m->n2, static_cast<uint32_t>(t1), static_cast<uint32_t>(t2), planes * t1 * t2 * 32};
+    break;
+  }
+  return o;
 }
 
 int check_common(int64_t rows, int64_t D, int x_dtype, int w_dtype) {
@@ -594,6 +936,7 @@ int gtk_layernorm_forward(const void* x, const gtk_rows* x_rows, int x_dtype, co
   ln::Args a = {};
   bool vec = aligned16(y);
   if (int e = ln::row_map(x_rows, x, rows, D, dtype_bytes(x_dtype), "x", &a.xm, &vec)) return e;
+  a.order = ln::order_for(rows, a.xm, nullptr);
   if (int e = check_device()) return e;
   a.x = x, a.w = weight, a.b = bias, a.y = y, a.mean = mean, a.rstd = rstd;
   a.rows = rows, a.D = static_cast<int>(D), a.eps = eps, a.st = static_cast<cudaStream_t>(stream);
@@ -625,6 +968,10 @@ int gtk_layernorm_backward(const void* dy, const gtk_rows* dy_rows, const void* 
   bool vec = aligned16(dx);
   if (int e = ln::row_map(x_rows, x, rows, D, dtype_bytes(x_dtype), "x", &a.xm, &vec)) return e;
   if (int e = ln::row_map(dy_rows, dy, rows, D, dtype_bytes(x_dtype), "dy", &a.dm, &vec)) return e;
+  // vectors are laid over the rows of all tensors at once: with a strided tensor, rows that all
+  // begin on a boundary
+  if ((x_rows || dy_rows) && (D * dtype_bytes(x_dtype)) % 16) vec = false;
+  a.order = ln::order_for(rows, a.xm, &a.dm);
   if (int e = check_device()) return e;
   a.x = x, a.dy = dy, a.w = weight, a.dx = dx, a.dw = dweight, a.db = dbias;
   a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);

@@ -122,6 +122,31 @@ struct Vec {
   }
 };
 
+// fp32 arithmetic on pairs: one instruction for two elements.
+__device__ __forceinline__ unsigned long long pair_bits(float2 a) { return *reinterpret_cast<unsigned long long*>(&a); }
+__device__ __forceinline__ float2 pair_of(unsigned long long b) { return *reinterpret_cast<float2*>(&b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return pair_of(r);
+}
+// A product that is rounded before anything is added to it (the assembler fuses mul.rn.f32x2, and
+// even a product with -0 added, with an add that follows).
+__device__ __forceinline__ float2 rounded_mul2(float2 a, float2 b) {
+  return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y));
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> ld_vec(const T* p) {
   Vec<T, V> v;

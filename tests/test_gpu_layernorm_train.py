@@ -102,9 +102,9 @@ def _run_and_check(x, dy, w, b, eps=EPS):
 
 @pytest.mark.parametrize("dtype,pdtype", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"),
                                           ("f16", "f32")])
-@pytest.mark.parametrize("rows,D", [(1, 8), (1, 384), (5, 33), (37, 384), (300, 128), (2000, 16), (257, 1000),
+@pytest.mark.parametrize("rows,D", [(1, 8), (2, 9), (1, 384), (5, 33), (37, 384), (300, 128), (2000, 16), (257, 1000),
                                     (65, 512), (66, 520), (64, 1024), (700, 2048), (9, 5003), (5, 8192), (3, 8193),
-                                    (4, 8200), (4, 16384), (3, 16385), (2, 40000)])
+                                    (4, 8200), (4, 16384), (5, 8185), (5, 8191), (3, 16377), (3, 16379), (3, 16385), (2, 40000)])
 def test_matches_the_formula(rows, D, dtype, pdtype):
     dev = require_gpu()
     x, dy, w, b = _inputs((rows, D), DT[dtype], DT[pdtype], rows * 7 + D, dev)
@@ -115,7 +115,7 @@ def test_matches_the_formula(rows, D, dtype, pdtype):
 def test_many_rows(dtype):
     """More rows than the grid has groups, with a last turn that is not full."""
     dev = require_gpu()
-    for rows, D in ((100003, 40), (20011, 128), (6007, 777)):
+    for rows, D in ((100003, 40), (20011, 128), (6007, 777), (50001, 37), (3001, 1001), (5000, 513), (2999, 2050)):
         _run_and_check(*_inputs((rows, D), DT[dtype], torch.float32, rows, dev))
 
 
@@ -134,7 +134,8 @@ def test_shortest_rows(D):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("B,N,D", [(1, 9, 128), (2, 7, 128), (3, 5, 33), (2, 6, 64)])
+@pytest.mark.parametrize("B,N,D", [(1, 9, 128), (2, 7, 128), (3, 5, 33), (2, 6, 64), (1, 8, 128), (2, 37, 96),
+                                   (1, 70, 600)])
 def test_transposed_pair_axes_are_read_in_place(B, N, D, dtype):
     dev = require_gpu()
     x, dy, w, b = _inputs((B, N, N, D), DT[dtype], torch.float32, N, dev)
