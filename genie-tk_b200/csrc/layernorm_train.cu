@@ -53,35 +53,69 @@ constexpr int kJoinThreads = 1024;
 constexpr int kMaxStages = 4;             // rows of the ring
 constexpr int kRingBytes = 200 * 1024;    // of an SM
 
-// Where row r of a tensor with up to three leading axes begins: r = (a n1 + b) n2 + c lies
-// at a s0 + b s1 + c s2 (element strides); n1 = n2 = 0: rows follow one another, s2 apart.
-struct RowMap {
-  int64_t s0, s1, s2;
-  uint32_t n1, n2;
+// Division of n < 2^31 by a constant of the launch.
+struct Divisor {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> shift; }
 };
 
-__device__ __forceinline__ int64_t row_offset(const RowMap& m, uint32_t r) {
-  if (m.n2 == 0) return static_cast<int64_t>(r) * m.s2;
-  const uint32_t t = r / m.n2, c = r - t * m.n2;
-  const uint32_t a = t / m.n1, b = t - a * m.n1;
-  return a * m.s0 + b * m.s1 + c * m.s2;
+// With l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1, floor(n m / 2^(31 + l)) is n / d for
+// n < 2^31 (m d exceeds 2^(31 + l) by e <= d <= 2^l, and n e < 2^(31 + l)).
+Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  if (d <= 1) return Divisor{1, 0, 0};
+  return Divisor{d, static_cast<uint32_t>((uint64_t(1) << (31 + l)) / d + 1), l - 1};
 }
 
-// The order in which rows are visited: as they come (n1 = 0), or the n1 x n2 planes of rows in
+// Where row r of a tensor with up to three leading axes begins: r = (a n1 + b) n2 + c lies
+// at a s0 + b s1 + c s2 (element strides); `plain`: rows follow one another, s2 apart.
+struct RowMap {
+  int64_t s0, s1, s2;
+  Divisor n1, n2;
+  bool plain;
+};
+
+// The order in which rows are visited: as they come, or (`tiled`) the n1 x n2 planes of rows in
 // tiles of 8 x 4, t1 x t2 of them (the last ones in part outside). `visits` counts places.
 struct Order {
-  uint32_t n1, n2, t1, t2;
+  Divisor t1, t2;
+  uint32_t n1, n2;
   uint64_t visits;
+  bool tiled;
 };
 constexpr uint32_t kNoRow = 0xffffffffu;
 
-__device__ __forceinline__ uint32_t row_at(const Order& o, uint64_t v) {
-  if (v >= o.visits) return kNoRow;
-  if (o.n1 == 0) return static_cast<uint32_t>(v);
-  const uint32_t tile = static_cast<uint32_t>(v >> 5), t = tile / o.t2, a = t / o.t1;
-  const uint32_t b = (t - a * o.t1) * 8 + (static_cast<uint32_t>(v) & 7u);
-  const uint32_t c = (tile - t * o.t2) * 4 + (static_cast<uint32_t>(v >> 3) & 3u);
-  return b < o.n1 && c < o.n2 ? (a * o.n1 + b) * o.n2 + c : kNoRow;
+// A row and, with tiles, its coordinates.
+struct Place {
+  uint32_t r, a, b, c;
+};
+
+__device__ __forceinline__ Place place_at(const Order& o, uint64_t v) {
+  Place p = {kNoRow, 0, 0, 0};
+  if (v >= o.visits) return p;
+  if (!o.tiled) {
+    p.r = static_cast<uint32_t>(v);
+    return p;
+  }
+  const uint32_t tile = static_cast<uint32_t>(v >> 5), t = o.t2.quotient(tile);
+  p.a = o.t1.quotient(t);
+  p.b = (t - p.a * o.t1.d) * 8 + (static_cast<uint32_t>(v) & 7u);
+  p.c = (tile - t * o.t2.d) * 4 + (static_cast<uint32_t>(v >> 3) & 3u);
+  if (p.b < o.n1 && p.c < o.n2) p.r = (p.a * o.n1 + p.b) * o.n2 + p.c;
+  return p;
+}
+
+__device__ __forceinline__ int64_t row_offset(const RowMap& m, uint32_t r) {
+  if (m.plain) return static_cast<int64_t>(r) * m.s2;
+  const uint32_t t = m.n2.quotient(r), c = r - t * m.n2.d;
+  const uint32_t a = m.n1.quotient(t), b = t - a * m.n1.d;
+  return a * m.s0 + b * m.s1 + c * m.s2;
+}
+
+__device__ __forceinline__ int64_t row_offset(const RowMap& m, const Order& o, const Place& p) {
+  if (o.tiled && !m.plain && m.n1.d == o.n1 && m.n2.d == o.n2) return p.a * m.s0 + p.b * m.s1 + p.c * m.s2;
+  return row_offset(m, p.r);
 }
 
 // Sums over a group of G <= 32 lanes of a warp.
@@ -137,17 +171,21 @@ __device__ __forceinline__ void block_sum(float (&v)[n], float* buf, int& half) 
   }
 }
 
-// How a group's vectors lie over its rows: vector i covers the columns i V - lead .. + V - 1.
+// How a group's vectors lie over its rows: vector i covers the columns i V - lead .. + V - 1. kEdge:
+// the width is no multiple of V, so that rows begin and end inside a vector.
+template <bool kEdge>
 struct Lay {
-  int lane, G, nv, lead, D;
+  int lane, G, nv, lead_, D;
+  __device__ __forceinline__ int lead() const { return kEdge ? lead_ : 0; }
 };
 
 // A thread's elements of a row: K vectors of V at vector indices lane + G k < nv. Vectors come
 // through a ring slot in shared memory ([k][thread], 16 bytes each; slots of vectors that do not
 // exist hold zeros from the start); single elements (V = 1: rows that begin anywhere) through
 // registers, without a row ahead.
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool kEdge>
 struct Row {
+  using L = Lay<kEdge>;
   static constexpr bool kAsync = V > 1;
   static constexpr int kBytes = 16;
   Vec<T, V> e[kAsync ? 1 : K];
@@ -156,23 +194,28 @@ struct Row {
 
   // `p`: the row's first element. The last vector reads no further than the row; the first one
   // begins with up to V - 1 elements of the row before.
-  static __device__ __forceinline__ void request(char* slot, int pitch, const T* p, const Lay& l) {
+  static __device__ __forceinline__ void request(char* slot, int pitch, const T* p, const L& l) {
     if constexpr (kAsync) {
       const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
-      const T* from = p - l.lead + l.lane * V;
+      const T* from = p - l.lead() + l.lane * V;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int i = l.lane + l.G * k;
         if (i >= l.nv) continue;
-        const int left = (l.lead + l.D - i * V) * static_cast<int>(sizeof(T));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * pitch),
-                     "l"(from + static_cast<int64_t>(l.G) * k * V), "r"(left < 16 ? left : 16)
-                     : "memory");
+        const T* src = from + l.G * k * V;
+        if constexpr (kEdge) {
+          const int left = (l.lead() + l.D - i * V) * static_cast<int>(sizeof(T));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * pitch), "l"(src),
+                       "r"(left < 16 ? left : 16)
+                       : "memory");
+        } else {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * pitch), "l"(src) : "memory");
+        }
       }
     }
   }
   // What was requested (kAsync), or now.
-  __device__ __forceinline__ void open(const char* s, int pt, const T* p, const Lay& l) {
+  __device__ __forceinline__ void open(const char* s, int pt, const T* p, const L& l) {
     if constexpr (kAsync) {
       slot = s;
       pitch = pt;
@@ -185,19 +228,19 @@ struct Row {
     }
   }
   // Vector k; elements before the row are zeros.
-  __device__ __forceinline__ Vec<T, V> vec(int k, const Lay& l) const {
+  __device__ __forceinline__ Vec<T, V> vec(int k, const L& l) const {
     if constexpr (!kAsync) return e[k];
     Vec<T, V> v = ld_vec<T, V>(reinterpret_cast<const T*>(slot + k * pitch));
-    if (k == 0 && l.lead > l.lane * V) {
+    if (kEdge && k == 0 && l.lead() > l.lane * V) {
       float f[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = j < l.lead ? 0.f : v.get(j);
+      for (int j = 0; j < V; ++j) f[j] = j < l.lead() ? 0.f : v.get(j);
       v = Vec<T, V>::of(f);
     }
     return v;
   }
   // The thread's elements in pairs: 2 p and 2 p + 1.
-  __device__ __forceinline__ void pairs(float2 (&out)[K * V / 2], const Lay& l) const {
+  __device__ __forceinline__ void pairs(float2 (&out)[K * V / 2], const L& l) const {
     if constexpr (V == 1) {
 #pragma unroll
       for (int p = 0; p < K / 2; ++p) out[p] = make_float2(e[2 * p].get(0), e[2 * p + 1].get(0));
@@ -214,8 +257,8 @@ struct Row {
 
 // Stores the thread's elements of a row; the first and last vector by element where the row
 // begins or ends inside.
-template <typename T, int V, int K>
-__device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], const Lay& l) {
+template <typename T, int V, int K, bool kEdge>
+__device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], const Lay<kEdge>& l) {
   if constexpr (V == 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -225,12 +268,12 @@ __device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], co
   } else {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int i = l.lane + l.G * k, c = i * V - l.lead;
+      const int i = l.lane + l.G * k, c = i * V - l.lead();
       if (i >= l.nv) continue;
       float o[V];
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) o[2 * j] = f[k * (V / 2) + j].x, o[2 * j + 1] = f[k * (V / 2) + j].y;
-      if (c >= 0 && c + V <= l.D) {
+      if (!kEdge || (c >= 0 && c + V <= l.D)) {
         st_vec<T, V>(p + c, Vec<T, V>::of(o));
       } else {
 #pragma unroll
@@ -242,10 +285,13 @@ __device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], co
 }
 
 // The column of the thread's element e (0 .. K V - 1); negative or >= D where there is none.
-template <int V>
-__device__ __forceinline__ int column_of(int e, const Lay& l) {
-  return (l.lane + l.G * (e / V)) * V - l.lead + e % V;
+template <int V, bool kEdge>
+__device__ __forceinline__ int column_of(int e, const Lay<kEdge>& l) {
+  return (l.lane + l.G * (e / V)) * V - l.lead() + e % V;
 }
+
+// Floats of dw (and of db) in a partial row: the columns, and room for a lead.
+__host__ __device__ __forceinline__ int partial_pitch(int D) { return D % 8 ? (D + 14) / 8 * 8 : D; }
 
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the newest `stages` - 1 groups of this thread's copies have arrived.
@@ -262,68 +308,75 @@ __device__ __forceinline__ void wait_copies(int stages) {
 
 // The thread's columns of a parameter in pairs: kept in registers with 16 elements per thread,
 // read again for every row (from the L1 cache) with 32.
-template <typename W, int V, int K>
+template <typename W, int V, int K, bool kEdge>
 struct Columns {
+  using L = Lay<kEdge>;
   static constexpr bool kKeep = V * K <= 16;
   float2 f[kKeep ? V * K / 2 : 1];
   const W* w;
   float other;
-  __device__ __forceinline__ float element(int e, const Lay& l) const {
-    const int c = column_of<V>(e, l);
+  __device__ __forceinline__ float element(int e, const L& l) const {
+    const int c = column_of<V, kEdge>(e, l);
     return w && c >= 0 && c < l.D ? Elem<W>::load(w[c]) : other;
   }
-  __device__ __forceinline__ Columns(const W* p, float absent, const Lay& l) : w(p), other(absent) {
+  __device__ __forceinline__ Columns(const W* p, float absent, const L& l) : w(p), other(absent) {
     if constexpr (kKeep) {
 #pragma unroll
       for (int i = 0; i < V * K / 2; ++i) f[i] = make_float2(element(2 * i, l), element(2 * i + 1, l));
     }
   }
-  __device__ __forceinline__ float2 get(int i, const Lay& l) const {
+  __device__ __forceinline__ float2 get(int i, const L& l) const {
     if constexpr (kKeep) return f[i];
     return make_float2(element(2 * i, l), element(2 * i + 1, l));
   }
 };
 
-__device__ __forceinline__ void zero_ring(char* ring, int bytes) {
-  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-    *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
-  __syncthreads();
+// Zeros in the thread's slots of vectors that do not exist, in `rows` rows of the ring.
+template <typename T, int V, int K, bool kEdge>
+__device__ __forceinline__ void zero_missing(char* mine, int pitch, int rows, const Lay<kEdge>& l) {
+  if (V == 1 || l.nv >= l.G * K) return;
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (l.lane + l.G * k >= l.nv) *reinterpret_cast<uint4*>(mine + (r * K + k) * pitch) = make_uint4(0, 0, 0, 0);
 }
 
 // Forward. kBlock: the block is one group of blockDim.x threads; else groups of G <= 32. A turn of
 // the loop takes N rows of each group.
-template <typename T, typename W, int V, int K, bool kBlock, int N>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
 __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     forward_kernel(const T* __restrict__ x, RowMap xm, Order order, const W* __restrict__ w,
                    const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean_out,
                    float* __restrict__ rstd_out, int D, int G, int stages, float eps) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float red[128];
-  using R = Row<T, V, K>;
+  using R = Row<T, V, K, kEdge>;
+  using L = Lay<kEdge>;
   constexpr int P = K * V / 2;
   int half = 0;
   const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
   const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
   const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
-  const int lead = static_cast<int>(first * D & (V - 1));
-  const Lay l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+  const int lead = kEdge ? static_cast<int>(first * D & (V - 1)) : 0;
+  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
                  (lead + D + V - 1) / V, lead, D};
   const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch;
   char* mine = ring + threadIdx.x * R::kBytes;
   const float inv_d = 1.0f / static_cast<float>(D);
-  if constexpr (R::kAsync) zero_ring(ring, stages * N * row_bytes);
-  const Columns<W, V, K> wc(w, 1.f, l), bc(b, 0.f, l);
+  zero_missing<T, V, K>(mine, pitch, stages * N, l);
   auto request = [&](int s, uint64_t v) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const uint32_t r = row_at(order, v + q * step);
-      if (r != kNoRow) R::request(mine + (s * N + q) * row_bytes, pitch, x + row_offset(xm, r), l);
+      const Place at = place_at(order, v + q * step);
+      if (at.r != kNoRow)
+        R::request(mine + (s * N + q) * row_bytes, pitch, x + row_offset(xm, order, at), l);
     }
     commit_copies();
   };
   if constexpr (R::kAsync)
     for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+  const Columns<W, V, K, kEdge> wc(w, 1.f, l), bc(b, 0.f, l);
   int now = 0;
   // every group of the block makes the same number of turns, so that shuffles and barriers meet
   for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
@@ -336,8 +389,8 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     float s[N], sq[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      r[q] = row_at(order, v0 + q * step);
-      Lay lq = l;
+      r[q] = place_at(order, v0 + q * step).r;
+      L lq = l;
       if (r[q] == kNoRow) lq.nv = 0;
       R row;
       row.open(mine + (now * N + q) * row_bytes, pitch, x + row_offset(xm, r[q] == kNoRow ? 0u : r[q]), lq);
@@ -360,12 +413,14 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
       for (int p = 0; p < P; ++p) {
         v[q][p] = add2(v[q][p], both(-s[q]));
         if constexpr (V == 1) {  // elements that do not exist have no deviation
-          if (column_of<V>(2 * p, l) >= D) v[q][p].x = 0.f;
-          if (column_of<V>(2 * p + 1, l) >= D) v[q][p].y = 0.f;
+          if (column_of<V, kEdge>(2 * p, l) >= D) v[q][p].x = 0.f;
+          if (column_of<V, kEdge>(2 * p + 1, l) >= D) v[q][p].y = 0.f;
+        } else if constexpr (!kEdge) {
+          if (l.lane + l.G * (2 * p / V) >= l.nv) v[q][p] = make_float2(0.f, 0.f);
         } else {
-          const int c = column_of<V>(2 * p / V * V, l);
+          const int c = column_of<V, kEdge>(2 * p / V * V, l);
           if (c < 0 || c + V > D) {
-            const int c2 = column_of<V>(2 * p, l);
+            const int c2 = column_of<V, kEdge>(2 * p, l);
             if (c2 < 0 || c2 >= D) v[q][p].x = 0.f;
             if (c2 + 1 < 0 || c2 + 1 >= D) v[q][p].y = 0.f;
           }
@@ -384,7 +439,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
       const float rstd = 1.0f / sqrtf(sq[q] * inv_d + eps);
 #pragma unroll
       for (int p = 0; p < P; ++p) v[q][p] = fma2(mul2(v[q][p], both(rstd)), wc.get(p, l), bc.get(p, l));
-      store_row<T, V, K>(y + static_cast<int64_t>(r[q]) * D, v[q], l);
+      store_row<T, V, K, kEdge>(y + static_cast<int64_t>(r[q]) * D, v[q], l);
       if (l.lane == 0) {
         mean_out[r[q]] = s[q];
         rstd_out[r[q]] = rstd;
@@ -395,22 +450,23 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
 
 // Backward: dx and, per block, one partial row [dw | db] of 2 D floats. The ring's stage holds N
 // x rows, N dy rows and, for each warp (group, where that is smaller), their mean and rstd.
-template <typename T, typename W, int V, int K, bool kBlock, int N>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
 __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBlock ? 1 : 2)
     backward_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm, Order order,
                     const W* __restrict__ w, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                     T* __restrict__ dx, float* __restrict__ partial, int D, int G, int stages) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float red[128];
-  using R = Row<T, V, K>;
+  using R = Row<T, V, K, kEdge>;
+  using L = Lay<kEdge>;
   constexpr int P = K * V / 2;
   int half = 0;
   const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
   const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
   const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
-  const int lead = static_cast<int>(first * D & (V - 1));
-  const Lay l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+  const int lead = kEdge ? static_cast<int>(first * D & (V - 1)) : 0;
+  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
                  (lead + D + V - 1) / V, lead, D};
   const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch, stage_bytes = 2 * N * row_bytes;
   const int share = kBlock ? 32 : G;  // threads that share a copy of the statistics
@@ -418,19 +474,19 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
   float* stats = reinterpret_cast<float*>(ring + stages * stage_bytes) + threadIdx.x / share * 2 * N;
   const int stats_stage = blockDim.x / share * 2 * N;
   const float inv_d = 1.0f / static_cast<float>(D);
-  if constexpr (R::kAsync) zero_ring(ring, stages * stage_bytes);
-  const Columns<W, V, K> wc(w, 1.f, l);
+  zero_missing<T, V, K>(mine, pitch, stages * 2 * N, l);
   float2 aw[P], ab[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) aw[p] = ab[p] = make_float2(0.f, 0.f);
   auto request = [&](int s, uint64_t v) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const uint32_t r = row_at(order, v + q * step);
+      const Place at = place_at(order, v + q * step);
+      const uint32_t r = at.r;
       if (r == kNoRow) continue;
       char* to = mine + s * stage_bytes + 2 * q * row_bytes;
-      R::request(to, pitch, x + row_offset(xm, r), l);
-      R::request(to + row_bytes, pitch, dy + row_offset(dm, r), l);
+      R::request(to, pitch, x + row_offset(xm, order, at), l);
+      R::request(to + row_bytes, pitch, dy + row_offset(dm, order, at), l);
       if (threadIdx.x % share == 0) {
         const uint32_t st = static_cast<uint32_t>(__cvta_generic_to_shared(stats + s * stats_stage + 2 * q));
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st), "l"(mean_in + r) : "memory");
@@ -441,6 +497,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
   };
   if constexpr (R::kAsync)
     for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+  const Columns<W, V, K, kEdge> wc(w, 1.f, l);
   int now = 0;
   for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
     if constexpr (R::kAsync) {
@@ -453,9 +510,9 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
     float mean[N], rstd[N], c[2 * N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      r[q] = row_at(order, v0 + q * step);
+      r[q] = place_at(order, v0 + q * step).r;
       const bool valid = r[q] != kNoRow;
-      Lay lq = l;
+      L lq = l;
       if (!valid) lq.nv = 0;
       mean[q] = rstd[q] = 0.f;
       if constexpr (R::kAsync) {
@@ -505,27 +562,39 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
         const float2 g = rounded_mul2(gp[p], wc.get(p, l));
         xp[p] = mul2(both(rstd[q]), fma2(xh, both(-c2), add2(g, both(-c1))));
       }
-      store_row<T, V, K>(dx + static_cast<int64_t>(r[q]) * D, xp, l);
+      store_row<T, V, K, kEdge>(dx + static_cast<int64_t>(r[q]) * D, xp, l);
     }
   }
   if (!partial) return;
-  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
-  float* pb = pw + D;
+  const int ld = partial_pitch(D);
+  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * ld;
   if (kBlock) {
+    // as the vectors lie: column c at c + lead
 #pragma unroll
-    for (int e = 0; e < K * V; ++e) {
-      const int col = column_of<V>(e, l);
-      if (col < 0 || col >= D) continue;
-      pw[col] = e & 1 ? aw[e / 2].y : aw[e / 2].x;
-      pb[col] = e & 1 ? ab[e / 2].y : ab[e / 2].x;
+    for (int k = 0; k < K; ++k) {
+      const int i = l.lane + l.G * k;
+      if (i >= l.nv) continue;
+      if constexpr (V == 1) {
+        pw[i] = k & 1 ? aw[k / 2].y : aw[k / 2].x;
+        pw[ld + i] = k & 1 ? ab[k / 2].y : ab[k / 2].x;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V / 2; j += 2) {
+          const int p = k * (V / 2) + j;
+          *reinterpret_cast<float4*>(pw + i * V + 2 * j) = make_float4(aw[p].x, aw[p].y, aw[p + 1].x, aw[p + 1].y);
+          *reinterpret_cast<float4*>(pw + ld + i * V + 2 * j) = make_float4(ab[p].x, ab[p].y, ab[p + 1].x, ab[p + 1].y);
+        }
+      }
     }
     return;
   }
-  // the groups one after another in the ring's memory; groups that lie alike are added in the
-  // warp first (with a lead, the groups of a warp lie differently)
+  // every warp adds its groups in the ring's memory, then the block the warps. Groups that lie
+  // alike are added by shuffles (with a lead, the groups of a warp lie differently).
   wait_copies(1);
-  const bool alike = D % V == 0;
-  if (alike)
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  float* cols = reinterpret_cast<float*>(ring) + warp * 2 * D;
+  if (!kEdge) {
 #pragma unroll
     for (int p = 0; p < P; ++p)
       for (int o = G; o < 32; o <<= 1) {
@@ -534,41 +603,53 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
         ab[p].x += __shfl_xor_sync(0xffffffffu, ab[p].x, o);
         ab[p].y += __shfl_xor_sync(0xffffffffu, ab[p].y, o);
       }
-  __syncthreads();
-  float* cols = reinterpret_cast<float*>(ring);  // [2][D]
-  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) cols[i] = 0.f;
-  __syncthreads();
-  const int unit = alike ? 32 : G;  // threads that add at once
-  for (int t = 0; t < static_cast<int>(blockDim.x) / unit; ++t) {
-    if (static_cast<int>(threadIdx.x) / unit == t && static_cast<int>(threadIdx.x) % unit < G)
+  } else {
+    for (int i = threadIdx.x & 31; i < 2 * D; i += 32) cols[i] = 0.f;
+    __syncwarp();
+  }
+  for (int t = 0; t < (kEdge ? 32 / G : 1); ++t) {
+    if (static_cast<int>(threadIdx.x & 31) / G == t)
 #pragma unroll
       for (int e = 0; e < K * V; ++e) {
-        const int col = column_of<V>(e, l);
+        const int col = column_of<V, kEdge>(e, l);
         if (col < 0 || col >= D) continue;
-        cols[col] += e & 1 ? aw[e / 2].y : aw[e / 2].x;
-        cols[D + col] += e & 1 ? ab[e / 2].y : ab[e / 2].x;
+        cols[col] = (kEdge ? cols[col] : 0.f) + (e & 1 ? aw[e / 2].y : aw[e / 2].x);
+        cols[D + col] = (kEdge ? cols[D + col] : 0.f) + (e & 1 ? ab[e / 2].y : ab[e / 2].x);
       }
-    __syncthreads();
+    __syncwarp();
   }
-  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) pw[i] = cols[i];
+  __syncthreads();
+  cols = reinterpret_cast<float*>(ring);
+  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+    float t = 0.f;
+    for (int q = 0; q < warps; ++q) t += cols[q * 2 * D + i];
+    pw[i < D ? i : i - D + ld] = t;
+  }
 }
 
-// dw, db: the sum of `n` partial rows of 2 D floats, in a fixed order and 64 bits. A warp covers
-// kCols columns of 32 / kCols rows at a time.
+// dw, db: the sum of `n` partial rows of two times `ld` floats, in a fixed order and 64 bits. Partial
+// row i holds column c at c + (i D mod V) (shift: V - 1, or 0). A warp covers kCols columns of
+// 32 / kCols rows at a time; blocks of dw come first, then those of db.
 template <typename W, int kCols>
 __global__ void __launch_bounds__(kJoinThreads)
-    join_kernel(const float* __restrict__ partial, int n, int D, W* __restrict__ dw, W* __restrict__ db) {
+    join_kernel(const float* __restrict__ partial, int n, int D, int ld, uint32_t shift, W* __restrict__ dw,
+                W* __restrict__ db) {
   wait_previous_kernel();
   constexpr int kWarps = kJoinThreads / 32, kRows = 32 / kCols;
   __shared__ double part[kWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * kCols + (lane & (kCols - 1));
+  const int half = (D + kCols - 1) / kCols;  // blocks
+  const bool second = static_cast<int>(blockIdx.x) >= half;
+  const int c0 = (static_cast<int>(blockIdx.x) - (second ? half : 0)) * kCols;
+  W* out = second ? db : dw;
+  if (!out) return;
+  const int c = c0 + (lane & (kCols - 1));
   double s = 0.0;
-  if (c < 2 * D) {
-    const float* p = partial + c;
-    const int64_t ld = 2 * static_cast<int64_t>(D);
+  if (c < D) {
+    const float* p = partial + c + (second ? ld : 0);
 #pragma unroll 8
-    for (int i = warp * kRows + lane / kCols; i < n; i += kWarps * kRows) s += static_cast<double>(p[i * ld]);
+    for (int i = warp * kRows + lane / kCols; i < n; i += kWarps * kRows)
+      s += static_cast<double>(p[static_cast<int64_t>(i) * 2 * ld + (static_cast<uint32_t>(i) * static_cast<uint32_t>(D) & shift)]);
   }
 #pragma unroll
   for (int o = kCols; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -579,13 +660,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     double t = part[lane][k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    const int col = blockIdx.x * kCols + k;
-    if (lane) continue;
-    if (col < D) {
-      if (dw) dw[col] = Elem<W>::store(static_cast<float>(t));
-    } else if (col < 2 * D) {
-      if (db) db[col - D] = Elem<W>::store(static_cast<float>(t));
-    }
+    if (lane == 0 && c0 + k < D) out[c0 + k] = Elem<W>::store(static_cast<float>(t));
   }
 }
 
@@ -668,9 +743,10 @@ __global__ void __launch_bounds__(256)
     sw = fmaf(d, (v - mean_in[r]) * rstd_in[r], sw);
     sb += d;
   }
-  float* p = partial + static_cast<int64_t>(slab) * 2 * D;
+  const int ld = partial_pitch(D);
+  float* p = partial + static_cast<int64_t>(slab) * 2 * ld;
   p[c] = sw;
-  p[D + c] = sb;
+  p[ld + c] = sb;
 }
 
 // ---- Host ---------------------------------------------------------------------------------
@@ -758,11 +834,11 @@ int64_t grid_for(uint64_t visits, int64_t per, int N, int64_t cap, int D) {
   return blocks;
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
 int run_forward(const Args& a, const Shape& s) {
-  auto kernel = forward_kernel<T, W, V, K, kBlock, N>;
+  auto kernel = forward_kernel<T, W, V, K, kBlock, N, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
-  const Ring ring = ring_for<Row<T, V, K>>(threads, K, N, 512 / threads, 0);
+  const Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, N, 512 / threads, 0);
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   const int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
@@ -773,23 +849,24 @@ int run_forward(const Args& a, const Shape& s) {
 }
 
 template <typename W>
-int run_join(const Args& a, int64_t n) {
+int run_join(const Args& a, int64_t n, int shift) {
   // eight columns a block until that makes more blocks than the device takes at once
-  const int64_t cols = 2 * static_cast<int64_t>(a.D);
-  const bool narrow = cols <= 8 * 296;
+  const bool narrow = a.D <= 8 * 148;
+  const int cols = narrow ? 8 : 32;
   return launch("layernorm gradient join", narrow ? join_kernel<W, 8> : join_kernel<W, 32>,
-                narrow ? (cols + 7) / 8 : (cols + 31) / 32, kJoinThreads, 0, a.st, true,
-                static_cast<const float*>(a.partial), static_cast<int>(n), a.D, static_cast<W*>(a.dw),
-                static_cast<W*>(a.db));
+                2 * ((static_cast<int64_t>(a.D) + cols - 1) / cols), kJoinThreads, 0, a.st, true,
+                static_cast<const float*>(a.partial), static_cast<int>(n), a.D, partial_pitch(a.D),
+                static_cast<uint32_t>(shift), static_cast<W*>(a.dw), static_cast<W*>(a.db));
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
 int run_backward(const Args& a, const Shape& s) {
-  auto kernel = backward_kernel<T, W, V, K, kBlock, N>;
+  auto kernel = backward_kernel<T, W, V, K, kBlock, N, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
   // a stage's statistics: 8 bytes a row for each warp or smaller group; the ring also joins the groups
-  Ring ring = ring_for<Row<T, V, K>>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N);
-  if (!kBlock && ring.bytes < 2 * a.D * 4) ring.bytes = 2 * a.D * 4;
+  Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N);
+  const int join_bytes = kGroupThreads / 32 * 2 * a.D * 4;
+  if (!kBlock && ring.bytes < join_bytes) ring.bytes = join_bytes;
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
@@ -801,7 +878,7 @@ int run_backward(const Args& a, const Shape& s) {
                      static_cast<const W*>(a.w), static_cast<const float*>(a.mean),
                      static_cast<const float*>(a.rstd), static_cast<T*>(a.dx), a.partial, a.D, s.G, ring.stages))
     return e;
-  return a.partial ? run_join<W>(a, blocks) : GTK_OK;
+  return a.partial ? run_join<W>(a, blocks, kBlock && kEdge ? V - 1 : 0) : GTK_OK;
 }
 
 template <typename T, typename W>
@@ -828,29 +905,37 @@ int run_wide(const Args& a, bool backward) {
                      static_cast<const float*>(a.mean), static_cast<const float*>(a.rstd), a.partial, rows, per, a.D,
                      col_blocks))
     return e;
-  return run_join<W>(a, slabs);
+  return run_join<W>(a, slabs, 0);
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
 int run_one(const Args& a, const Shape& s, bool backward) {
-  return backward ? run_backward<T, W, V, K, kBlock, N>(a, s) : run_forward<T, W, V, K, kBlock, N>(a, s);
+  return backward ? run_backward<T, W, V, K, kBlock, N, kEdge>(a, s) : run_forward<T, W, V, K, kBlock, N, kEdge>(a, s);
+}
+
+// Vectors of 16 bytes.
+template <typename T, typename W, bool kEdge>
+int run_vectors(const Args& a, const Shape& s, bool backward) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if (s.thirty_two) return run_one<T, W, V, 32 / V, true, 1, kEdge>(a, s, backward);
+  if (!s.block) return run_one<T, W, V, 16 / V, false, 1, kEdge>(a, s, backward);
+  // two rows a turn, once there are more rows than blocks
+  if (a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G))
+    return run_one<T, W, V, 16 / V, true, 1, kEdge>(a, s, backward);
+  return run_one<T, W, V, 16 / V, true, 2, kEdge>(a, s, backward);
 }
 
 template <typename T, typename W>
 int run_typed(const Args& a, bool vec, bool backward) {
-  constexpr int VX = 16 / static_cast<int>(sizeof(T));
   const Shape s = choose(a.D);
   if (s.wide) return run_wide<T, W>(a, backward);
   if (vec) {
-    if (s.thirty_two) return run_one<T, W, VX, 32 / VX, true, 1>(a, s, backward);
-    if (!s.block) return run_one<T, W, VX, 16 / VX, false, 1>(a, s, backward);
-    // two rows a turn, once there are more rows than blocks
-    if (a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G)) return run_one<T, W, VX, 16 / VX, true, 1>(a, s, backward);
-    return run_one<T, W, VX, 16 / VX, true, 2>(a, s, backward);
+    const bool edge = a.D % (16 / static_cast<int>(sizeof(T))) != 0;
+    return edge ? run_vectors<T, W, true>(a, s, backward) : run_vectors<T, W, false>(a, s, backward);
   }
-  if (s.thirty_two) return run_one<T, W, 1, 32, true, 1>(a, s, backward);
-  if (s.block) return run_one<T, W, 1, 16, true, 1>(a, s, backward);
-  return run_one<T, W, 1, 16, false, 1>(a, s, backward);
+  if (s.thirty_two) return run_one<T, W, 1, 32, true, 1, false>(a, s, backward);
+  if (s.block) return run_one<T, W, 1, 16, true, 1, false>(a, s, backward);
+  return run_one<T, W, 1, 16, false, 1, false>(a, s, backward);
 }
 
 int run(const Args& a, int xt, int wt, bool vec, bool backward) {
@@ -868,7 +953,7 @@ int row_map(const gtk_rows* v, const void* base, int64_t rows, int64_t D, size_t
             bool* vec) {
   if (!aligned16(base)) *vec = false;
   if (!v) {
-    *out = RowMap{0, 0, D, 0, 0};
+    *out = RowMap{0, 0, D, divisor(1), divisor(1), true};
     return GTK_OK;
   }
   if ((D * bytes) % 16) *vec = false;
@@ -880,20 +965,21 @@ int row_map(const gtk_rows* v, const void* base, int64_t rows, int64_t D, size_t
   }
   if (v->size[0] * v->size[1] > rows || v->size[0] * v->size[1] * v->size[2] != rows)
     return fail(GTK_ERR_INVALID_ARG, std::string("layernorm: the leading sizes of ") + what + " do not make up rows");
-  *out = RowMap{v->stride[0], v->stride[1], v->stride[2], static_cast<uint32_t>(v->size[1]),
-                static_cast<uint32_t>(v->size[2])};
+  *out = RowMap{v->stride[0], v->stride[1], v->stride[2], divisor(static_cast<uint32_t>(v->size[1])),
+                divisor(static_cast<uint32_t>(v->size[2])), false};
   return GTK_OK;
 }
 
 // Tiles where a tensor's rows lie closer along its second axis than along its third.
 Order order_for(int64_t rows, const RowMap& a, const RowMap* b) {
-  Order o = {0, 0, 0, 0, static_cast<uint64_t>(rows)};
+  Order o = {divisor(1), divisor(1), 0, 0, static_cast<uint64_t>(rows), false};
   for (const RowMap* m : {&a, b}) {
-    if (!m || m->n2 < 4 || m->n1 < 8 || m->s1 >= m->s2) continue;
-    const uint64_t t1 = (m->n1 + 7) / 8, t2 = (m->n2 + 3) / 4, planes = rows / (static_cast<uint64_t>(m->n1) * m->n2);
-    if (planes * t1 * t2 > (uint64_t(1) << 31)) continue;
-    o = Order{m->n1, m->n2, static_cast<uint32_t>(t1), static_cast<uint32_t>(t2), planes * t1 * t2 * 32};
-    break;
+    if (!m || m->plain || m->n2.d < 4 || m->n1.d < 8 || m->s1 >= m->s2) continue;
+    const uint64_t t1 = (m->n1.d + 7) / 8, t2 = (m->n2.d + 3) / 4;
+    const uint64_t planes = rows / (static_cast<uint64_t>(m->n1.d) * m->n2.d);
+    if (planes * t1 * t2 >= (uint64_t(1) << 31)) continue;
+    return Order{divisor(static_cast<uint32_t>(t1)), divisor(static_cast<uint32_t>(t2)), m->n1.d, m->n2.d,
+                 planes * t1 * t2 * 32, true};
   }
   return o;
 }
@@ -917,7 +1003,7 @@ extern "C" {
 
 size_t gtk_layernorm_backward_workspace_bytes(int64_t rows, int64_t D) {
   if (!dims_ok(rows, (int64_t(1) << 31) - 1) || !dims_ok(D, ln::kMaxWidth)) return 0;
-  return static_cast<size_t>(ln::max_partials(rows, D)) * 2 * D * sizeof(float);
+  return static_cast<size_t>(ln::max_partials(rows, D)) * 2 * ln::partial_pitch(static_cast<int>(D)) * sizeof(float);
 }
 
 int gtk_layernorm_forward(const void* x, const gtk_rows* x_rows, int x_dtype, const void* weight, const void* bias,
