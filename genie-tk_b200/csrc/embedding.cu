@@ -16,8 +16,9 @@
 // that cross chunks are joined in the block, and those that cross blocks from a scratch buffer
 // of at most two rows a block, by a last kernel and in order. Rows of tokens that do not occur are
 // zeroed by further blocks of the same launch, which look them up in the sorted keys.
-// No atomics on floating-point values: the same inputs give the same bits. Sums are fp32 in a
-// chunk (at most 1024 rows, by fours) and 64-bit between chunks; dW is rounded once.
+// No atomics on floating-point values: the same inputs give the same bits. Sums are fp32, of at
+// most 1024 rows one after another (by fours) and of partial rows in trees, and dW is rounded once.
+// (64-bit additions between the chunks took twice the time of the joining kernel.)
 #include <cooperative_groups.h>
 
 #include "train_common.cuh"
@@ -273,11 +274,19 @@ __global__ void __launch_bounds__(kSortThreads)
   const int bins = 1 << bits, slices = kSortThreads >> bits;
   const int bin = threadIdx.x & (bins - 1), slice = threadIdx.x >> bits;
   uint32_t before = 0, total = 0;
-#pragma unroll 8
-  for (int t = slice; t < tiles; t += slices) {
-    const uint32_t n = counts[static_cast<int64_t>(t) * kBins + bin];
-    total += n;
-    before += t < static_cast<int>(blockIdx.x) ? n : 0;
+  constexpr int kAtOnce = 8;
+  for (int t0 = slice; t0 < tiles; t0 += slices * kAtOnce) {
+    uint32_t n[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int t = t0 + u * slices;
+      n[u] = t < tiles ? counts[static_cast<int64_t>(t) * kBins + bin] : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      total += n[u];
+      before += t0 + u * slices < static_cast<int>(blockIdx.x) ? n[u] : 0u;
+    }
   }
   before_part[threadIdx.x] = before;
   total_part[threadIdx.x] = total;
@@ -488,28 +497,28 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
   for (int x = threadIdx.x; x < 32 * V; x += kSumThreads) {
     const int c = slab * 32 * V + x;
     if (c >= D) continue;
-    double acc = 0.0;
+    float acc = 0.f;
     bool carrying = false, began_here = false;
     for (int w = 0; w < kSumWarps; ++w) {
       const uint32_t f = how[w];
       if (f & kHead) {
-        acc += static_cast<double>(edge[w][0][x]);
+        acc += edge[w][0][x];
         carrying = true;
         if (!(f & kHeadOn)) {
           if (began_here)
-            dw[static_cast<int64_t>(run_key[w]) * D + c] = Elem<W>::store(static_cast<float>(acc * scale));
+            dw[static_cast<int64_t>(run_key[w]) * D + c] = Elem<W>::store(acc * scale);
           else
-            partial[unit * 2 * D + c] = static_cast<float>(acc);
-          acc = 0.0;
+            partial[unit * 2 * D + c] = acc;
+          acc = 0.f;
           carrying = began_here = false;
         }
       }
       if (f & kTail) {
-        acc = static_cast<double>(edge[w][1][x]);
+        acc = edge[w][1][x];
         carrying = began_here = true;
       }
     }
-    if (carrying) partial[(unit * 2 + (began_here ? 1 : 0)) * D + c] = static_cast<float>(acc);
+    if (carrying) partial[(unit * 2 + (began_here ? 1 : 0)) * D + c] = acc;
   }
 }
 
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     join_runs_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, W* __restrict__ dw,
                      int64_t n, uint32_t vocab, int D, int64_t unit_len, int slabs, float scale) {
   wait_previous_kernel();
-  __shared__ double part[kJoinWarps][kJoinCols];
+  __shared__ float part[kJoinWarps][kJoinCols];
   const int64_t u = blockIdx.x / static_cast<uint32_t>(slabs);
   const int col0 = static_cast<int>(blockIdx.x - u * slabs) * kJoinCols;
   const int64_t i0 = u * unit_len, i1 = i0 + unit_len;
@@ -579,23 +588,34 @@ __global__ void __launch_bounds__(kJoinThreads)
     count = __syncthreads_count(j < n && keys[j] == k);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double s[kJoinCols / 32] = {};
-#pragma unroll 8
-  for (int64_t j = warp; j <= heads; j += kJoinWarps) {  // 0: the tail, then the heads
-    const float* p = partial + (j == 0 ? u * 2 + 1 : (u + j) * 2) * D + col0 + lane;
+  float s[kJoinCols / 32] = {};
+  constexpr int kAtOnce = 8;
+  for (int64_t j0 = warp; j0 <= heads; j0 += kJoinWarps * kAtOnce) {  // 0: the tail, then the heads
+    float t[kAtOnce][kJoinCols / 32];
+#pragma unroll
+    for (int v = 0; v < kAtOnce; ++v) {
+      const int64_t j = j0 + v * kJoinWarps;
+      const float* p = partial + (j == 0 ? u * 2 + 1 : (u + j) * 2) * D + col0 + lane;
+#pragma unroll
+      for (int i = 0; i < kJoinCols / 32; ++i) t[v][i] = j <= heads && col0 + lane + 32 * i < D ? p[32 * i] : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < kJoinCols / 32; ++i)
-      if (col0 + lane + 32 * i < D) s[i] += static_cast<double>(p[32 * i]);
+      s[i] += ((t[0][i] + t[1][i]) + (t[2][i] + t[3][i])) + ((t[4][i] + t[5][i]) + (t[6][i] + t[7][i]));
   }
 #pragma unroll
   for (int i = 0; i < kJoinCols / 32; ++i) part[warp][lane + 32 * i] = s[i];
   __syncthreads();
   const int c = col0 + threadIdx.x;
   if (threadIdx.x >= kJoinCols || c >= D) return;
-  double t = part[0][threadIdx.x];
+  float t[kJoinWarps];
 #pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) t += part[w][threadIdx.x];
-  dw[static_cast<int64_t>(k) * D + c] = Elem<W>::store(static_cast<float>(t * scale));
+  for (int w = 0; w < kJoinWarps; ++w) t[w] = part[w][threadIdx.x];
+#pragma unroll
+  for (int o = kJoinWarps / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int w = 0; w < o; ++w) t[w] += t[w + o];
+  dw[static_cast<int64_t>(k) * D + c] = Elem<W>::store(t[0] * scale);
 }
 
 // ---- Forward ----------------------------------------------------------------------------------
@@ -716,28 +736,14 @@ int sort_cluster(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), smem)) return e;
   int blocks = 1;
   while (static_cast<int64_t>(blocks) * kSortThreads * N < a.T) blocks <<= 1;
-  cudaLaunchConfig_t cfg = {};
   const int64_t zero_bytes = p.zero_first ? a.dw_bytes : 0;
   // two blocks per SM, in whole clusters, but no more than there are 64 KB pieces
   int64_t zero_blocks = (zero_bytes + 65535) / 65536;
   if (zero_blocks > 2 * num_sms()) zero_blocks = 2 * num_sms();
   zero_blocks = (zero_blocks + blocks - 1) / blocks * blocks;
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks + zero_blocks));
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = a.st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(a.tokens), static_cast<int>(a.T),
-                                           static_cast<uint32_t>(a.vocab), a.padding, p.passes, p.bits, keys, pos,
-                                           static_cast<uint4*>(a.dw), zero_bytes, a.status);
-  if (e == cudaSuccess) return GTK_OK;
-  cudaGetLastError();
-  return fail(GTK_ERR_CUDA, std::string("embedding token sort: ") + cudaGetErrorString(e));
+  return launch_clusters("embedding token sort", kernel, blocks + zero_blocks, kSortThreads, smem, blocks, a.st,
+                         static_cast<const I*>(a.tokens), static_cast<int>(a.T), static_cast<uint32_t>(a.vocab),
+                         a.padding, p.passes, p.bits, keys, pos, static_cast<uint4*>(a.dw), zero_bytes, a.status);
 }
 
 template <typename I>

@@ -224,9 +224,15 @@ __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoars
 
 // The norm from all blocks' partials, the same in every block.
 __device__ __forceinline__ double total_norm(const double* partial, int n, bool inf_norm) {
+  constexpr int kAtOnce = (kMaxBlocks + kThreads - 1) / kThreads;  // all of one launch
   double v = 0.0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += kThreads) v = join(v, partial[i], inf_norm);
+  for (int i0 = threadIdx.x; i0 < n; i0 += kThreads * kAtOnce) {
+    double t[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) t[u] = i0 + u * kThreads < n ? partial[i0 + u * kThreads] : 0.0;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) v = join(v, t[u], inf_norm);
+  }
   v = block_total(v, inf_norm);
   return inf_norm ? static_cast<double>(__uint_as_float(static_cast<uint32_t>(__double_as_longlong(v)))) : sqrt(v);
 }

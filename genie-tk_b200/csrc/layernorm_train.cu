@@ -81,7 +81,7 @@ struct RowMap {
 struct Order {
   Divisor t1, t2;
   uint32_t n1, n2;
-  uint64_t visits;
+  uint32_t visits;  // below 2^31
   bool tiled;
 };
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -91,17 +91,17 @@ struct Place {
   uint32_t r, a, b, c;
 };
 
-__device__ __forceinline__ Place place_at(const Order& o, uint64_t v) {
+__device__ __forceinline__ Place place_at(const Order& o, uint32_t v) {
   Place p = {kNoRow, 0, 0, 0};
   if (v >= o.visits) return p;
   if (!o.tiled) {
-    p.r = static_cast<uint32_t>(v);
+    p.r = v;
     return p;
   }
-  const uint32_t tile = static_cast<uint32_t>(v >> 5), t = o.t2.quotient(tile);
+  const uint32_t tile = v >> 5, t = o.t2.quotient(tile);
   p.a = o.t1.quotient(t);
-  p.b = (t - p.a * o.t1.d) * 8 + (static_cast<uint32_t>(v) & 7u);
-  p.c = (tile - t * o.t2.d) * 4 + (static_cast<uint32_t>(v >> 3) & 3u);
+  p.b = (t - p.a * o.t1.d) * 8 + (v & 7u);
+  p.c = (tile - t * o.t2.d) * 4 + (v >> 3 & 3u);
   if (p.b < o.n1 && p.c < o.n2) p.r = (p.a * o.n1 + p.b) * o.n2 + p.c;
   return p;
 }
@@ -127,8 +127,9 @@ __device__ __forceinline__ void group_sum(float (&v)[n], int G) {
 }
 
 // Sums of n = 1, 2 or 4 values over the block (at most 16 warps). The values are spread over the
-// lanes as they are added up, 5 or 6 shuffles for all of them. `buf` alternates between two
-// halves, so that one barrier per reduction is enough.
+// lanes as they are added up, so that all of them take 5 or 6 shuffles in the warp and, behind the
+// barrier, 4 or 5 over the warps and n to hand them out. `buf` (two halves of 64 floats, zeros at
+// first) alternates, so that one barrier per reduction is enough.
 template <int n>
 __device__ __forceinline__ void block_sum(float (&v)[n], float* buf, int& half) {
   const int lane = threadIdx.x & 31;
@@ -154,21 +155,19 @@ __device__ __forceinline__ void block_sum(float (&v)[n], float* buf, int& half) 
   constexpr int kEach = 32 / n;  // lanes that hold one value
   if (lane % kEach == 0) s[(threadIdx.x >> 5) * n + lane / kEach] = x;
   __syncthreads();
-  const int nw = blockDim.x >> 5;
+  // lane = (warp, value), values fastest
+  x = s[n == 1 ? (lane & 15) : lane];
+  if constexpr (n == 4) x += s[32 + lane];
 #pragma unroll
-  for (int i = 0; i < n; ++i) v[i] = 0.f;
-#pragma unroll 4
-  for (int w = 0; w < nw; ++w) {
-    if constexpr (n == 4) {
-      const float4 t = reinterpret_cast<const float4*>(s)[w];
-      v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
-    } else if constexpr (n == 2) {
-      const float2 t = reinterpret_cast<const float2*>(s)[w];
-      v[0] += t.x, v[1] += t.y;
-    } else {
-      v[0] += s[w];
-    }
-  }
+  for (int o = n == 4 ? 16 : n == 2 ? 16 : 8; o >= n; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+#pragma unroll
+  for (int i = 0; i < n; ++i) v[i] = n == 1 ? x : __shfl_sync(0xffffffffu, x, i);
+}
+
+// Zeros in the buffers of block_sum.
+__device__ __forceinline__ void block_sum_init(float* buf) {
+  for (int i = threadIdx.x; i < 128; i += blockDim.x) buf[i] = 0.f;
+  __syncthreads();
 }
 
 // How a group's vectors lie over its rows: vector i covers the columns i V - lead .. + V - 1. kEdge:
@@ -192,12 +191,10 @@ struct Row {
   const char* slot;
   int pitch;
 
-  // `p`: the row's first element. The last vector reads no further than the row; the first one
-  // begins with up to V - 1 elements of the row before.
-  static __device__ __forceinline__ void request(char* slot, int pitch, const T* p, const L& l) {
+  // `from`: where the thread's first vector begins in the row. The last vector reads no further than
+  // the row; the first one begins with up to V - 1 elements of the row before.
+  static __device__ __forceinline__ void request(uint32_t to, int pitch, const T* from, const L& l) {
     if constexpr (kAsync) {
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
-      const T* from = p - l.lead() + l.lane * V;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int i = l.lane + l.G * k;
@@ -255,30 +252,29 @@ struct Row {
   }
 };
 
-// Stores the thread's elements of a row; the first and last vector by element where the row
-// begins or ends inside.
+// Stores the thread's elements of a row, `from` where its first vector begins; the row's first and last
+// vector by element where the row begins or ends inside.
 template <typename T, int V, int K, bool kEdge>
-__device__ __forceinline__ void store_row(T* p, const float2 (&f)[K * V / 2], const Lay<kEdge>& l) {
+__device__ __forceinline__ void store_row(T* from, const float2 (&f)[K * V / 2], const Lay<kEdge>& l) {
   if constexpr (V == 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = l.lane + l.G * k;
-      if (c < l.D) p[c] = Elem<T>::store(k & 1 ? f[k / 2].y : f[k / 2].x);
-    }
+    for (int k = 0; k < K; ++k)
+      if (l.lane + l.G * k < l.D) from[l.G * k] = Elem<T>::store(k & 1 ? f[k / 2].y : f[k / 2].x);
   } else {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = l.lane + l.G * k, c = i * V - l.lead();
       if (i >= l.nv) continue;
+      T* p = from + l.G * k * V;
       float o[V];
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) o[2 * j] = f[k * (V / 2) + j].x, o[2 * j + 1] = f[k * (V / 2) + j].y;
       if (!kEdge || (c >= 0 && c + V <= l.D)) {
-        st_vec<T, V>(p + c, Vec<T, V>::of(o));
+        st_vec<T, V>(p, Vec<T, V>::of(o));
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (c + j >= 0 && c + j < l.D) p[c + j] = Elem<T>::store(o[j]);
+          if (c + j >= 0 && c + j < l.D) p[j] = Elem<T>::store(o[j]);
       }
     }
   }
@@ -341,47 +337,78 @@ __device__ __forceinline__ void zero_missing(char* mine, int pitch, int rows, co
       if (l.lane + l.G * k >= l.nv) *reinterpret_cast<uint4*>(mine + (r * K + k) * pitch) = make_uint4(0, 0, 0, 0);
 }
 
+// The rows of a tensor in visiting order, for one thread: addresses of its first vector. kPlain: one
+// row follows the other, so the address moves by a fixed step; else it is computed for each row.
+template <typename T, int V, bool kPlain, bool kEdge>
+struct Rows {
+  T* at;         // kPlain: of the next visit asked for
+  int64_t step;  // elements from a visit of the group to its next
+  __device__ __forceinline__ Rows(T* base, const RowMap& m, uint32_t first, uint32_t visits_apart, const Lay<kEdge>& l) {
+    at = base + (kPlain ? static_cast<int64_t>(first) * l.D : 0) - l.lead() + l.lane * V;
+    step = static_cast<int64_t>(visits_apart) * l.D;
+  }
+  __device__ __forceinline__ T* row(int q, const RowMap& m, const Order& o, const Place& p) const {
+    return at + (kPlain ? q * step : row_offset(m, o, p));
+  }
+  __device__ __forceinline__ void advance(int n) {
+    if (kPlain) at += n * step;
+  }
+};
+
+template <bool kPlain>
+__device__ __forceinline__ Place visit(const Order& o, uint32_t v) {
+  if constexpr (kPlain) return Place{v < o.visits ? v : kNoRow, 0, 0, 0};
+  return place_at(o, v);
+}
+
 // Forward. kBlock: the block is one group of blockDim.x threads; else groups of G <= 32. A turn of
 // the loop takes N rows of each group.
-template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     forward_kernel(const T* __restrict__ x, RowMap xm, Order order, const W* __restrict__ w,
                    const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean_out,
                    float* __restrict__ rstd_out, int D, int G, int stages, float eps) {
   extern __shared__ __align__(16) char ring[];
-  __shared__ __align__(16) float red[128];
+  __shared__ float red[128];
   using R = Row<T, V, K, kEdge>;
   using L = Lay<kEdge>;
   constexpr int P = K * V / 2;
   int half = 0;
-  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
-  const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
-  const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
-  const int lead = kEdge ? static_cast<int>(first * D & (V - 1)) : 0;
+  const uint32_t per_block = kBlock ? 1u : blockDim.x / G;
+  const uint32_t block_first = blockIdx.x * per_block;
+  const uint32_t first = kBlock ? block_first : block_first + threadIdx.x / G;
+  const uint32_t step = gridDim.x * per_block;
+  const int lead = kEdge ? static_cast<int>(first * static_cast<uint32_t>(D) & (V - 1)) : 0;
   const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
-                 (lead + D + V - 1) / V, lead, D};
-  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch;
+               (lead + D + V - 1) / V, lead, D};
+  const bool full = l.nv >= l.G * K;  // every vector of the thread exists
+  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch, stage_bytes = N * row_bytes;
   char* mine = ring + threadIdx.x * R::kBytes;
+  const uint32_t mine_at = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
   const float inv_d = 1.0f / static_cast<float>(D);
+  const RowMap ym = {0, 0, D, {}, {}, true};
+  Rows<const T, V, kPlain, kEdge> from(x, xm, first, step, l);
+  Rows<T, V, true, kEdge> to(y, ym, kPlain ? first : 0, step, l);
   zero_missing<T, V, K>(mine, pitch, stages * N, l);
-  auto request = [&](int s, uint64_t v) {
+  auto request = [&](int slot, uint32_t v) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const Place at = place_at(order, v + q * step);
-      if (at.r != kNoRow)
-        R::request(mine + (s * N + q) * row_bytes, pitch, x + row_offset(xm, order, at), l);
+      const Place at = visit<kPlain>(order, v + q * step);
+      if (at.r != kNoRow) R::request(mine_at + slot + q * row_bytes, pitch, from.row(q, xm, order, at), l);
     }
+    from.advance(N);
     commit_copies();
   };
+  const int last_slot = (stages - 1) * stage_bytes;
   if constexpr (R::kAsync)
-    for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+    for (int s = 0; s + 1 < stages; ++s) request(s * stage_bytes, first + s * (N * step));
   const Columns<W, V, K, kEdge> wc(w, 1.f, l), bc(b, 0.f, l);
-  int now = 0;
+  if constexpr (kBlock) block_sum_init(red);
+  int now = 0;  // the slot of this turn, in bytes
   // every group of the block makes the same number of turns, so that shuffles and barriers meet
-  for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
+  for (uint32_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
     if constexpr (R::kAsync) {
-      request(now ? now - 1 : stages - 1, v0 + (stages - 1) * (N * step));
+      request(now ? now - stage_bytes : last_slot, v0 + (stages - 1) * (N * step));
       wait_copies(stages);
     }
     uint32_t r[N];
@@ -389,18 +416,23 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
     float s[N], sq[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      r[q] = place_at(order, v0 + q * step).r;
-      L lq = l;
-      if (r[q] == kNoRow) lq.nv = 0;
+      const Place at = visit<kPlain>(order, v0 + q * step);
+      r[q] = at.r;
       R row;
-      row.open(mine + (now * N + q) * row_bytes, pitch, x + row_offset(xm, r[q] == kNoRow ? 0u : r[q]), lq);
+      if constexpr (R::kAsync) {
+        row.open(mine + now + q * row_bytes, pitch, nullptr, l);
+      } else {
+        L lq = l;
+        if (r[q] == kNoRow) lq.nv = 0;
+        row.open(nullptr, 0, r[q] == kNoRow ? x : x + row_offset(xm, order, at), lq);
+      }
       row.pairs(v[q], l);
       float2 t = make_float2(0.f, 0.f);
 #pragma unroll
       for (int p = 0; p < P; ++p) t = add2(t, v[q][p]);
       s[q] = t.x + t.y;
     }
-    now = now + 1 < stages ? now + 1 : 0;
+    now = now == last_slot ? 0 : now + stage_bytes;
     if constexpr (kBlock)
       block_sum<N>(s, red, half);
     else
@@ -408,25 +440,19 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       s[q] *= inv_d;
+#pragma unroll
+      for (int p = 0; p < P; ++p) v[q][p] = add2(v[q][p], both(-s[q]));
+      if (kEdge || !full) {  // elements that do not exist have no deviation
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const int c = column_of<V, kEdge>(2 * p, l), c2 = column_of<V, kEdge>(2 * p + 1, l);
+          if (c < 0 || c >= D) v[q][p].x = 0.f;
+          if (c2 < 0 || c2 >= D) v[q][p].y = 0.f;
+        }
+      }
       float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        v[q][p] = add2(v[q][p], both(-s[q]));
-        if constexpr (V == 1) {  // elements that do not exist have no deviation
-          if (column_of<V, kEdge>(2 * p, l) >= D) v[q][p].x = 0.f;
-          if (column_of<V, kEdge>(2 * p + 1, l) >= D) v[q][p].y = 0.f;
-        } else if constexpr (!kEdge) {
-          if (l.lane + l.G * (2 * p / V) >= l.nv) v[q][p] = make_float2(0.f, 0.f);
-        } else {
-          const int c = column_of<V, kEdge>(2 * p / V * V, l);
-          if (c < 0 || c + V > D) {
-            const int c2 = column_of<V, kEdge>(2 * p, l);
-            if (c2 < 0 || c2 >= D) v[q][p].x = 0.f;
-            if (c2 + 1 < 0 || c2 + 1 >= D) v[q][p].y = 0.f;
-          }
-        }
-        t = fma2(v[q][p], v[q][p], t);
-      }
+      for (int p = 0; p < P; ++p) t = fma2(v[q][p], v[q][p], t);
       sq[q] = t.x + t.y;
     }
     if constexpr (kBlock)
@@ -439,69 +465,80 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
       const float rstd = 1.0f / sqrtf(sq[q] * inv_d + eps);
 #pragma unroll
       for (int p = 0; p < P; ++p) v[q][p] = fma2(mul2(v[q][p], both(rstd)), wc.get(p, l), bc.get(p, l));
-      store_row<T, V, K, kEdge>(y + static_cast<int64_t>(r[q]) * D, v[q], l);
+      store_row<T, V, K, kEdge>(kPlain ? to.at + q * to.step : to.at + static_cast<int64_t>(r[q]) * D, v[q], l);
       if (l.lane == 0) {
         mean_out[r[q]] = s[q];
         rstd_out[r[q]] = rstd;
       }
     }
+    if (kPlain) to.advance(N);
   }
 }
 
 // Backward: dx and, per block, one partial row [dw | db] of 2 D floats. The ring's stage holds N
 // x rows, N dy rows and, for each warp (group, where that is smaller), their mean and rstd.
-template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBlock ? 1 : 2)
     backward_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm, Order order,
                     const W* __restrict__ w, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                     T* __restrict__ dx, float* __restrict__ partial, int D, int G, int stages) {
   extern __shared__ __align__(16) char ring[];
-  __shared__ __align__(16) float red[128];
+  __shared__ float red[128];
   using R = Row<T, V, K, kEdge>;
   using L = Lay<kEdge>;
   constexpr int P = K * V / 2;
   int half = 0;
-  const uint32_t per_block = kBlock ? 1u : static_cast<uint32_t>(blockDim.x / G);
-  const uint64_t block_first = static_cast<uint64_t>(blockIdx.x) * per_block;
-  const uint64_t first = kBlock ? block_first : block_first + threadIdx.x / G;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * per_block;
-  const int lead = kEdge ? static_cast<int>(first * D & (V - 1)) : 0;
+  const uint32_t per_block = kBlock ? 1u : blockDim.x / G;
+  const uint32_t block_first = blockIdx.x * per_block;
+  const uint32_t first = kBlock ? block_first : block_first + threadIdx.x / G;
+  const uint32_t step = gridDim.x * per_block;
+  const int lead = kEdge ? static_cast<int>(first * static_cast<uint32_t>(D) & (V - 1)) : 0;
   const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
-                 (lead + D + V - 1) / V, lead, D};
-  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch, stage_bytes = 2 * N * row_bytes;
+               (lead + D + V - 1) / V, lead, D};
+  const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch;
   const int share = kBlock ? 32 : G;  // threads that share a copy of the statistics
+  const int stats_stage = blockDim.x / share * 2 * N * 4;  // bytes
+  const int stage_bytes = 2 * N * row_bytes;
   char* mine = ring + threadIdx.x * R::kBytes;
-  float* stats = reinterpret_cast<float*>(ring + stages * stage_bytes) + threadIdx.x / share * 2 * N;
-  const int stats_stage = blockDim.x / share * 2 * N;
+  const uint32_t mine_at = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+  char* stats = ring + stages * stage_bytes + threadIdx.x / share * (2 * N * 4);
+  const uint32_t stats_at = static_cast<uint32_t>(__cvta_generic_to_shared(stats));
+  const bool leader = threadIdx.x % share == 0;
   const float inv_d = 1.0f / static_cast<float>(D);
+  const RowMap om = {0, 0, D, {}, {}, true};
+  Rows<const T, V, kPlain, kEdge> xs(x, xm, first, step, l), gs(dy, dm, first, step, l);
+  Rows<T, V, true, kEdge> to(dx, om, kPlain ? first : 0, step, l);
   zero_missing<T, V, K>(mine, pitch, stages * 2 * N, l);
   float2 aw[P], ab[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) aw[p] = ab[p] = make_float2(0.f, 0.f);
-  auto request = [&](int s, uint64_t v) {
+  auto request = [&](int slot, int stat, uint32_t v) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const Place at = place_at(order, v + q * step);
-      const uint32_t r = at.r;
-      if (r == kNoRow) continue;
-      char* to = mine + s * stage_bytes + 2 * q * row_bytes;
-      R::request(to, pitch, x + row_offset(xm, order, at), l);
-      R::request(to + row_bytes, pitch, dy + row_offset(dm, order, at), l);
-      if (threadIdx.x % share == 0) {
-        const uint32_t st = static_cast<uint32_t>(__cvta_generic_to_shared(stats + s * stats_stage + 2 * q));
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st), "l"(mean_in + r) : "memory");
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + 4), "l"(rstd_in + r) : "memory");
+      const Place at = visit<kPlain>(order, v + q * step);
+      if (at.r == kNoRow) continue;
+      R::request(mine_at + slot + 2 * q * row_bytes, pitch, xs.row(q, xm, order, at), l);
+      R::request(mine_at + slot + (2 * q + 1) * row_bytes, pitch, gs.row(q, dm, order, at), l);
+      if (leader) {
+        const uint32_t st = stats_at + stat + 8 * q;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st), "l"(mean_in + at.r) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + 4), "l"(rstd_in + at.r) : "memory");
       }
     }
+    xs.advance(N);
+    gs.advance(N);
     commit_copies();
   };
+  const int last_slot = (stages - 1) * stage_bytes, last_stat = (stages - 1) * stats_stage;
   if constexpr (R::kAsync)
-    for (int s = 0; s + 1 < stages; ++s) request(s, first + s * (N * step));
+    for (int s = 0; s + 1 < stages; ++s) request(s * stage_bytes, s * stats_stage, first + s * (N * step));
   const Columns<W, V, K, kEdge> wc(w, 1.f, l);
-  int now = 0;
-  for (uint64_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
+  if constexpr (kBlock) block_sum_init(red);
+  int now = 0, stat = 0;  // the slots of this turn, in bytes
+  for (uint32_t base = block_first, v0 = first; base < order.visits; base += N * step, v0 += N * step) {
     if constexpr (R::kAsync) {
-      request(now ? now - 1 : stages - 1, v0 + (stages - 1) * (N * step));
+      request(now ? now - stage_bytes : last_slot, now ? stat - stats_stage : last_stat,
+              v0 + (stages - 1) * (N * step));
       wait_copies(stages);
       __syncwarp();  // the statistics come from the first lane's copies
     }
@@ -510,23 +547,25 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
     float mean[N], rstd[N], c[2 * N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      r[q] = place_at(order, v0 + q * step).r;
+      const Place at = visit<kPlain>(order, v0 + q * step);
+      r[q] = at.r;
       const bool valid = r[q] != kNoRow;
-      L lq = l;
-      if (!valid) lq.nv = 0;
       mean[q] = rstd[q] = 0.f;
       if constexpr (R::kAsync) {
+        const float2 st = *reinterpret_cast<const float2*>(stats + stat + 8 * q);
+        if (valid) mean[q] = st.x, rstd[q] = st.y;
+        xr[q].open(mine + now + 2 * q * row_bytes, pitch, nullptr, l);
+        gr[q].open(mine + now + (2 * q + 1) * row_bytes, pitch, nullptr, l);
+      } else {
+        L lq = l;
+        if (!valid) lq.nv = 0;
         if (valid) {
-          mean[q] = stats[now * stats_stage + 2 * q];
-          rstd[q] = stats[now * stats_stage + 2 * q + 1];
+          mean[q] = __ldg(mean_in + r[q]);
+          rstd[q] = __ldg(rstd_in + r[q]);
         }
-      } else if (valid) {
-        mean[q] = __ldg(mean_in + r[q]);
-        rstd[q] = __ldg(rstd_in + r[q]);
+        xr[q].open(nullptr, 0, valid ? x + row_offset(xm, order, at) : x, lq);
+        gr[q].open(nullptr, 0, valid ? dy + row_offset(dm, order, at) : dy, lq);
       }
-      const char* slot = mine + now * stage_bytes + 2 * q * row_bytes;
-      xr[q].open(slot, pitch, x + row_offset(xm, valid ? r[q] : 0u), lq);
-      gr[q].open(slot + row_bytes, pitch, dy + row_offset(dm, valid ? r[q] : 0u), lq);
       c[2 * q] = c[2 * q + 1] = 0.f;
       if (!valid) continue;
       float2 xp[P], gp[P], c1 = make_float2(0.f, 0.f), c2 = c1;
@@ -544,7 +583,6 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
       c[2 * q] = c1.x + c1.y;
       c[2 * q + 1] = c2.x + c2.y;
     }
-    now = now + 1 < stages ? now + 1 : 0;
     if constexpr (kBlock)
       block_sum<2 * N>(c, red, half);
     else
@@ -562,8 +600,11 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
         const float2 g = rounded_mul2(gp[p], wc.get(p, l));
         xp[p] = mul2(both(rstd[q]), fma2(xh, both(-c2), add2(g, both(-c1))));
       }
-      store_row<T, V, K, kEdge>(dx + static_cast<int64_t>(r[q]) * D, xp, l);
+      store_row<T, V, K, kEdge>(kPlain ? to.at + q * to.step : to.at + static_cast<int64_t>(r[q]) * D, xp, l);
     }
+    if (kPlain) to.advance(N);
+    now = now == last_slot ? 0 : now + stage_bytes;
+    stat = now ? stat + stats_stage : 0;
   }
   if (!partial) return;
   const int ld = partial_pitch(D);
@@ -627,7 +668,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
   }
 }
 
-// dw, db: the sum of `n` partial rows of two times `ld` floats, in a fixed order and 64 bits. Partial
+// dw, db: the sum of `n` partial rows of two times `ld` floats, in a fixed order, as a tree. Partial
 // row i holds column c at c + (i D mod V) (shift: V - 1, or 0). A warp covers kCols columns of
 // 32 / kCols rows at a time; blocks of dw come first, then those of db.
 template <typename W, int kCols>
@@ -636,7 +677,7 @@ __global__ void __launch_bounds__(kJoinThreads)
                 W* __restrict__ db) {
   wait_previous_kernel();
   constexpr int kWarps = kJoinThreads / 32, kRows = 32 / kCols;
-  __shared__ double part[kWarps][kCols];
+  __shared__ float part[kWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = (D + kCols - 1) / kCols;  // blocks
   const bool second = static_cast<int>(blockIdx.x) >= half;
@@ -644,12 +685,14 @@ __global__ void __launch_bounds__(kJoinThreads)
   W* out = second ? db : dw;
   if (!out) return;
   const int c = c0 + (lane & (kCols - 1));
-  double s = 0.0;
+  float s = 0.f;
   if (c < D) {
-    const float* p = partial + c + (second ? ld : 0);
-#pragma unroll 8
-    for (int i = warp * kRows + lane / kCols; i < n; i += kWarps * kRows)
-      s += static_cast<double>(p[static_cast<int64_t>(i) * 2 * ld + (static_cast<uint32_t>(i) * static_cast<uint32_t>(D) & shift)]);
+    constexpr int kStep = kWarps * kRows;  // a multiple of V: all rows of a thread lie alike
+    int i = warp * kRows + lane / kCols;
+    const int64_t row = 2 * static_cast<int64_t>(ld), apart = kStep * row;
+    const float* p = partial + c + (second ? ld : 0) + i * row + (static_cast<uint32_t>(i) * static_cast<uint32_t>(D) & shift);
+    for (; i + 3 * kStep < n; i += 4 * kStep, p += 4 * apart) s += (p[0] + p[apart]) + (p[2 * apart] + p[3 * apart]);
+    for (; i < n; i += kStep, p += apart) s += *p;
   }
 #pragma unroll
   for (int o = kCols; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -657,10 +700,10 @@ __global__ void __launch_bounds__(kJoinThreads)
   __syncthreads();
   // warp k adds column k over the warps
   for (int k = warp; k < kCols; k += kWarps) {
-    double t = part[lane][k];
+    float t = part[lane][k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0 && c0 + k < D) out[c0 + k] = Elem<W>::store(static_cast<float>(t));
+    if (lane == 0 && c0 + k < D) out[c0 + k] = Elem<W>::store(t);
   }
 }
 
@@ -671,7 +714,8 @@ __global__ void __launch_bounds__(kMaxBlockGroup)
     forward_wide_kernel(const T* __restrict__ x, RowMap xm, const W* __restrict__ w, const W* __restrict__ b,
                         T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, uint32_t rows,
                         int D, float eps) {
-  __shared__ __align__(16) float red[128];
+  __shared__ float red[128];
+  block_sum_init(red);
   int half = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -702,7 +746,8 @@ __global__ void __launch_bounds__(kMaxBlockGroup)
     backward_wide_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm,
                          const W* __restrict__ w, const float* __restrict__ mean_in,
                          const float* __restrict__ rstd_in, T* __restrict__ dx, uint32_t rows, int D) {
-  __shared__ __align__(16) float red[128];
+  __shared__ float red[128];
+  block_sum_init(red);
   int half = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -824,25 +869,26 @@ int64_t cached_residency(std::atomic<int64_t>* cache, F kernel, int threads, int
   return v;
 }
 
-// Blocks for `visits` rows in turns of N per group: all that fit the device at once; with a lead,
-// a multiple of eight rows apart (see the file comment).
-int64_t grid_for(uint64_t visits, int64_t per, int N, int64_t cap, int D) {
-  const int64_t need = static_cast<int64_t>((visits + static_cast<uint64_t>(per) * N - 1) / (per * N));
-  if (need <= cap && N == 1) return need;
-  int64_t blocks = need < cap ? need : cap;
-  if (per % 8 && D % 8 && blocks > 8) blocks &= ~int64_t(7);
-  return blocks;
+// Blocks for `visits` rows in turns of N per group: all that fit the device at once. `edge`: rows
+// begin inside vectors, so a group's rows have to lie a multiple of eight apart: either the
+// groups of all blocks together are one, or no group has a second row.
+int64_t grid_for(int64_t visits, int64_t per, int N, int64_t cap, bool edge) {
+  const int64_t turn = per * N;
+  int64_t blocks = (visits + turn - 1) / turn;
+  if (blocks > cap) blocks = cap;
+  if (!edge || per % 8 == 0) return blocks;
+  return blocks >= 8 ? blocks & ~int64_t(7) : visits;
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 int run_forward(const Args& a, const Shape& s) {
-  auto kernel = forward_kernel<T, W, V, K, kBlock, N, kEdge>;
+  auto kernel = forward_kernel<T, W, V, K, kBlock, N, kPlain, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
   const Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, N, 512 / threads, 0);
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   const int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
-  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, a.D);
+  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
   return launch("layernorm forward", kernel, blocks, threads, ring.bytes, a.st, false, static_cast<const T*>(a.x),
                 a.xm, a.order, static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean,
                 a.rstd, a.D, s.G, ring.stages, a.eps);
@@ -859,9 +905,9 @@ int run_join(const Args& a, int64_t n, int shift) {
                 static_cast<uint32_t>(shift), static_cast<W*>(a.dw), static_cast<W*>(a.db));
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 int run_backward(const Args& a, const Shape& s) {
-  auto kernel = backward_kernel<T, W, V, K, kBlock, N, kEdge>;
+  auto kernel = backward_kernel<T, W, V, K, kBlock, N, kPlain, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
   // a stage's statistics: 8 bytes a row for each warp or smaller group; the ring also joins the groups
   Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N);
@@ -872,7 +918,7 @@ int run_backward(const Args& a, const Shape& s) {
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
   const int64_t most = max_partials(a.rows, a.D);
   if (cap > most) cap = most;
-  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, a.D);
+  const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
   if (int e = launch("layernorm backward", kernel, blocks, threads, ring.bytes, a.st, false,
                      static_cast<const T*>(a.dy), a.dm, static_cast<const T*>(a.x), a.xm, a.order,
                      static_cast<const W*>(a.w), static_cast<const float*>(a.mean),
@@ -908,21 +954,22 @@ int run_wide(const Args& a, bool backward) {
   return run_join<W>(a, slabs, 0);
 }
 
-template <typename T, typename W, int V, int K, bool kBlock, int N, bool kEdge>
+template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 int run_one(const Args& a, const Shape& s, bool backward) {
-  return backward ? run_backward<T, W, V, K, kBlock, N, kEdge>(a, s) : run_forward<T, W, V, K, kBlock, N, kEdge>(a, s);
+  return backward ? run_backward<T, W, V, K, kBlock, N, kPlain, kEdge>(a, s)
+                  : run_forward<T, W, V, K, kBlock, N, kPlain, kEdge>(a, s);
 }
 
 // Vectors of 16 bytes.
-template <typename T, typename W, bool kEdge>
+template <typename T, typename W, bool kPlain, bool kEdge>
 int run_vectors(const Args& a, const Shape& s, bool backward) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  if (s.thirty_two) return run_one<T, W, V, 32 / V, true, 1, kEdge>(a, s, backward);
-  if (!s.block) return run_one<T, W, V, 16 / V, false, 1, kEdge>(a, s, backward);
+  if (s.thirty_two) return run_one<T, W, V, 32 / V, true, 1, kPlain, kEdge>(a, s, backward);
+  if (!s.block) return run_one<T, W, V, 16 / V, false, 1, kPlain, kEdge>(a, s, backward);
   // two rows a turn, once there are more rows than blocks
   if (a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G))
-    return run_one<T, W, V, 16 / V, true, 1, kEdge>(a, s, backward);
-  return run_one<T, W, V, 16 / V, true, 2, kEdge>(a, s, backward);
+    return run_one<T, W, V, 16 / V, true, 1, kPlain, kEdge>(a, s, backward);
+  return run_one<T, W, V, 16 / V, true, 2, kPlain, kEdge>(a, s, backward);
 }
 
 template <typename T, typename W>
@@ -930,12 +977,13 @@ int run_typed(const Args& a, bool vec, bool backward) {
   const Shape s = choose(a.D);
   if (s.wide) return run_wide<T, W>(a, backward);
   if (vec) {
-    const bool edge = a.D % (16 / static_cast<int>(sizeof(T))) != 0;
-    return edge ? run_vectors<T, W, true>(a, s, backward) : run_vectors<T, W, false>(a, s, backward);
+    const bool plain = a.xm.plain && (!backward || a.dm.plain);
+    if (a.D % (16 / static_cast<int>(sizeof(T)))) return run_vectors<T, W, true, true>(a, s, backward);
+    return plain ? run_vectors<T, W, true, false>(a, s, backward) : run_vectors<T, W, false, false>(a, s, backward);
   }
-  if (s.thirty_two) return run_one<T, W, 1, 32, true, 1, false>(a, s, backward);
-  if (s.block) return run_one<T, W, 1, 16, true, 1, false>(a, s, backward);
-  return run_one<T, W, 1, 16, false, 1, false>(a, s, backward);
+  if (s.thirty_two) return run_one<T, W, 1, 32, true, 1, false, false>(a, s, backward);
+  if (s.block) return run_one<T, W, 1, 16, true, 1, false, false>(a, s, backward);
+  return run_one<T, W, 1, 16, false, 1, false, false>(a, s, backward);
 }
 
 int run(const Args& a, int xt, int wt, bool vec, bool backward) {
@@ -972,14 +1020,14 @@ int row_map(const gtk_rows* v, const void* base, int64_t rows, int64_t D, size_t
 
 // Tiles where a tensor's rows lie closer along its second axis than along its third.
 Order order_for(int64_t rows, const RowMap& a, const RowMap* b) {
-  Order o = {divisor(1), divisor(1), 0, 0, static_cast<uint64_t>(rows), false};
+  Order o = {divisor(1), divisor(1), 0, 0, static_cast<uint32_t>(rows), false};
   for (const RowMap* m : {&a, b}) {
     if (!m || m->plain || m->n2.d < 4 || m->n1.d < 8 || m->s1 >= m->s2) continue;
     const uint64_t t1 = (m->n1.d + 7) / 8, t2 = (m->n2.d + 3) / 4;
     const uint64_t planes = rows / (static_cast<uint64_t>(m->n1.d) * m->n2.d);
-    if (planes * t1 * t2 >= (uint64_t(1) << 31)) continue;
+    if (planes * t1 * t2 * 32 >= (uint64_t(1) << 31)) continue;
     return Order{divisor(static_cast<uint32_t>(t1)), divisor(static_cast<uint32_t>(t2)), m->n1.d, m->n2.d,
-                 planes * t1 * t2 * 32, true};
+                 static_cast<uint32_t>(planes * t1 * t2 * 32), true};
   }
   return o;
 }

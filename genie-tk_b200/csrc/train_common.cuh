@@ -184,6 +184,27 @@ int launch(const char* what, void (*kernel)(KArgs...), int64_t blocks, int threa
   return GTK_OK;
 }
 
+// The same in clusters of `cluster` blocks (a divisor of `blocks`).
+template <typename... KArgs, typename... Args>
+int launch_clusters(const char* what, void (*kernel)(KArgs...), int64_t blocks, int threads, int smem, int cluster,
+                    cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  if (e == cudaSuccess) return GTK_OK;
+  cudaGetLastError();
+  return fail(GTK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
 // Resident blocks of `kernel` on the whole device.
 template <typename F>
 int64_t resident_blocks(F kernel, int threads, int smem) {

@@ -534,7 +534,7 @@ GTK_API int gtk_clip_grad_norm(const void* const* grads, void* const* outs, cons
  * type (dtype); dy [n_tokens, D] (dy_dtype), dweight [vocab, D] in GTK_F32 or dy's type, all of
  * it written. n_tokens, vocab < 2^31, D <= 2^20. The row `padding` (-1: none) of dweight is
  * zeros; the lookup reads it like any other. Tokens out of range set GTK_STATUS_BAD_TOKEN.
- * fp32 and 64-bit sums in a fixed order, one rounding at the end; no floating-point atomics:
+ * fp32 sums in a fixed order, one rounding at the end; no floating-point atomics:
  * the same inputs give the same bits. The workspace is aligned to 256 bytes.
  * ------------------------------------------------------------------------------- */
 GTK_API int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight, int dtype, void* y,

@@ -2,9 +2,10 @@
 gtk_embedding_backward) against sums in 64 bits.
 
 Tolerances, with u = 2^-24 and h the half step of the result's type: the lookup rounds the
-product once in fp32 and once in its type. In the gradient at most 1024 rows of a token are summed
-one after another in fp32, and these sums in 64 bits: (1024 + 8) u times the sum of magnitudes, or
-with n < 1024 occurrences (n + 8) u, and then the product with the scale and the rounding."""
+product once in fp32 and once in its type. In the gradient the n rows of a token are added in some
+fixed order: at most n - 1 roundings, whatever the order, and never more than 300 one on another
+(fours of at most 1024 rows, then trees): (min(n, 1024) + 8) u times the sum of magnitudes covers
+both, and then come the product with the scale and the rounding."""
 
 import pytest
 import torch
