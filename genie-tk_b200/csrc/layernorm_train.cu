@@ -50,8 +50,8 @@ constexpr int kMaxWidth = 1 << 20;
 constexpr int kGroupThreads = 256;  // block of the kernels whose groups are at most a warp
 constexpr int kMaxBlockGroup = 512;
 constexpr int kJoinThreads = 1024;
-constexpr int kMaxStages = 4;             // rows of the ring
-constexpr int kRingBytes = 200 * 1024;    // of an SM
+constexpr int kMaxStages = 2;             // turns in the ring: this one and the next
+constexpr int kRingBytes = 200 * 1024;    // most of an SM
 
 // Division of n < 2^31 by a constant of the launch.
 struct Divisor {
@@ -292,11 +292,7 @@ __host__ __device__ __forceinline__ int partial_pitch(int D) { return D % 8 ? (D
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the newest `stages` - 1 groups of this thread's copies have arrived.
 __device__ __forceinline__ void wait_copies(int stages) {
-  if (stages >= 4)
-    asm volatile("cp.async.wait_group 3;" ::: "memory");
-  else if (stages == 3)
-    asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else if (stages == 2)
+  if (stages >= 2)
     asm volatile("cp.async.wait_group 1;" ::: "memory");
   else
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -843,16 +839,22 @@ struct Args {
   cudaStream_t st;
 };
 
-// Stages of the ring and its bytes: as many as fit `sharing` blocks of an SM, four at most.
+// The ring: stages, bytes, and the blocks of an SM. What is on its way should be about what HBM
+// needs for its latency, 64 KB an SM; 16-bit rows take twice that, as their arithmetic takes longer.
+// More costs: reads far ahead of the writes leave the DRAM pages that the writes need (512 x 512 x
+// 128 fp32, forward / backward: 46 / 66 us with 64 KB an SM, 49 / 71 us with 200 KB; 4096 x 4096
+// bf16: 14.4 / 28.7 us, against 16.4 / 29.1 us).
 struct Ring {
-  int stages, bytes;
+  int stages, bytes, blocks;
 };
 template <typename R>
-Ring ring_for(int threads, int K, int tensors, int sharing, int extra) {
-  Ring r = {1, 0};
+Ring ring_for(int threads, int K, int tensors, int most_blocks, int extra, size_t elem_bytes) {
+  Ring r = {1, 0, most_blocks < 1 ? 1 : most_blocks};
   const int stage = tensors * K * threads * R::kBytes + extra;
   if (R::kAsync) {
-    r.stages = kRingBytes / (sharing < 1 ? 1 : sharing) / stage;
+    const int want = (elem_bytes == 4 ? 64 : 128) * 1024 / (kMaxStages * stage);
+    if (r.blocks > want) r.blocks = want < 1 ? 1 : want;
+    r.stages = kRingBytes / r.blocks / stage;
     r.stages = r.stages < 1 ? 1 : r.stages > kMaxStages ? kMaxStages : r.stages;
     r.bytes = r.stages * stage;
   }
@@ -883,11 +885,13 @@ int64_t grid_for(int64_t visits, int64_t per, int N, int64_t cap, bool edge) {
 template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 int run_forward(const Args& a, const Shape& s) {
   auto kernel = forward_kernel<T, W, V, K, kBlock, N, kPlain, kEdge>;
+  using R = Row<T, V, K, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
-  const Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, N, 512 / threads, 0);
+  const Ring ring = ring_for<R>(threads, K, N, 1024 / threads, 0, sizeof(T));
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
-  const int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
+  int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
+  if (R::kAsync && cap > static_cast<int64_t>(num_sms()) * ring.blocks) cap = static_cast<int64_t>(num_sms()) * ring.blocks;
   const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
   return launch("layernorm forward", kernel, blocks, threads, ring.bytes, a.st, false, static_cast<const T*>(a.x),
                 a.xm, a.order, static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean,
@@ -908,14 +912,16 @@ int run_join(const Args& a, int64_t n, int shift) {
 template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain, bool kEdge>
 int run_backward(const Args& a, const Shape& s) {
   auto kernel = backward_kernel<T, W, V, K, kBlock, N, kPlain, kEdge>;
+  using R = Row<T, V, K, kEdge>;
   const int threads = kBlock ? s.G : kGroupThreads;
   // a stage's statistics: 8 bytes a row for each warp or smaller group; the ring also joins the groups
-  Ring ring = ring_for<Row<T, V, K, kEdge>>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N);
+  Ring ring = ring_for<R>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N, sizeof(T));
   const int join_bytes = kGroupThreads / 32 * 2 * a.D * 4;
   if (!kBlock && ring.bytes < join_bytes) ring.bytes = join_bytes;
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
+  if (R::kAsync && cap > static_cast<int64_t>(num_sms()) * ring.blocks) cap = static_cast<int64_t>(num_sms()) * ring.blocks;
   const int64_t most = max_partials(a.rows, a.D);
   if (cap > most) cap = most;
   const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
@@ -966,8 +972,9 @@ int run_vectors(const Args& a, const Shape& s, bool backward) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   if (s.thirty_two) return run_one<T, W, V, 32 / V, true, 1, kPlain, kEdge>(a, s, backward);
   if (!s.block) return run_one<T, W, V, 16 / V, false, 1, kPlain, kEdge>(a, s, backward);
-  // two rows a turn, once there are more rows than blocks
-  if (a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G))
+  // two rows a turn, once there are more rows than blocks and where two turns of them fit the ring
+  if (2 * 2 * (backward ? 2 : 1) * (16 / V) * s.G * 16 > kRingBytes - 4096 ||
+      a.rows <= static_cast<int64_t>(num_sms()) * (512 / s.G))
     return run_one<T, W, V, 16 / V, true, 1, kPlain, kEdge>(a, s, backward);
   return run_one<T, W, V, 16 / V, true, 2, kPlain, kEdge>(a, s, backward);
 }
