@@ -32,7 +32,7 @@ namespace clip {
 constexpr int kThreads = 256;
 // Elements per thread and chunk. Few elements in all are cut finely, to spread them over the
 // device; many coarsely, so that a thread has 128 bytes in flight (see `coarse` below).
-constexpr int kFine = 16, kCoarse = 64;
+constexpr int kFine = 16, kCoarse = 64;  // chunks of 2^12 and 2^14 elements
 constexpr int kFineBlocks = 8, kCoarseBlocks = 4;  // per SM
 constexpr int kBlocksPerSm = kFineBlocks;
 constexpr int kMaxBlocks = 148 * kBlocksPerSm;  // partials per launch
@@ -369,14 +369,15 @@ template <int N>
 int norm_part(const Request& r, size_t first, size_t n, int partials, Part* part) {
   Table<N> tab;
   const bool big = coarse(r.elements);
-  const int64_t chunk = kThreads * (big ? kCoarse : kFine);
+  const int shift = big ? 14 : 12;
+  static_assert(kThreads * kCoarse == 1 << 14 && kThreads * kFine == 1 << 12, "chunk sizes");
   uint32_t chunks = 0;
   for (size_t i = 0; i < n; ++i) {
     tab.t[i] = r.t[first + i];
     const int64_t lead = lead_of(tab.t[i].in, tab.t[i].in_type), numel = r.numel[first + i];
-    const int64_t m = (numel + lead + chunk - 1) / chunk;
+    const int64_t m = (numel + lead + (int64_t(1) << shift) - 1) >> shift;
     tab.t[i].first_chunk = chunks;
-    tab.t[i].last_len = static_cast<uint16_t>(m == 1 ? numel : numel + lead - (m - 1) * chunk);
+    tab.t[i].last_len = static_cast<uint16_t>(m == 1 ? numel : numel + lead - ((m - 1) << shift));
     chunks += static_cast<uint32_t>(m);
   }
   const int64_t cap = std::min<int64_t>(static_cast<int64_t>(num_sms()) * (big ? kCoarseBlocks : kFineBlocks),
@@ -457,33 +458,47 @@ int gather(const void* const* grads, void* const* outs, const int64_t* numel, co
            const int* out_dtypes, int64_t n, Request* r) {
   if (n < 0 || (n > 0 && (!grads || !numel || !dtypes)))
     return fail(GTK_ERR_INVALID_ARG, "gradient norm: bad tensor list");
-  std::vector<Range> in, out;
   r->t.reserve(n);
   r->numel.reserve(n);
-  if (r->scale) out.reserve(n);
-  if (r->scale && outs) in.reserve(n);
+  // what is read and what is written, as far as one look at each tensor tells
+  uintptr_t in_low = ~uintptr_t(0), in_high = 0, out_low = ~uintptr_t(0), out_high = 0;
+  bool ascending = true;  // every output begins behind the end of the one before
   for (int64_t i = 0; i < n; ++i) {
-    if (numel[i] < 0 || numel[i] > (int64_t(1) << 40))
+    const int64_t m = numel[i];
+    if (m < 0 || m > (int64_t(1) << 40))
       return fail(GTK_ERR_INVALID_ARG, "gradient norm: bad size of tensor " + std::to_string(i));
-    const int ot = (outs && out_dtypes) ? out_dtypes[i] : dtypes[i];
-    if (!dtype_ok(dtypes[i]) || !(ot == dtypes[i] || ot == GTK_F32))
+    const int it = dtypes[i], ot = (outs && out_dtypes) ? out_dtypes[i] : it;
+    if (!dtype_ok(it) || !(ot == it || ot == GTK_F32))
       return fail(GTK_ERR_UNSUPPORTED,
                   "gradient norm: gradients are fp32, bf16 or fp16, outputs fp32 or the gradient's type");
-    if (!numel[i]) continue;
+    if (!m) continue;
     void* o = outs ? outs[i] : const_cast<void*>(grads[i]);
     if (!grads[i] || !o) return fail(GTK_ERR_INVALID_ARG, "gradient norm: NULL tensor " + std::to_string(i));
     const uintptr_t a = reinterpret_cast<uintptr_t>(grads[i]), b = reinterpret_cast<uintptr_t>(o);
-    if (a % dtype_bytes(dtypes[i]) || b % dtype_bytes(ot))
+    if ((a & (dtype_bytes(it) - 1)) || (b & (dtype_bytes(ot) - 1)))
       return fail(GTK_ERR_ALIGNMENT, "gradient norm: tensor " + std::to_string(i) + " is misaligned");
-    r->t.push_back(Tensor{grads[i], o, 0, 0, static_cast<uint8_t>(dtypes[i]), static_cast<uint8_t>(ot)});
-    r->numel.push_back(numel[i]);
-    r->elements += numel[i];
-    if (!r->scale) continue;
-    out.push_back(Range{b, b + numel[i] * dtype_bytes(ot), i});
-    if (outs) in.push_back(Range{a, a + numel[i] * dtype_bytes(dtypes[i]), i});
+    r->t.push_back(Tensor{grads[i], o, 0, 0, static_cast<uint8_t>(it), static_cast<uint8_t>(ot)});
+    r->numel.push_back(m);
+    r->elements += m;
+    in_low = std::min(in_low, a);
+    in_high = std::max(in_high, a + m * dtype_bytes(it));
+    ascending = ascending && b >= out_high;
+    out_low = std::min(out_low, b);
+    out_high = std::max(out_high, b + m * dtype_bytes(ot));
   }
   if (r->elements > (int64_t(1) << 42)) return fail(GTK_ERR_UNSUPPORTED, "gradient norm: too many elements");
-  if (r->scale && outputs_clash(std::move(in), std::move(out), !outs))
+  const bool apart = !outs || in_high <= out_low || out_high <= in_low;
+  if (!r->scale || (ascending && apart)) return GTK_OK;
+  std::vector<Range> in, out;
+  out.reserve(r->t.size());
+  if (outs) in.reserve(r->t.size());
+  for (size_t i = 0; i < r->t.size(); ++i) {
+    const Tensor& t = r->t[i];
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t.in), b = reinterpret_cast<uintptr_t>(t.out);
+    out.push_back(Range{b, b + r->numel[i] * dtype_bytes(t.out_type), static_cast<int64_t>(i)});
+    if (outs) in.push_back(Range{a, a + r->numel[i] * dtype_bytes(t.in_type), static_cast<int64_t>(i)});
+  }
+  if (outputs_clash(std::move(in), std::move(out), !outs))
     return fail(GTK_ERR_INVALID_ARG,
                 outs ? "gradient clipping: outputs overlap one another or other gradients"
                      : "gradient clipping: the gradients overlap one another (the same tensor twice?)");

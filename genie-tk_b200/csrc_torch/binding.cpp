@@ -247,10 +247,9 @@ struct Gradients {
   std::vector<std::pair<Tensor, Tensor>> write_back;  // (gradient, its clipped copy)
 };
 
-// Element i of a list or tuple of tensors. (Reads the TensorImpl directly from here on: a list may
-// hold hundreds of gradients, and every call on a Tensor counts.)
-c10::TensorImpl* tensor_at(PyObject* seq, const char* name, Py_ssize_t i) {
-  PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+// Item i of a list of tensors. (Reads the TensorImpl directly from here on: a list may hold
+// hundreds of gradients, and every call on a Tensor counts.)
+c10::TensorImpl* tensor_at(PyObject* o, const char* name, Py_ssize_t i) {
   if (!THPVariable_Check(o)) type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.defined()) type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
@@ -261,10 +260,17 @@ Tensor handle(c10::TensorImpl* t) {
   return Tensor(c10::intrusive_ptr<c10::TensorImpl, c10::UndefinedTensorImpl>::reclaim_copy(t));
 }
 
-bool dense(c10::TensorImpl* t) { return t->is_contiguous() || t->is_non_overlapping_and_dense(); }
-
-void written(c10::TensorImpl* t) {
-  if (!t->is_inference()) t->bump_version();
+// Has the tensors that are a few places ahead in the list brought near: their objects, and of
+// nearer ones what the objects point to.
+void prefetch(PyObject** items, Py_ssize_t i, Py_ssize_t n) {
+  if (i + 12 < n) __builtin_prefetch(items[i + 12]);
+  if (i + 8 < n) __builtin_prefetch(reinterpret_cast<char*>(items[i + 8]) + 64);
+  if (i + 6 < n && THPVariable_CheckExact(items[i + 6])) {
+    const char* t = reinterpret_cast<const char*>(THPVariable_Unpack(items[i + 6]).unsafeGetTensorImpl());
+    __builtin_prefetch(t);
+    __builtin_prefetch(t + 64);
+    __builtin_prefetch(t + 128);
+  }
 }
 
 // Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
@@ -273,11 +279,14 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
   if (!fast) throw py::error_already_set();
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
   if (n == 0) value_error("the list of gradients is empty");
+  PyObject** items = PySequence_Fast_ITEMS(fast.ptr());
   py::object fast_out;
+  PyObject** out_items = nullptr;
   if (outs) {
     fast_out = py::reinterpret_steal<py::object>(PySequence_Fast(outs->ptr(), "out must be a sequence"));
     if (!fast_out) throw py::error_already_set();
     if (PySequence_Fast_GET_SIZE(fast_out.ptr()) != n) value_error("out must have one tensor for each gradient");
+    out_items = PySequence_Fast_ITEMS(fast_out.ptr());
   }
   g->in.resize(n);
   g->numel.resize(n);
@@ -286,25 +295,28 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     g->out.resize(n);
     g->out_type.resize(n);
   }
-  require_cuda(handle(tensor_at(fast.ptr(), "grads", 0)), "grads[0]");
-  const c10::Device device = tensor_at(fast.ptr(), "grads", 0)->device();
+  require_cuda(handle(tensor_at(items[0], "grads", 0)), "grads[0]");
+  const c10::Device device = tensor_at(items[0], "grads", 0)->device();
   for (Py_ssize_t i = 0; i < n; ++i) {
-    c10::TensorImpl* t = tensor_at(fast.ptr(), "grads", i);
+    prefetch(items, i, n);
+    c10::TensorImpl* t = tensor_at(items[i], "grads", i);
     if (t->device() != device)
       throw std::runtime_error(kPrefix + "all gradients must be CUDA tensors on one device");
     if (t->layout() != at::kStrided) type_error("gradients must be dense tensors");
     const at::ScalarType st = c10::typeMetaToScalarType(t->dtype());
     const int code = code_of(st);
     if (code < 0) type_error("gradients must be float32, bfloat16 or float16, got " + name_of(st));
+    const bool plain = t->is_contiguous();
     if (outs) {
-      c10::TensorImpl* o = tensor_at(fast_out.ptr(), "out", i);
+      prefetch(out_items, i, n);
+      c10::TensorImpl* o = tensor_at(out_items[i], "out", i);
       if (o->device() != device || o->layout() != at::kStrided)
         throw std::runtime_error(kPrefix + "out must hold dense CUDA tensors on the gradients' device");
       if (o->sizes() != t->sizes()) value_error("out[" + std::to_string(i) + "] must have its gradient's shape");
       const at::ScalarType ot = c10::typeMetaToScalarType(o->dtype());
       if (ot != at::kFloat && ot != st)
         type_error("out must be float32 or the gradient's type, got " + name_of(ot));
-      const bool alike = (t->is_contiguous() && o->is_contiguous()) ||
+      const bool alike = (plain && o->is_contiguous()) ||
                          (t->is_non_overlapping_and_dense() && t->strides() == o->strides());
       if (!alike) {
         if (!o->is_contiguous()) value_error("out[" + std::to_string(i) + "] must be contiguous");
@@ -313,17 +325,19 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
       }
       g->out[i] = o->mutable_data();
       g->out_type[i] = code_of(ot);
-    } else if (!dense(t)) {
-      g->keep.push_back(handle(t).contiguous());
-      if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
-      t = g->keep.back().unsafeGetTensorImpl();
+      if (!o->is_inference()) o->bump_version();
+    } else {
+      if (clip && !t->is_inference()) t->bump_version();
+      if (!plain && !t->is_non_overlapping_and_dense()) {
+        g->keep.push_back(handle(t).contiguous());
+        if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
+        t = g->keep.back().unsafeGetTensorImpl();
+      }
     }
     g->in[i] = t->data();
     g->numel[i] = t->numel();
     g->in_type[i] = code;
   }
-  // only now, when nothing is refused any more: what is written counts as written
-  for (Py_ssize_t i = 0; clip && i < n; ++i) written(tensor_at(outs ? fast_out.ptr() : fast.ptr(), "grads", i));
   return device;
 }
 
