@@ -72,7 +72,6 @@ struct Table {
   Tensor t[N];
   int n;
   uint32_t chunks;  // of all tensors
-  uint32_t per;     // chunks of one block
 };
 
 // What the second kernel needs of a launch's table, in the workspace.
@@ -201,12 +200,9 @@ __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoars
     for (int i = blockIdx.x * kThreads + threadIdx.x; i < tab.n; i += gridDim.x * kThreads) shadow->t[i] = tab.t[i];
   constexpr int kChunk = kThreads * kPer;
   double acc = 0.0;
-  const uint32_t c0 = blockIdx.x * tab.per;
-  const uint32_t c1 = min(c0 + tab.per, tab.chunks);
-  int t = c0 < c1 ? find([&](int i) { return tab.t[i].first_chunk; }, tab.n, c0) : 0;
-  for (uint32_t c = c0; c < c1; ++c) {
-    uint32_t next = t + 1 < tab.n ? tab.t[t + 1].first_chunk : tab.chunks;
-    if (next <= c) next = ++t + 1 < tab.n ? tab.t[t + 1].first_chunk : tab.chunks;  // every tensor has a chunk
+  for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    const int t = find([&](int i) { return tab.t[i].first_chunk; }, tab.n, c);
+    const uint32_t next = t + 1 < tab.n ? tab.t[t + 1].first_chunk : tab.chunks;
     const Tensor& e = tab.t[t];
     const Span sp = span_of(e, c - e.first_chunk, c + 1 == next, kChunk);
     const int64_t off = sp.off;
@@ -290,7 +286,7 @@ __device__ __forceinline__ void scale_chunk(const void* in, void* out, int64_t o
 
 template <int kPer>
 __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoarseBlocks)
-    clip_scale_kernel(const Shadow* __restrict__ shadow, int tensors, uint32_t chunks, uint32_t per,
+    clip_scale_kernel(const Shadow* __restrict__ shadow, int tensors, uint32_t chunks,
                       const double* __restrict__ partial, int partials, bool inf_norm, double max_norm, bool in_place,
                       float* __restrict__ norm_out) {
   wait_previous_kernel();
@@ -303,14 +299,11 @@ __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoars
   const float k = static_cast<float>(q < 1.0 || isnan(q) ? q : 1.0);
   if (in_place && k == 1.f) return;
   constexpr int kChunk = kThreads * kPer;
-  const uint32_t c0 = blockIdx.x * per;
-  const uint32_t c1 = min(c0 + per, chunks);
-  if (c0 >= c1) return;
-  int t = find([&](int i) { return first[i]; }, tensors, c1 - 1);
-  Tensor e = shadow->t[t];
 #pragma unroll 1
-  for (uint32_t c = c1; c-- > c0;) {
-    if (first[t] > c) e = shadow->t[--t];
+  for (uint32_t back = blockIdx.x; back < chunks; back += gridDim.x) {
+    const uint32_t c = chunks - 1 - back;
+    const int t = find([&](int i) { return first[i]; }, tensors, c);
+    const Tensor e = shadow->t[t];
     const Span sp = span_of(e, c - first[t], c + 1 == first[t + 1], kChunk);
     const int64_t off = sp.off;
     const int n = sp.n;
@@ -356,7 +349,7 @@ size_t workspace_bytes(int64_t n) {
 
 struct Part {
   int tensors, blocks;
-  uint32_t chunks, per;
+  uint32_t chunks;
   Shadow* shadow;
 };
 
@@ -385,8 +378,7 @@ int norm_part(const Request& r, size_t first, size_t n, int partials, Part* part
   const uint32_t blocks = chunks < cap ? chunks : static_cast<uint32_t>(cap);
   tab.n = part->tensors = static_cast<int>(n);
   tab.chunks = part->chunks = chunks;
-  tab.per = part->per = (chunks + blocks - 1) / blocks;
-  part->blocks = static_cast<int>((chunks + tab.per - 1) / tab.per);
+  part->blocks = static_cast<int>(blocks);
   return launch("gradient norm", big ? clip_norm_kernel<N, kCoarse> : clip_norm_kernel<N, kFine>, part->blocks,
                 kThreads, 0, r.st, false, tab, reinterpret_cast<double*>(r.ws) + partials,
                 r.scale ? part->shadow : nullptr, r.inf_norm);
@@ -414,7 +406,7 @@ int run(const Request& r, int64_t n_given) {
                   r.inf_norm, r.norm);
   for (size_t i = 0; i < launches; ++i)
     if (int e = launch("gradient clipping", coarse(r.elements) ? clip_scale_kernel<kCoarse> : clip_scale_kernel<kFine>, parts[i].blocks, kThreads, 0, r.st, i == 0,
-                       static_cast<const Shadow*>(parts[i].shadow), parts[i].tensors, parts[i].chunks, parts[i].per,
+                       static_cast<const Shadow*>(parts[i].shadow), parts[i].tensors, parts[i].chunks,
                        partial, partials, r.inf_norm, r.max_norm, r.in_place,
                        i == 0 ? r.norm : static_cast<float*>(nullptr)))
       return e;

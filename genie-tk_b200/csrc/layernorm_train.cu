@@ -37,8 +37,12 @@
 //
 // dw and db: a thread meets the same columns in every row of its group, so it sums them in
 // registers over all the group's rows; the block's groups are then joined in shared memory,
-// the block writes one partial row, and a second kernel adds the partials in a fixed order.
+// the block writes one partial row, and a second kernel adds the partials in a fixed order. A grid
+// of up to eight blocks is launched as one cluster and adds them itself, through distributed shared
+// memory (37 rows of 384: 9.6 us a call instead of 7).
 // No atomics: the same inputs give the same bits.
+#include <cooperative_groups.h>
+
 #include <atomic>
 
 #include "train_common.cuh"
@@ -49,9 +53,10 @@ namespace ln {
 constexpr int kMaxWidth = 1 << 20;
 constexpr int kGroupThreads = 256;  // block of the kernels whose groups are at most a warp
 constexpr int kMaxBlockGroup = 512;
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512;
 constexpr int kMaxStages = 2;             // turns in the ring: this one and the next
 constexpr int kRingBytes = 200 * 1024;    // most of an SM
+constexpr int kMaxCluster = 8;
 
 // Division of n < 2^31 by a constant of the launch.
 struct Divisor {
@@ -477,7 +482,8 @@ template <typename T, typename W, int V, int K, bool kBlock, int N, bool kPlain,
 __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBlock ? 1 : 2)
     backward_kernel(const T* __restrict__ dy, RowMap dm, const T* __restrict__ x, RowMap xm, Order order,
                     const W* __restrict__ w, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-                    T* __restrict__ dx, float* __restrict__ partial, int D, int G, int stages) {
+                    T* __restrict__ dx, float* __restrict__ partial, W* __restrict__ dw, W* __restrict__ db, int D,
+                    int G, int stages) {
   extern __shared__ __align__(16) char ring[];
   __shared__ float red[128];
   using R = Row<T, V, K, kEdge>;
@@ -602,10 +608,11 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
     now = now == last_slot ? 0 : now + stage_bytes;
     stat = now ? stat + stats_stage : 0;
   }
-  if (!partial) return;
+  const bool direct = dw || db;  // the grid is one cluster, which joins its blocks' sums itself
+  if (!partial && !direct) return;
   const int ld = partial_pitch(D);
   float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * ld;
-  if (kBlock) {
+  if (kBlock && !direct) {
     // as the vectors lie: column c at c + lead
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -626,12 +633,13 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
     return;
   }
   // every warp adds its groups in the ring's memory, then the block the warps. Groups that lie
-  // alike are added by shuffles (with a lead, the groups of a warp lie differently).
+  // alike are added by shuffles (with a lead, the groups of a warp lie differently); a block that
+  // is one group has its sums in its threads.
   wait_copies(1);
   __syncthreads();
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  float* cols = reinterpret_cast<float*>(ring) + warp * 2 * D;
-  if (!kEdge) {
+  const int warp = threadIdx.x >> 5, parts = kBlock ? 1 : blockDim.x >> 5;
+  float* cols = reinterpret_cast<float*>(ring) + (kBlock ? 0 : warp * 2 * D);
+  if (!kBlock && !kEdge) {
 #pragma unroll
     for (int p = 0; p < P; ++p)
       for (int o = G; o < 32; o <<= 1) {
@@ -640,28 +648,49 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
         ab[p].x += __shfl_xor_sync(0xffffffffu, ab[p].x, o);
         ab[p].y += __shfl_xor_sync(0xffffffffu, ab[p].y, o);
       }
-  } else {
+  } else if (!kBlock) {
     for (int i = threadIdx.x & 31; i < 2 * D; i += 32) cols[i] = 0.f;
     __syncwarp();
   }
-  for (int t = 0; t < (kEdge ? 32 / G : 1); ++t) {
-    if (static_cast<int>(threadIdx.x & 31) / G == t)
+  for (int t = 0; t < (!kBlock && kEdge ? 32 / G : 1); ++t) {
+    if (kBlock || static_cast<int>(threadIdx.x & 31) / G == t)
 #pragma unroll
       for (int e = 0; e < K * V; ++e) {
         const int col = column_of<V, kEdge>(e, l);
         if (col < 0 || col >= D) continue;
-        cols[col] = (kEdge ? cols[col] : 0.f) + (e & 1 ? aw[e / 2].y : aw[e / 2].x);
-        cols[D + col] = (kEdge ? cols[D + col] : 0.f) + (e & 1 ? ab[e / 2].y : ab[e / 2].x);
+        const bool more = !kBlock && kEdge;
+        cols[col] = (more ? cols[col] : 0.f) + (e & 1 ? aw[e / 2].y : aw[e / 2].x);
+        cols[D + col] = (more ? cols[D + col] : 0.f) + (e & 1 ? ab[e / 2].y : ab[e / 2].x);
       }
     __syncwarp();
   }
   __syncthreads();
   cols = reinterpret_cast<float*>(ring);
-  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
-    float t = 0.f;
-    for (int q = 0; q < warps; ++q) t += cols[q * 2 * D + i];
-    pw[i < D ? i : i - D + ld] = t;
+  if (!direct) {
+    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+      float t = 0.f;
+      for (int q = 0; q < parts; ++q) t += cols[q * 2 * D + i];
+      pw[i < D ? i : i - D + ld] = t;
+    }
+    return;
   }
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks());
+  cluster.sync();
+  for (int i = cluster.block_rank() * blockDim.x + threadIdx.x; i < 2 * D; i += blocks * blockDim.x) {
+    float t = 0.f;
+    for (int r = 0; r < blocks; ++r) {
+      const float* there = cluster.map_shared_rank(cols, r);
+      for (int q = 0; q < parts; ++q) t += there[q * 2 * D + i];
+    }
+    if (i < D) {
+      if (dw) dw[i] = Elem<W>::store(t);
+    } else if (db) {
+      db[i - D] = Elem<W>::store(t);
+    }
+  }
+  cluster.sync();  // nobody leaves while others read its memory
 }
 
 // dw, db: the sum of `n` partial rows of two times `ld` floats, in a fixed order, as a tree. Partial
@@ -696,7 +725,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   __syncthreads();
   // warp k adds column k over the warps
   for (int k = warp; k < kCols; k += kWarps) {
-    float t = part[lane][k];
+    float t = lane < kWarps ? part[lane][k] : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0 && c0 + k < D) out[c0 + k] = Elem<W>::store(t);
@@ -918,6 +947,7 @@ int run_backward(const Args& a, const Shape& s) {
   Ring ring = ring_for<R>(threads, K, 2 * N, 512 / threads, threads / (kBlock ? 32 : s.G) * 8 * N, sizeof(T));
   const int join_bytes = kGroupThreads / 32 * 2 * a.D * 4;
   if (!kBlock && ring.bytes < join_bytes) ring.bytes = join_bytes;
+  if (kBlock && ring.bytes < 2 * a.D * 4) ring.bytes = 2 * a.D * 4;
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
@@ -925,10 +955,18 @@ int run_backward(const Args& a, const Shape& s) {
   const int64_t most = max_partials(a.rows, a.D);
   if (cap > most) cap = most;
   const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
+  // Up to eight blocks are one cluster, which needs neither a second launch nor partial rows.
+  if (a.partial && blocks <= kMaxCluster)
+    return launch_clusters("layernorm backward", kernel, blocks, threads, ring.bytes, static_cast<int>(blocks), a.st,
+                           static_cast<const T*>(a.dy), a.dm, static_cast<const T*>(a.x), a.xm, a.order,
+                           static_cast<const W*>(a.w), static_cast<const float*>(a.mean),
+                           static_cast<const float*>(a.rstd), static_cast<T*>(a.dx), static_cast<float*>(nullptr),
+                           static_cast<W*>(a.dw), static_cast<W*>(a.db), a.D, s.G, ring.stages);
   if (int e = launch("layernorm backward", kernel, blocks, threads, ring.bytes, a.st, false,
                      static_cast<const T*>(a.dy), a.dm, static_cast<const T*>(a.x), a.xm, a.order,
                      static_cast<const W*>(a.w), static_cast<const float*>(a.mean),
-                     static_cast<const float*>(a.rstd), static_cast<T*>(a.dx), a.partial, a.D, s.G, ring.stages))
+                     static_cast<const float*>(a.rstd), static_cast<T*>(a.dx), a.partial, static_cast<W*>(nullptr),
+                     static_cast<W*>(nullptr), a.D, s.G, ring.stages))
     return e;
   return a.partial ? run_join<W>(a, blocks, kBlock && kEdge ? V - 1 : 0) : GTK_OK;
 }
