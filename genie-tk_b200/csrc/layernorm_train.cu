@@ -331,11 +331,13 @@ struct Columns {
 // Zeros in the thread's slots of vectors that do not exist, in `rows` rows of the ring.
 template <typename T, int V, int K, bool kEdge>
 __device__ __forceinline__ void zero_missing(char* mine, int pitch, int rows, const Lay<kEdge>& l) {
-  if (V == 1 || l.nv >= l.G * K) return;
-  for (int r = 0; r < rows; ++r)
+  if constexpr (V > 1) {
+    if (l.nv >= l.G * K) return;
+    for (int r = 0; r < rows; ++r)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (l.lane + l.G * k >= l.nv) *reinterpret_cast<uint4*>(mine + (r * K + k) * pitch) = make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < K; ++k)
+        if (l.lane + l.G * k >= l.nv) *reinterpret_cast<uint4*>(mine + (r * K + k) * pitch) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // The rows of a tensor in visiting order, for one thread: addresses of its first vector. kPlain: one

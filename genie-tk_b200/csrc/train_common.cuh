@@ -158,6 +158,15 @@ __device__ __forceinline__ void st_vec(T* p, const Vec<T, V>& v) {
   *reinterpret_cast<typename Vec<T, V>::W::type*>(p) = v.r;
 }
 
+// The same, marked as not to be kept in the L2 cache: for outputs larger than it.
+template <typename T, int V>
+__device__ __forceinline__ void st_vec_streaming(T* p, const Vec<T, V>& v) {
+  if constexpr (sizeof(T) * V >= 4)
+    __stcs(reinterpret_cast<typename Vec<T, V>::W::type*>(p), v.r);
+  else
+    st_vec<T, V>(p, v);
+}
+
 // Waits until the kernel before this one on the stream has finished and its writes are
 // visible; at once when the launch carried no programmatic dependency.
 __device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
