@@ -30,8 +30,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kMaxCluster = 8;                    // sorting blocks that exchange through their shared memory
 constexpr int kClusterPer = 4;                    // most tokens per thread of such a block
 constexpr int64_t kClusterTokens = static_cast<int64_t>(kSortThreads) * kClusterPer * kMaxCluster;
-constexpr int kPer = 8;                           // tokens per thread of the sort over many tiles
-constexpr int kTile = kSortThreads * kPer;
+constexpr int kMaxPer = 8;                        // tokens per thread of the sort over many tiles
 constexpr int kMaxBits = 8;                       // of a digit
 constexpr int kBins = 1 << kMaxBits;
 constexpr int kWarps = kSortThreads / 32;
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(kSortThreads)
 // Pass `pass` of the sort over many tiles, first half: the tile's digit counts. The first pass
 // reads the tokens, later ones the keys of the pass before. Warps count in four histograms; 32
 // equal digits (frequent tokens, sorted data) are one addition.
-template <typename I>
+template <typename I, int N>
 __global__ void __launch_bounds__(kSortThreads)
     count_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys, int64_t T, uint32_t V,
                  int64_t padding, int pass, int bits, uint32_t* __restrict__ counts, uint32_t* status) {
@@ -227,17 +226,17 @@ __global__ void __launch_bounds__(kSortThreads)
   (&hist[0][0])[threadIdx.x] = 0;
   __syncthreads();
   bool bad = false;
-  uint32_t digit[kPer];
+  uint32_t digit[N];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
+  for (int i = 0; i < N; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kSortThreads * N) + tile_index<N>(i);
     uint32_t k = 0;
     if (t < T) k = pass == 0 ? key_of(static_cast<int64_t>(tokens[t]), V, padding, &bad) : keys[t];
     digit[i] = t < T ? (k >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
   }
   uint32_t* h = hist[(threadIdx.x >> 5) & 3];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < N; ++i) {
     const uint32_t first = __shfl_sync(0xffffffffu, digit[i], 0);
     if (__all_sync(0xffffffffu, digit[i] == first)) {
       if ((threadIdx.x & 31) == 0 && first < kBins) atomicAdd(h + first, 32u);
@@ -253,7 +252,7 @@ __global__ void __launch_bounds__(kSortThreads)
 }
 
 // Second half: where the tile's elements go, from all tiles' counts.
-template <typename I>
+template <typename I, int N>
 __global__ void __launch_bounds__(kSortThreads)
     scatter_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                    int64_t T, uint32_t V, int64_t padding, int pass, int bits, const uint32_t* __restrict__ counts,
@@ -261,11 +260,11 @@ __global__ void __launch_bounds__(kSortThreads)
   wait_previous_kernel();
   __shared__ SortShared s;
   __shared__ uint32_t before_part[kSortThreads], total_part[kSortThreads];
-  uint32_t key[kPer], p0[kPer], digit[kPer], rank[kPer];
-  int64_t token[kPer];  // requested here, looked at after the counts, which are on their way meanwhile
+  uint32_t key[N], p0[N], digit[N], rank[N];
+  int64_t token[N];  // requested here, looked at after the counts, which are on their way meanwhile
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
+  for (int i = 0; i < N; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kSortThreads * N) + tile_index<N>(i);
     p0[i] = static_cast<uint32_t>(t);
     token[i] = t >= T ? 0 : pass == 0 ? static_cast<int64_t>(tokens[t]) : static_cast<int64_t>(keys[t]);
     if (pass && t < T) p0[i] = pos[t];
@@ -292,8 +291,8 @@ __global__ void __launch_bounds__(kSortThreads)
   total_part[threadIdx.x] = total;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTile + tile_index<kPer>(i);
+  for (int i = 0; i < N; ++i) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kSortThreads * N) + tile_index<N>(i);
     key[i] = pass == 0 ? key_of(token[i], V, padding, &bad) : static_cast<uint32_t>(token[i]);
     digit[i] = t < T ? (key[i] >> (bits * pass)) & ((1u << bits) - 1u) : kBins;
   }
@@ -306,10 +305,10 @@ __global__ void __launch_bounds__(kSortThreads)
     }
   const uint32_t base = scan_bins(s, total);
   if (threadIdx.x < kBins) s.base[threadIdx.x] = base + before;
-  rank_tile<kPer>(s, digit, rank, bits);
+  rank_tile<N>(s, digit, rank, bits);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
+  for (int i = 0; i < N; ++i)
     if (digit[i] < kBins) {
       const uint32_t to = s.base[digit[i]] + s.count[threadIdx.x >> 5][digit[i]] + rank[i];
       keys_out[to] = key[i];
@@ -681,6 +680,7 @@ int vec_width(int64_t D, size_t bytes, bool aligned) {
 // The backward's plan: what the workspace holds and how the sorted list is cut.
 struct Plan {
   int passes, bits;  // of the sort, for keys 0 .. vocab
+  int per;           // tokens per thread, of the sort over tiles
   int64_t tiles;
   bool zero_first;   // all of dW is zeroed beside the sort
   int64_t L, units;                            // entries of a warp's chunk; units of kSumWarps chunks
@@ -693,18 +693,22 @@ Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype, int w_dtype) {
   while (vocab >> bits) ++bits;
   p.passes = (bits + kMaxBits - 1) / kMaxBits;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.tiles = (T + kTile - 1) / kTile;
+  // up to 128 tiles: a tile's places come from all tiles' counts, but its scattered stores (the longest
+  // part, 19 us with 8192 tokens a tile) take the shorter the fewer they are
+  p.per = 1;
+  while (p.per < kMaxPer && T > int64_t(128) * kSortThreads * p.per) p.per <<= 1;
+  p.tiles = (T + kSortThreads * p.per - 1) / (kSortThreads * p.per);
   // The sort of a short list leaves most of the device idle for some 8 us, in which it can zero
   // all of dW. The rows that do occur are then written twice, which costs less than that time
   // as long as they are at most 32 MB (8192 tokens, 32000 x 1024 bf16: the whole gradient takes
   // 26 us, against 37 us when the absent rows are looked up and zeroed after the sort).
   p.zero_first = T <= kClusterTokens &&
                  (T < vocab ? T : vocab) * D * static_cast<int64_t>(dtype_bytes(w_dtype)) <= (32 << 20);
-  // About 24 warps per SM get a chunk, of whole batches. Up to 512 tokens make one unit: the
+  // About 8 warps per SM get a chunk, of whole batches (24: 5 to 15% slower, more runs cross chunks). Up to 512 tokens make one unit: the
   // launch that joins units costs more than the longer chunks.
   const int64_t slab = 32 * 16 / static_cast<int64_t>(dtype_bytes(dy_dtype));
   const int64_t slabs = (D + slab - 1) / slab;
-  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 24 - 1) / (148 * 24);
+  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 8 - 1) / (148 * 8);
   L = (L + kBatch - 1) / kBatch * kBatch;
   p.L = L > 1024 ? 1024 : L;
   p.units = (T + p.L * kSumWarps - 1) / (p.L * kSumWarps);
@@ -750,30 +754,21 @@ int sort_cluster(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
                          a.padding, p.passes, p.bits, keys, pos, static_cast<uint4*>(a.dw), zero_bytes, a.status);
 }
 
-template <typename I>
-int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** pos) {
-  const size_t half = round_up(4 * a.T, 256);
-  uint32_t* k[2] = {reinterpret_cast<uint32_t*>(a.ws + p.keys), reinterpret_cast<uint32_t*>(a.ws + p.keys + half)};
-  uint32_t* q[2] = {reinterpret_cast<uint32_t*>(a.ws + p.pos), reinterpret_cast<uint32_t*>(a.ws + p.pos + half)};
+// Two launches a pass; keys and positions alternate between two buffers.
+template <typename I, int N>
+int sort_tiles(const Args& a, const Plan& p, uint32_t* const (&k)[2], uint32_t* const (&q)[2], const uint32_t** keys,
+               const uint32_t** pos) {
   const I* tokens = static_cast<const I*>(a.tokens);
   const uint32_t V = static_cast<uint32_t>(a.vocab);
-  if (a.T <= kClusterTokens) {
-    *keys = k[0];
-    *pos = q[0];
-    // as few tokens per thread as the cluster allows: their ranks are found one after another
-    if (a.T <= kSortThreads * kMaxCluster) return sort_cluster<I, 1>(a, p, k[0], q[0]);
-    if (a.T <= 2 * kSortThreads * kMaxCluster) return sort_cluster<I, 2>(a, p, k[0], q[0]);
-    return sort_cluster<I, kClusterPer>(a, p, k[0], q[0]);
-  }
   uint32_t* counts = reinterpret_cast<uint32_t*>(a.ws + p.counts);
   const uint32_t *ki = nullptr, *qi = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {
     uint32_t *ko = k[pass & 1], *qo = q[pass & 1];
-    if (int e = launch("embedding token count", count_kernel<I>, p.tiles, kSortThreads, 0, a.st, pass > 0, tokens, ki,
-                       a.T, V, a.padding, pass, p.bits, counts, a.status))
+    if (int e = launch("embedding token count", count_kernel<I, N>, p.tiles, kSortThreads, 0, a.st, pass > 0, tokens,
+                       ki, a.T, V, a.padding, pass, p.bits, counts, a.status))
       return e;
-    if (int e = launch("embedding token scatter", scatter_kernel<I>, p.tiles, kSortThreads, 0, a.st, true, tokens, ki,
-                       qi, a.T, V, a.padding, pass, p.bits, static_cast<const uint32_t*>(counts),
+    if (int e = launch("embedding token scatter", scatter_kernel<I, N>, p.tiles, kSortThreads, 0, a.st, true, tokens,
+                       ki, qi, a.T, V, a.padding, pass, p.bits, static_cast<const uint32_t*>(counts),
                        static_cast<int>(p.tiles), ko, qo))
       return e;
     ki = ko;
@@ -782,6 +777,31 @@ int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** p
   *keys = ki;
   *pos = qi;
   return GTK_OK;
+}
+
+template <typename I>
+int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** pos) {
+  const size_t half = round_up(4 * a.T, 256);
+  uint32_t* k[2] = {reinterpret_cast<uint32_t*>(a.ws + p.keys), reinterpret_cast<uint32_t*>(a.ws + p.keys + half)};
+  uint32_t* q[2] = {reinterpret_cast<uint32_t*>(a.ws + p.pos), reinterpret_cast<uint32_t*>(a.ws + p.pos + half)};
+  if (a.T <= kClusterTokens) {
+    *keys = k[0];
+    *pos = q[0];
+    // as few tokens per thread as the cluster allows: their ranks are found one after another
+    if (a.T <= kSortThreads * kMaxCluster) return sort_cluster<I, 1>(a, p, k[0], q[0]);
+    if (a.T <= 2 * kSortThreads * kMaxCluster) return sort_cluster<I, 2>(a, p, k[0], q[0]);
+    return sort_cluster<I, kClusterPer>(a, p, k[0], q[0]);
+  }
+  switch (p.per) {
+    case 1:
+      return sort_tiles<I, 1>(a, p, k, q, keys, pos);
+    case 2:
+      return sort_tiles<I, 2>(a, p, k, q, keys, pos);
+    case 4:
+      return sort_tiles<I, 4>(a, p, k, q, keys, pos);
+    default:
+      return sort_tiles<I, kMaxPer>(a, p, k, q, keys, pos);
+  }
 }
 
 template <typename T, typename W, int V>

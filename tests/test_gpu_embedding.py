@@ -80,7 +80,7 @@ def test_gradient(T, V, D, dtype, wdtype):
 
 
 @pytest.mark.parametrize("kind", ["one", "down", "sorted"])
-@pytest.mark.parametrize("T", [1, 32, 33, 512, 513, 700, 1024, 1025, 4097, 8192, 8193, 16385, 32768, 32769, 50001])
+@pytest.mark.parametrize("T", [1, 32, 33, 512, 513, 700, 1024, 1025, 4097, 8192, 8193, 16385, 32768, 32769, 50001, 131073, 262145, 600001])
 def test_orders_of_tokens(kind, T):
     dev = require_gpu()
     gen = torch.Generator(device=dev).manual_seed(T)
