@@ -3,16 +3,17 @@
 //   y_t  = s W[tok_t]                      (a gather; zeros for a token outside 0 .. V-1)
 //   dW_v = s sum_{t : tok_t = v} dy_t      (zeros for a token that does not occur, and padding)
 //
-// Forward: HBM bound. It writes T rows and reads each row of W that occurs at least once; a
-// warp copies rows in 16-byte vectors, several rows at a time so that the loads of the tokens
-// and of the rows behind them overlap.
+// Forward: HBM bound. It writes T rows and reads each row of W that occurs at least once. The output
+// is written as one array, thread by thread in 16-byte vectors, whatever the width; the tokens and
+// the table's elements behind them come through the caches, four vectors at a time per thread.
 //
 // Backward: HBM bound too -- it reads dy once and writes the whole of dW once -- if the rows
 // of one token can be found together. So the tokens are sorted first (stable, least digit first,
 // up to 8 bits a pass; four bytes of key and four of position per token, small beside dy; one
 // cluster of blocks does it up to 32,768 tokens), and the sorted list is cut into chunks of equal length,
-// whatever the tokens' frequencies: a warp sums the dy rows of its chunk in registers, in list
-// order, with the next twelve rows in flight, and writes a row of dW at each change of token. Runs
+// whatever the tokens' frequencies: a group of 4 to 32 lanes (as the row is wide) sums the dy rows of
+// its chunk in registers, in list order, with the next twelve rows in flight, and writes a row of dW
+// at each change of token. Runs
 // that cross chunks are joined in the block, and those that cross blocks from a scratch buffer
 // of at most two rows a block, by a last kernel and in order. Rows of tokens that do not occur are
 // zeroed by further blocks of the same launch, which look them up in the sorted keys.
@@ -319,186 +320,242 @@ __global__ void __launch_bounds__(kSortThreads)
 // ---- Sums over the runs of equal tokens -----------------------------------------------------
 
 constexpr int kSumThreads = 256;
-constexpr int kSumWarps = kSumThreads / 32;
-constexpr int kBatch = 4;  // dy rows that a warp requests and adds at once
+constexpr int kBatch = 4;   // dy rows that a group requests and adds at once
+constexpr int kAhead = 3;   // batches on their way
 
-template <typename W, int V>
-__device__ __forceinline__ void write_row(W* dst, const float (&acc)[V], float scale) {
-  float f[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = acc[j] * scale;
-  constexpr int kMost = 16 / static_cast<int>(sizeof(W));  // elements of a store
-  constexpr int kEach = V < kMost ? V : kMost;
-#pragma unroll
-  for (int j = 0; j < V; j += kEach)
-    st_vec<W, kEach>(dst + j, Vec<W, kEach>::of(reinterpret_cast<const float(&)[kEach]>(f[j])));
+// A lane has V columns of a slab of S V: consecutive ones where V divides the width, else (kEdge) V
+// that are S apart.
+template <int V, int S, bool kEdge>
+__device__ __forceinline__ int column(int lane, int j) {
+  return kEdge ? lane + S * j : lane * V + j;
 }
 
-// The dy rows of a warp's chunk, requested some batches ahead of their use. 16-byte vectors go to
-// a ring in shared memory with cp.async, sixteen rows (8 KB) a warp, which takes no registers: a
-// lane reads only what it requested itself, so the lane's own wait is enough. Single elements
-// (odd widths) are too small for that and are loaded into registers, one batch ahead.
-template <typename T, int V>
+// The lane's columns of a row of dW; `row` is where the slab begins in it, `cols` the slab's columns.
+template <typename W, int V, int S, bool kEdge>
+__device__ __forceinline__ void write_row(W* row, const float (&acc)[V], float scale, int lane, int cols) {
+  if constexpr (!kEdge) {
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = acc[j] * scale;
+    constexpr int kMost = 16 / static_cast<int>(sizeof(W));  // elements of a store
+    constexpr int kEach = V < kMost ? V : kMost;
+#pragma unroll
+    for (int j = 0; j < V; j += kEach)
+      st_vec<W, kEach>(row + lane * V + j, Vec<W, kEach>::of(reinterpret_cast<const float(&)[kEach]>(f[j])));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (lane + S * j < cols) row[lane + S * j] = Elem<W>::store(acc[j] * scale);
+  }
+}
+
+// The dy rows of a group's chunk, requested three batches ahead of their use: 16-byte vectors to a ring
+// in shared memory with cp.async, which takes no registers. Where V divides the width, a lane reads
+// only what it requested itself, and its own wait is enough. Else the rows begin anywhere: the group
+// copies the vectors that hold its slab of the row, from the boundary at or before it on (dy begins
+// on one, so that this is never outside of it), and its lanes meet before they read their elements.
+template <typename T, int V, int S, bool kEdge>
 struct Rows {
-  static constexpr bool kAsync = V > 1;
-  static constexpr int kSlots = kAsync ? 4 : 2;  // batches
-  static constexpr int kAhead = kSlots - 1;
-  static constexpr int kRingBytes = kAsync ? kSlots * kBatch * 32 * 16 : 0;  // of a warp
-  const T* base;
-  const int D;
-  const bool mine;
-  const uint32_t vocab;
+  static constexpr int kSlots = kAhead + 1;
+  static constexpr int kRowBytes = S * 16 + (kEdge ? 16 : 0);
+  static constexpr int kGroupBytes = kSlots * kBatch * kRowBytes;
+  static constexpr int kRingBytes = kSumThreads / S * kGroupBytes;
+  const T* dy;  // where the slab begins in the first row
+  const int D, cols, lane;
+  const bool mine;  // the lane has columns
+  const uint32_t vocab, mask;
   char* ring;
-  Vec<T, V> held[kAsync ? 1 : kSlots][kBatch];
+  uint32_t lead[kEdge ? kSlots : 1];  // elements from the boundary to the slab, four bits for each row
 
-  __device__ __forceinline__ Rows(const T* b, int d, bool m, uint32_t v, char* r)
-      : base(b), D(d), mine(m), vocab(v), ring(r + (threadIdx.x & 31) * 16) {}
+  __device__ __forceinline__ Rows(const T* d, int width, int slab, int ln, uint32_t v, char* r)
+      : dy(d + slab * S * V),
+        D(width),
+        cols(width - slab * S * V < S * V ? width - slab * S * V : S * V),
+        lane(ln),
+        mine((kEdge ? ln : ln * V) < cols),
+        vocab(v),
+        mask(S == 32 ? 0xffffffffu : ((1u << (S & 31)) - 1u) << (threadIdx.x & 31 & ~(S - 1))),
+        ring(r + threadIdx.x / S * kGroupBytes) {}
 
-  // Batch g: entries q .. q + 3 of the 32 whose keys and positions the lanes hold.
-  __device__ __forceinline__ void request(int g, uint32_t k32, uint32_t p32, int q) {
+  __device__ __forceinline__ void request(int slot, const uint32_t (&k)[kBatch], const uint32_t (&p)[kBatch]) {
+    if constexpr (kEdge) {
+      __syncwarp(mask);  // the slot's last rows have been read
+      lead[slot] = 0;
+    }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const uint32_t k = __shfl_sync(0xffffffffu, k32, q + u);
-      const uint32_t p = __shfl_sync(0xffffffffu, p32, q + u);
-      if (!mine || k >= vocab) continue;
-      const T* src = base + static_cast<int64_t>(p) * D;
-      if constexpr (kAsync)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
-                         __cvta_generic_to_shared(ring + ((g % kSlots) * kBatch + u) * 512))),
-                     "l"(src)
-                     : "memory");
-      else
-        held[g % kSlots][u] = ld_vec<T, V>(src);
+      if (k[u] >= vocab) continue;
+      const T* row = dy + static_cast<int64_t>(p[u]) * D;
+      uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring + (slot * kBatch + u) * kRowBytes));
+      if constexpr (!kEdge) {
+        if (mine)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + lane * 16), "l"(row + lane * V) : "memory");
+      } else {
+        const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u);
+        const char* from = reinterpret_cast<const char*>(row) - before;
+        const int bytes = static_cast<int>(before) + cols * static_cast<int>(sizeof(T));
+        lead[slot] |= (before / static_cast<uint32_t>(sizeof(T))) << (4 * u);
+        for (int i = lane * 16; i < bytes; i += S * 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i), "l"(from + i),
+                       "r"(bytes - i < 16 ? bytes - i : 16)
+                       : "memory");
+      }
     }
-    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  __device__ __forceinline__ void take(int g, Vec<T, V> (&to)[kBatch]) {
-    if constexpr (kAsync) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+  // The batch requested kAhead batches ago.
+  __device__ __forceinline__ void arrived() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+    if constexpr (kEdge) __syncwarp(mask);
+  }
+  __device__ __forceinline__ void take(int slot, int u, float (&f)[V]) const {
+    const char* row = ring + (slot * kBatch + u) * kRowBytes;
+    if constexpr (!kEdge) {
+      const Vec<T, V> v = ld_vec<T, V>(reinterpret_cast<const T*>(row + lane * 16));
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        to[u] = ld_vec<T, V>(reinterpret_cast<const T*>(ring + ((g % kSlots) * kBatch + u) * 512));
+      for (int j = 0; j < V; ++j) f[j] = v.get(j);
     } else {
+      const T* first = reinterpret_cast<const T*>(row) + (lead[slot] >> (4 * u) & 15u) + lane;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) to[u] = held[g % kSlots][u];
+      for (int j = 0; j < V; ++j) f[j] = lane + S * j < cols ? Elem<T>::load(first[S * j]) : 0.f;
     }
   }
-
-  __device__ __forceinline__ void drain() {
-    if constexpr (kAsync) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  }
+  __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 };
 
-// How a warp's chunk meets its neighbours. kHead: its first run began before it; kHeadOn: and
+// How a group's chunk meets its neighbours. kHead: its first run began before it; kHeadOn: and
 // that run goes on behind it (the chunk is one run). kTail: its last run begins in it and goes on.
 constexpr uint32_t kHead = 1, kHeadOn = 2, kTail = 4;
 
-// Warp c sums the sorted entries [c L, (c + 1) L) over a slab of 32 V columns; a block is one slab
-// of eight consecutive chunks (a unit), joined in shared memory, so that at most two partial
-// rows a unit go to memory: partial[2 u] for the run that began before it, partial[2 u + 1]
-// for the one that begins in it and goes on.
-template <typename T, typename W, int V>
+// A group of S lanes sums the sorted entries [c L, (c + 1) L) over a slab of columns (S = 32, or
+// fewer where the row is that narrow: one slab). A block is one slab of 256 / S consecutive chunks
+// (a unit), joined in shared memory, so that at most two partial rows a unit go to memory:
+// partial[2 u] for the run that began before it, partial[2 u + 1] for the one that begins in it
+// and goes on. Groups of a warp take their own ways; what lanes exchange, they exchange in the group.
+template <typename T, typename W, int V, int S, bool kEdge>
 __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_t* __restrict__ keys,
                                          const uint32_t* __restrict__ pos, W* __restrict__ dw,
                                          float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
-                                         int64_t unit, int slab, float scale, float (*edge)[2][32 * V],
-                                         uint32_t* how, uint32_t* run_key, char* ring) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t i0 = (unit * kSumWarps + warp) * L;
-  const int col = (slab * 32 + lane) * V;
-  const bool mine = col < D;
-  if (lane == 0) how[warp] = 0;
+                                         int64_t unit, int slab, float scale, float (*edge)[2][S * V], uint32_t* how,
+                                         uint32_t* run_key, char* ring) {
+  constexpr int kGroups = kSumThreads / S, kRing = kAhead + 1;
+  const int lane = threadIdx.x % S, group = threadIdx.x / S;
+  const int64_t i0 = (unit * kGroups + group) * L;
+  if (lane == 0) how[group] = 0;
   if (i0 < n) {
-    const int64_t i1 = i0 + L < n ? i0 + L : n;
-    const int m = static_cast<int>(i1 - i0);
+    const int m = static_cast<int>(i0 + L < n ? L : n - i0);
+    const int batches = (m + kBatch - 1) / kBatch;
     const uint32_t left = i0 > 0 ? keys[i0 - 1] : 0xffffffffu;
-    const uint32_t right = i1 < n ? keys[i1] : 0xffffffffu;
-    // the keys and positions of 32 entries, one per lane, and those of the next 32
-    uint32_t k_now = lane < m ? keys[i0 + lane] : 0xffffffffu;
-    uint32_t p_now = lane < m ? pos[i0 + lane] : 0u;
-    Rows<T, V> rows(dy + col, D, mine, vocab, ring);
+    const uint32_t right = i0 + m < n ? keys[i0 + m] : 0xffffffffu;
+    Rows<T, V, S, kEdge> rows(dy, D, slab, lane, vocab, ring);
+    W* dw_slab = dw + slab * S * V;
+    // The keys and positions of S batches, one batch per lane, and those of the next S. Chunks begin
+    // on 16-byte boundaries of both arrays, whose ends are padded; places that hold no entry get a
+    // key above all.
+    uint4 k_now = {}, p_now = {}, k_next = {}, p_next = {};
+    auto window = [&](int b, uint4& k, uint4& p) {
+      k = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
+      p = make_uint4(0, 0, 0, 0);
+      const int left_over = m - (b + lane) * kBatch;
+      if (left_over <= 0) return;
+      const uint4 a = *reinterpret_cast<const uint4*>(keys + i0 + (b + lane) * kBatch);
+      p = *reinterpret_cast<const uint4*>(pos + i0 + (b + lane) * kBatch);
+      k.x = a.x;
+      if (left_over > 1) k.y = a.y;
+      if (left_over > 2) k.z = a.z;
+      if (left_over > 3) k.w = a.w;
+    };
+    uint32_t key[kRing][kBatch];
+    auto request = [&](int slot, int b) {  // b: of the window
+      uint32_t p[kBatch];
+      key[slot][0] = __shfl_sync(rows.mask, k_now.x, b, S);
+      key[slot][1] = __shfl_sync(rows.mask, k_now.y, b, S);
+      key[slot][2] = __shfl_sync(rows.mask, k_now.z, b, S);
+      key[slot][3] = __shfl_sync(rows.mask, k_now.w, b, S);
+      p[0] = __shfl_sync(rows.mask, p_now.x, b, S);
+      p[1] = __shfl_sync(rows.mask, p_now.y, b, S);
+      p[2] = __shfl_sync(rows.mask, p_now.z, b, S);
+      p[3] = __shfl_sync(rows.mask, p_now.w, b, S);
+      rows.request(slot, key[slot], p);
+    };
+    window(0, k_now, p_now);
+    window(S, k_next, p_next);
 #pragma unroll
-    for (int g = 0; g < Rows<T, V>::kAhead; ++g) rows.request(g, k_now, p_now, g * kBatch);
+    for (int b = 0; b < kAhead; ++b) request(b, b);
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
-    uint32_t cur = __shfl_sync(0xffffffffu, k_now, 0);
+    uint32_t cur = key[0][0];
     bool continued = cur == left;  // the current run began in an earlier chunk
     uint32_t flags = continued && cur < vocab ? kHead : 0u;
-    if (lane == 0) run_key[warp] = cur;
-    for (int b = 0; b < m; b += 32) {
-      const int e = b + 32 + lane;
-      const uint32_t k_next = e < m ? keys[i0 + e] : 0xffffffffu;
-      const uint32_t p_next = e < m ? pos[i0 + e] : 0u;
+    if (lane == 0) run_key[group] = cur;
+    for (int b0 = 0; b0 < batches; b0 += kRing) {
 #pragma unroll
-      for (int g = 0; g < 32 / kBatch; ++g) {
-        if (b + g * kBatch >= m) break;
-        // a later batch is on its way while this one is added up
-        const int ahead = g + Rows<T, V>::kAhead;
-        if (ahead < 32 / kBatch)
-          rows.request(ahead, k_now, p_now, ahead * kBatch);
-        else
-          rows.request(ahead, k_next, p_next, (ahead - 32 / kBatch) * kBatch);
-        Vec<T, V> now[kBatch];
-        rows.take(g, now);
-        const uint32_t k0 = __shfl_sync(0xffffffffu, k_now, g * kBatch);
-        const uint32_t k3 = __shfl_sync(0xffffffffu, k_now, g * kBatch + kBatch - 1);
-        if (k0 == cur && k3 == cur && cur < vocab) {  // all of the current run: a tree
-          if (mine)
+      for (int g = 0; g < kRing; ++g) {
+        if (b0 + g >= batches) break;
+        // a later batch is on its way while this one is added up; the first of a window is
+        // always requested at g = 1
+        const int ahead = b0 + g + kAhead;
+        if (g == 1 && ahead % S == 0) {
+          k_now = k_next;
+          p_now = p_next;
+          window(ahead + S, k_next, p_next);
+        }
+        request((g + kAhead) % kRing, ahead % S);
+        rows.arrived();
+        const uint32_t(&k)[kBatch] = key[g];
+        float f[kBatch][V];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-              acc[j] += (now[0].get(j) + now[1].get(j)) +
-                        (now[2].get(j) + now[3].get(j));
+        for (int u = 0; u < kBatch; ++u) rows.take(g, u, f[u]);
+        if (k[0] == cur && k[kBatch - 1] == cur && cur < vocab) {  // all of the current run: a tree
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] += (f[0][j] + f[1][j]) + (f[2][j] + f[3][j]);
           continue;
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const uint32_t k = __shfl_sync(0xffffffffu, k_now, g * kBatch + u);
-          if (k >= vocab) continue;  // none, or sorted last: nothing follows but more of them
-          if (k != cur) {
-            if (mine) {
+          if (k[u] >= vocab) continue;  // none, or sorted last: nothing follows but more of them
+          if (k[u] != cur) {
+            if (rows.mine) {
               if (continued)
 #pragma unroll
-                for (int j = 0; j < V; ++j) edge[warp][0][lane * V + j] = acc[j];
+                for (int j = 0; j < V; ++j) edge[group][0][column<V, S, kEdge>(lane, j)] = acc[j];
               else
-                write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
+                write_row<W, V, S, kEdge>(dw_slab + static_cast<int64_t>(cur) * D, acc, scale, lane, rows.cols);
             }
-            cur = k;
+            cur = k[u];
             continued = false;
 #pragma unroll
             for (int j = 0; j < V; ++j) acc[j] = 0.f;
           }
-          if (mine)
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += now[u].get(j);
+          for (int j = 0; j < V; ++j) acc[j] += f[u][j];
         }
       }
-      k_now = k_next;
-      p_now = p_next;
     }
     rows.drain();
     if (cur < vocab) {
       const bool goes_on = cur == right;
       if (!goes_on && !continued) {
-        if (mine) write_row<W, V>(dw + static_cast<int64_t>(cur) * D + col, acc, scale);
+        if (rows.mine) write_row<W, V, S, kEdge>(dw_slab + static_cast<int64_t>(cur) * D, acc, scale, lane, rows.cols);
       } else {
         flags |= continued ? (goes_on ? kHeadOn : 0u) : kTail;
-        if (mine)
+        if (rows.mine)
 #pragma unroll
-          for (int j = 0; j < V; ++j) edge[warp][continued ? 0 : 1][lane * V + j] = acc[j];
+          for (int j = 0; j < V; ++j) edge[group][continued ? 0 : 1][column<V, S, kEdge>(lane, j)] = acc[j];
       }
     }
-    if (lane == 0) how[warp] = flags;
+    if (lane == 0) how[group] = flags;
   }
   __syncthreads();
   // the unit's chunks in order, one column per thread
-  for (int x = threadIdx.x; x < 32 * V; x += kSumThreads) {
-    const int c = slab * 32 * V + x;
+  for (int x = threadIdx.x; x < S * V; x += kSumThreads) {
+    const int c = slab * S * V + x;
     if (c >= D) continue;
     float acc = 0.f;
     bool carrying = false, began_here = false;
-    for (int w = 0; w < kSumWarps; ++w) {
+    for (int w = 0; w < kGroups; ++w) {
       const uint32_t f = how[w];
       if (f & kHead) {
         acc += edge[w][0][x];
@@ -523,23 +580,24 @@ __device__ __forceinline__ void sum_unit(const T* __restrict__ dy, const uint32_
 
 // Blocks [0, units * slabs) sum; those behind them zero the rows of the tokens that do not occur:
 // 32 rows and zero_cols columns per warp, a binary search of the sorted keys for each row.
-template <typename T, typename W, int V>
-__global__ void __launch_bounds__(kSumThreads, 3)
+template <typename T, typename W, int V, int S, bool kEdge>
+__global__ void __launch_bounds__(kSumThreads, 2)
     run_sums_kernel(const T* __restrict__ dy, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                     W* __restrict__ dw, float* __restrict__ partial, int64_t n, uint32_t vocab, int D, int L,
                     int slabs, int64_t sum_blocks, int zero_cols, int zero_slabs, float scale) {
   wait_previous_kernel();
-  extern __shared__ __align__(16) char rings[];
-  __shared__ float edge[kSumWarps][2][32 * V];
-  __shared__ uint32_t how[kSumWarps], run_key[kSumWarps];
+  extern __shared__ __align__(16) char ring[];
+  constexpr int kGroups = kSumThreads / S;
+  __shared__ float edge[kGroups][2][S * V];
+  __shared__ uint32_t how[kGroups], run_key[kGroups];
   if (blockIdx.x < sum_blocks) {
     const int64_t unit = blockIdx.x / static_cast<uint32_t>(slabs);
-    sum_unit<T, W, V>(dy, keys, pos, dw, partial, n, vocab, D, L, unit, static_cast<int>(blockIdx.x - unit * slabs),
-                      scale, edge, how, run_key, rings + (threadIdx.x >> 5) * Rows<T, V>::kRingBytes);
+    sum_unit<T, W, V, S, kEdge>(dy, keys, pos, dw, partial, n, vocab, D, L, unit, static_cast<int>(blockIdx.x - unit * slabs),
+                         scale, edge, how, run_key, ring);
     return;
   }
   const int lane = threadIdx.x & 31;
-  const int64_t item = (blockIdx.x - sum_blocks) * kSumWarps + (threadIdx.x >> 5);
+  const int64_t item = (blockIdx.x - sum_blocks) * (kSumThreads / 32) + (threadIdx.x >> 5);
   const int64_t row0 = item / zero_slabs * 32;
   if (row0 >= vocab) return;
   const uint32_t v = static_cast<uint32_t>(row0) + lane;
@@ -554,10 +612,10 @@ __global__ void __launch_bounds__(kSumThreads, 3)
   uint32_t absent = __ballot_sync(0xffffffffu, v < vocab && !(lo < n && keys[lo] == v));
   const int c0 = static_cast<int>(item % zero_slabs) * zero_cols;
   const int c1 = c0 + zero_cols < D ? c0 + zero_cols : D;
-  const float zero[V] = {};
+  constexpr int Z = kEdge ? 1 : 16 / static_cast<int>(sizeof(W));
   for (; absent; absent &= absent - 1) {
     W* row = dw + (row0 + __ffs(absent) - 1) * D;
-    for (int c = c0 + lane * V; c < c1; c += 32 * V) write_row<W, V>(row + c, zero, 0.f);
+    for (int c = c0 + lane * Z; c < c1; c += 32 * Z) st_vec<W, Z>(row + c, Vec<W, Z>::zero());
   }
 }
 
@@ -619,45 +677,91 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // ---- Forward ----------------------------------------------------------------------------------
 
-constexpr int kRowsAtOnce = 4;
+constexpr int kAtOnce = 4;  // vectors of a thread on their way
 
-// y = scale W[tokens]; rows of nv vectors of V elements. One warp takes kRowsAtOnce rows.
-template <typename T, typename I, int V>
+// y = scale W[tokens], as one array in vectors of V elements: thread by thread along tiles of
+// `tile_rows` rows (which begin on 16-byte boundaries), so that narrow rows and those that no vector
+// divides (kEdge) are written in whole vectors as well. by_row divides by the row's vectors, or
+// with kEdge by its elements.
+template <typename T, typename I, int V, bool kEdge>
 __global__ void __launch_bounds__(256)
     lookup_kernel(const I* __restrict__ tokens, const T* __restrict__ w, T* __restrict__ y, int64_t n, int64_t vocab,
-                  int D, float scale, bool streaming, uint32_t* status) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-  const int nv = D / V;
+                  int D, Divisor by_row, int tile_rows, float scale, bool streaming, uint32_t* status) {
   bool bad = false;
-  for (int64_t r = ((static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5) * kRowsAtOnce; r < n;
-       r += warps * kRowsAtOnce) {
-    int64_t tok[kRowsAtOnce];
+  const int64_t tiles = (n + tile_rows - 1) / tile_rows;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t row0 = tile * tile_rows;
+    const int rows = static_cast<int>(n - row0 < tile_rows ? n - row0 : tile_rows);
+    const uint32_t elements = static_cast<uint32_t>(rows) * static_cast<uint32_t>(D);
+    const uint32_t vectors = (elements + V - 1) / V;
+    const I* tok = tokens + row0;
+    T* out = y + row0 * D;
+    auto token = [&](uint32_t r) {
+      const int64_t t = static_cast<int64_t>(tok[r]);
+      const bool ok = t >= 0 && t < vocab;
+      if (!ok) bad = true;
+      return ok ? t : int64_t(-1);
+    };
+    for (uint32_t v0 = threadIdx.x; v0 < vectors; v0 += blockDim.x * kAtOnce) {
+      Vec<T, V> e[kAtOnce];
+      if constexpr (!kEdge) {
+        int64_t at[kAtOnce];
 #pragma unroll
-    for (int q = 0; q < kRowsAtOnce; ++q) tok[q] = r + q < n ? static_cast<int64_t>(tokens[r + q]) : 0;
-    for (int i = lane; i < nv; i += 32) {
-      Vec<T, V> e[kRowsAtOnce];
+        for (int q = 0; q < kAtOnce; ++q) {
+          const uint32_t v = v0 + q * blockDim.x;
+          at[q] = -1;
+          if (v >= vectors) continue;
+          const uint32_t r = by_row.quotient(v);
+          const int64_t t = token(r);
+          if (t >= 0) at[q] = t * D + static_cast<int64_t>(v - r * by_row.d) * V;
+        }
 #pragma unroll
-      for (int q = 0; q < kRowsAtOnce; ++q) {
-        const bool ok = tok[q] >= 0 && tok[q] < vocab;
-        if (ok)
-          e[q] = ld_vec<T, V>(w + tok[q] * D + static_cast<int64_t>(i) * V);
-        else {
-          bad = true;
-          e[q] = Vec<T, V>::zero();
+        for (int q = 0; q < kAtOnce; ++q) e[q] = at[q] >= 0 ? ld_vec<T, V>(w + at[q]) : Vec<T, V>::zero();
+      } else {
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const uint32_t v = v0 + q * blockDim.x;
+          float f[V] = {};
+          if (v < vectors) {
+            uint32_t r = by_row.quotient(v * V), c = v * V - r * D;
+            int64_t t = token(r);
+            if (c + V <= static_cast<uint32_t>(D)) {  // inside one row
+              const T* from = w + (t >= 0 ? t * D + c : 0);
+#pragma unroll
+              for (int j = 0; j < V; ++j) f[j] = t >= 0 ? Elem<T>::load(from[j]) : 0.f;
+            } else {
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                if (v * V + j >= elements) break;
+                if (c == static_cast<uint32_t>(D)) {
+                  c = 0;
+                  t = token(++r);
+                }
+                if (t >= 0) f[j] = Elem<T>::load(w[t * D + c]);
+                ++c;
+              }
+            }
+          }
+          e[q] = Vec<T, V>::of(f);
         }
       }
 #pragma unroll
-      for (int q = 0; q < kRowsAtOnce; ++q) {
-        if (r + q >= n) continue;
+      for (int q = 0; q < kAtOnce; ++q) {
+        const uint32_t v = v0 + q * blockDim.x;
+        if (v >= vectors) continue;
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = e[q].get(j) * scale;
-        T* to = y + (r + q) * D + static_cast<int64_t>(i) * V;
-        if (streaming)
+        T* to = out + static_cast<int64_t>(v) * V;
+        if (kEdge && v * V + V > elements) {  // the last vector of the array
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (v * V + j < elements) to[j] = Elem<T>::store(o[j]);
+        } else if (streaming) {
           st_vec_streaming<T, V>(to, Vec<T, V>::of(o));
-        else
+        } else {
           st_vec<T, V>(to, Vec<T, V>::of(o));
+        }
       }
     }
   }
@@ -673,17 +777,14 @@ int check_sizes(int64_t T, int64_t vocab, int64_t D) {
   return GTK_OK;
 }
 
-int vec_width(int64_t D, size_t bytes, bool aligned) {
-  return aligned && (D * bytes) % 16 == 0 ? static_cast<int>(16 / bytes) : 1;
-}
-
 // The backward's plan: what the workspace holds and how the sorted list is cut.
 struct Plan {
   int passes, bits;  // of the sort, for keys 0 .. vocab
   int per;           // tokens per thread, of the sort over tiles
   int64_t tiles;
   bool zero_first;   // all of dW is zeroed beside the sort
-  int64_t L, units;                            // entries of a warp's chunk; units of kSumWarps chunks
+  int lanes;                                   // of a group: 4 to 32, as many as have columns
+  int64_t L, units;                            // entries of a group's chunk; units of 256 / lanes chunks
   size_t keys, pos, counts, partial, total;    // byte offsets (keys, pos: two buffers each)
 };
 
@@ -704,14 +805,18 @@ Plan plan_for(int64_t T, int64_t vocab, int64_t D, int dy_dtype, int w_dtype) {
   // 26 us, against 37 us when the absent rows are looked up and zeroed after the sort).
   p.zero_first = T <= kClusterTokens &&
                  (T < vocab ? T : vocab) * D * static_cast<int64_t>(dtype_bytes(w_dtype)) <= (32 << 20);
-  // About 8 warps per SM get a chunk, of whole batches (24: 5 to 15% slower, more runs cross chunks). Up to 512 tokens make one unit: the
+  const int each = 16 / static_cast<int>(dtype_bytes(dy_dtype));  // columns of a lane
+  p.lanes = 4;
+  while (p.lanes < 32 && static_cast<int64_t>(p.lanes) * each < D) p.lanes <<= 1;
+  // About 8 warps per SM, in whole batches (24: 5 to 15% slower, more runs cross chunks); 16 where rows
+  // are taken apart by element, which takes longer per byte. Up to 512 tokens make one unit: the
   // launch that joins units costs more than the longer chunks.
-  const int64_t slab = 32 * 16 / static_cast<int64_t>(dtype_bytes(dy_dtype));
-  const int64_t slabs = (D + slab - 1) / slab;
-  int64_t L = T <= 512 ? (T + kSumWarps - 1) / kSumWarps : (T * slabs + 148 * 8 - 1) / (148 * 8);
+  const int64_t slabs = (D + p.lanes * each - 1) / (p.lanes * each), groups = kSumThreads / p.lanes;
+  const int64_t per_device = 148 * (D % each ? 2 : 1) * groups;
+  int64_t L = T <= 512 ? (T + groups - 1) / groups : (T * slabs + per_device - 1) / per_device;
   L = (L + kBatch - 1) / kBatch * kBatch;
   p.L = L > 1024 ? 1024 : L;
-  p.units = (T + p.L * kSumWarps - 1) / (p.L * kSumWarps);
+  p.units = (T + p.L * groups - 1) / (p.L * groups);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -804,54 +909,72 @@ int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** p
   }
 }
 
-template <typename T, typename W, int V>
+template <typename T, typename W, int S, bool kEdge>
 int sums(const Args& a, const Plan& p, const uint32_t* keys, const uint32_t* pos) {
-  const int slabs = static_cast<int>((a.D + 32 * V - 1) / (32 * V));
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kCols = S * V;
+  const int slabs = static_cast<int>((a.D + kCols - 1) / kCols);
   const int64_t sum_blocks = p.units * slabs;
-  const int zero_cols = 2 * 32 * V;
+  constexpr int kPerBlock = kSumThreads / 32;
+  const int zero_cols = 1024;
   const int zero_slabs = static_cast<int>((a.D + zero_cols - 1) / zero_cols);
   const int64_t zero_blocks =
-      p.zero_first ? 0 : ((a.vocab + 31) / 32 * zero_slabs + kSumWarps - 1) / kSumWarps;
+      p.zero_first ? 0 : ((a.vocab + 31) / 32 * zero_slabs + kPerBlock - 1) / kPerBlock;
   const int join_slabs = static_cast<int>((a.D + kJoinCols - 1) / kJoinCols);
   if (sum_blocks + zero_blocks > (int64_t(1) << 31) - 1 || p.units * join_slabs > (int64_t(1) << 31) - 1)
     return fail(GTK_ERR_UNSUPPORTED, "embedding: tokens or vocabulary times width too large");
   float* partial = reinterpret_cast<float*>(a.ws + p.partial);
   const uint32_t V32 = static_cast<uint32_t>(a.vocab);
-  auto kernel = run_sums_kernel<T, W, V>;
-  constexpr int kSmem = kSumWarps * Rows<T, V>::kRingBytes;
-  if (kSmem)
-    if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
-  if (int e = launch("embedding run sums", kernel, sum_blocks + zero_blocks, kSumThreads, kSmem, a.st, true, static_cast<const T*>(a.dy), keys, pos, static_cast<W*>(a.dw), partial, a.T, V32,
+  auto kernel = run_sums_kernel<T, W, V, S, kEdge>;
+  constexpr int kSmem = Rows<T, V, S, kEdge>::kRingBytes;
+  if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
+  if (int e = launch("embedding run sums", kernel, sum_blocks + zero_blocks, kSumThreads, kSmem, a.st, true,
+                     static_cast<const T*>(a.dy), keys, pos, static_cast<W*>(a.dw), partial, a.T, V32,
                      static_cast<int>(a.D), static_cast<int>(p.L), slabs, sum_blocks, zero_cols, zero_slabs, a.scale))
     return e;
   if (p.units == 1) return GTK_OK;
   return launch("embedding run join", join_runs_kernel<W>, (p.units - 1) * join_slabs, kJoinThreads, 0, a.st, true,
                 keys, static_cast<const float*>(partial), static_cast<W*>(a.dw), a.T, V32, static_cast<int>(a.D),
-                p.L * kSumWarps, join_slabs, a.scale);
+                p.L * (kSumThreads / S), join_slabs, a.scale);
+}
+
+template <typename T, typename W, bool kEdge>
+int sums_by_lanes(const Args& a, const Plan& p, const uint32_t* keys, const uint32_t* pos) {
+  switch (p.lanes) {
+    case 4:
+      return sums<T, W, 4, kEdge>(a, p, keys, pos);
+    case 8:
+      return sums<T, W, 8, kEdge>(a, p, keys, pos);
+    case 16:
+      return sums<T, W, 16, kEdge>(a, p, keys, pos);
+    default:
+      return sums<T, W, 32, kEdge>(a, p, keys, pos);
+  }
 }
 
 template <typename T, typename W>
 int backward_typed(const Args& a, const Plan& p, const uint32_t* keys, const uint32_t* pos) {
-  constexpr int VX = 16 / static_cast<int>(sizeof(T));
-  const bool vec = vec_width(a.D, sizeof(T), aligned16(a.dy)) > 1 && a.D * sizeof(W) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(a.dw) % (sizeof(W) * VX) == 0;
-  return vec ? sums<T, W, VX>(a, p, keys, pos) : sums<T, W, 1>(a, p, keys, pos);
+  return a.D % (16 / static_cast<int>(sizeof(T))) ? sums_by_lanes<T, W, true>(a, p, keys, pos)
+                                                  : sums_by_lanes<T, W, false>(a, p, keys, pos);
 }
 
 template <typename T, typename I>
 int forward_typed(const Args& a, const void* w, void* y) {
   constexpr int VX = 16 / static_cast<int>(sizeof(T));
-  const bool vec = vec_width(a.D, sizeof(T), aligned16(w) && aligned16(y)) > 1;
-  auto kernel = vec ? lookup_kernel<T, I, VX> : lookup_kernel<T, I, 1>;
-  int64_t blocks = (a.T + kRowsAtOnce * 8 - 1) / (kRowsAtOnce * 8);
-  const int64_t cap = static_cast<int64_t>(num_sms()) * 8;
-  if (blocks > cap) blocks = cap;
+  const bool edge = a.D % VX != 0 || !aligned16(w);  // rows of the table by element
+  const bool vec = aligned16(y);                     // else the output too
+  auto kernel = !vec ? lookup_kernel<T, I, 1, false> : edge ? lookup_kernel<T, I, VX, true> : lookup_kernel<T, I, VX, false>;
+  // Tiles of about 8192 elements, smaller where that leaves the device idle, in whole vectors.
+  int64_t rows = 8192 / a.D, few = (a.T + 4 * num_sms() - 1) / (4 * num_sms());
+  if (rows > few) rows = few;
+  rows = rows < 8 ? (edge ? 8 : rows < 1 ? 1 : rows) : rows / 8 * 8;
+  const int64_t tiles = (a.T + rows - 1) / rows, cap = int64_t(1) << 30;
   // An output that the L2 cache cannot hold anyway is written past it (512 x 512 pairs of 128 fp32
   // channels: 23.2 us instead of 26.8); a small one stays there for its reader.
   const bool streaming = a.T * a.D * static_cast<int64_t>(sizeof(T)) > (int64_t(64) << 20);
-  return launch("embedding lookup", kernel, blocks, 256, 0, a.st, false, static_cast<const I*>(a.tokens),
-                static_cast<const T*>(w), static_cast<T*>(y), a.T, a.vocab, static_cast<int>(a.D), a.scale, streaming,
-                a.status);
+  const Divisor by_row = divisor(static_cast<uint32_t>(vec && !edge ? a.D / VX : a.D));
+  return launch("embedding lookup", kernel, tiles < cap ? tiles : cap, 256, 0, a.st, false,
+                static_cast<const I*>(a.tokens), static_cast<const T*>(w), static_cast<T*>(y), a.T, a.vocab,
+                static_cast<int>(a.D), by_row, static_cast<int>(rows), a.scale, streaming, a.status);
 }
 
 template <typename I>
@@ -904,15 +1027,15 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
   emb::Plan p = emb::plan_for(n_tokens, vocab, D, dy_dtype, w_dtype);
   if (workspace_bytes < p.total) return fail(GTK_ERR_WORKSPACE, "embedding: workspace too small");
   if (int e = emb::check_tokens(tokens, index_bits)) return e;
-  if (int e = check_ptr(dy, "dy", dtype_bytes(dy_dtype))) return e;
-  if (int e = check_ptr(dweight, "dweight", dtype_bytes(w_dtype))) return e;
+  if (int e = check_ptr(dy, "dy")) return e;
+  if (int e = check_ptr(dweight, "dweight")) return e;
   if (int e = check_ptr(workspace, "workspace", 256)) return e;
   if (int e = check_device()) return e;
   emb::Args a = {};
   a.tokens = tokens, a.dy = dy, a.dw = dweight, a.ws = static_cast<char*>(workspace), a.T = n_tokens;
   a.vocab = vocab, a.D = D, a.padding = padding, a.scale = scale, a.status = status;
   a.dw_bytes = vocab * D * static_cast<int64_t>(dtype_bytes(w_dtype));
-  p.zero_first = p.zero_first && aligned16(dweight) && a.dw_bytes % 16 == 0;
+  p.zero_first = p.zero_first && a.dw_bytes % 16 == 0;
   a.st = static_cast<cudaStream_t>(stream);
   const uint32_t *keys = nullptr, *pos = nullptr;
   if (int e = index_bits == 64 ? emb::sort<int64_t>(a, p, &keys, &pos) : emb::sort<int32_t>(a, p, &keys, &pos))

@@ -58,21 +58,6 @@ constexpr int kMaxStages = 2;             // turns in the ring: this one and the
 constexpr int kRingBytes = 200 * 1024;    // most of an SM
 constexpr int kMaxCluster = 8;
 
-// Division of n < 2^31 by a constant of the launch.
-struct Divisor {
-  uint32_t d, m, shift;
-  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> shift; }
-};
-
-// With l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1, floor(n m / 2^(31 + l)) is n / d for
-// n < 2^31 (m d exceeds 2^(31 + l) by e <= d <= 2^l, and n e < 2^(31 + l)).
-Divisor divisor(uint32_t d) {
-  uint32_t l = 0;
-  while ((uint64_t(1) << l) < d) ++l;
-  if (d <= 1) return Divisor{1, 0, 0};
-  return Divisor{d, static_cast<uint32_t>((uint64_t(1) << (31 + l)) / d + 1), l - 1};
-}
-
 // Where row r of a tensor with up to three leading axes begins: r = (a n1 + b) n2 + c lies
 // at a s0 + b s1 + c s2 (element strides); `plain`: rows follow one another, s2 apart.
 struct RowMap {

@@ -167,6 +167,21 @@ __device__ __forceinline__ void st_vec_streaming(T* p, const Vec<T, V>& v) {
     st_vec<T, V>(p, v);
 }
 
+// Division of n < 2^31 by a constant of the launch.
+struct Divisor {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> shift; }
+};
+
+// With l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1, floor(n m / 2^(31 + l)) is n / d for
+// n < 2^31 (m d exceeds 2^(31 + l) by e <= d <= 2^l, and n e < 2^(31 + l)).
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  if (d <= 1) return Divisor{1, 0, 0};
+  return Divisor{d, static_cast<uint32_t>((uint64_t(1) << (31 + l)) / d + 1), l - 1};
+}
+
 // Waits until the kernel before this one on the stream has finished and its writes are
 // visible; at once when the launch carried no programmatic dependency.
 __device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -431,7 +431,9 @@ Tensor embedding_backward(const Tensor& dy_in, const Tensor& tokens_in, int64_t 
   const auto options = dy_in.options().dtype(wd);
   if (n == 0 || D == 0) return at::zeros({vocab, D}, options);
   Tensor dw = at::empty({vocab, D}, options);
-  const Tensor tokens = contiguous(tokens_in), dy = contiguous(dy_in);
+  const Tensor tokens = contiguous(tokens_in);
+  Tensor dy = contiguous(dy_in);
+  if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone();  // a view that begins off a vector
   const size_t bytes = api.embedding_backward_workspace_bytes(n, vocab, D, gt);
   Tensor ws = scratch(bytes, dy);
   check(api.embedding_backward(dy.data_ptr(), gt, tokens.data_ptr(), bits, dw.data_ptr(), code_of(wd), n, vocab, D,

@@ -535,7 +535,7 @@ GTK_API int gtk_clip_grad_norm(const void* const* grads, void* const* outs, cons
  * it written. n_tokens, vocab < 2^31, D <= 2^20. The row `padding` (-1: none) of dweight is
  * zeros; the lookup reads it like any other. Tokens out of range set GTK_STATUS_BAD_TOKEN.
  * fp32 sums in a fixed order, one rounding at the end; no floating-point atomics:
- * the same inputs give the same bits. The workspace is aligned to 256 bytes.
+ * the same inputs give the same bits. dy and dweight are aligned to 16 bytes, the workspace to 256.
  * ------------------------------------------------------------------------------- */
 GTK_API int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight, int dtype, void* y,
                                   int64_t n_tokens, int64_t vocab, int64_t D, float scale, uint32_t* status,

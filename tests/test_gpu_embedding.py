@@ -79,6 +79,23 @@ def test_gradient(T, V, D, dtype, wdtype):
                             DT[wdtype])
 
 
+@pytest.mark.parametrize("D", [1, 2, 4, 7, 8, 15, 16, 17, 24, 31, 32, 40, 63, 64, 65, 96, 127, 129, 250, 256, 260, 515])
+def test_widths(D):
+    """Groups of 4 to 32 lanes, one slab of columns or several, vectors and single elements."""
+    dev = require_gpu()
+    from genie_tk import ops
+    gen = torch.Generator(device=dev).manual_seed(D)
+    for T, V in ((3, 5), (600, 7), (3000, 40), (9001, 5000)):
+        tok = _tokens("zipf", T, V, dev, T)
+        for dtype in (torch.float32, torch.bfloat16):
+            dy = torch.randn(T, D, generator=gen, device=dev).to(dtype)
+            _check_backward(dy, tok, V)
+            _check_backward(dy, tok, V, 2.0, 1, torch.float32)
+            w = torch.randn(V, D, generator=gen, device=dev).to(dtype)
+            assert torch.equal(ops.embedding_forward(tok, w), w[tok])
+            assert torch.equal(ops.embedding_forward(tok, w, 0.5), w[tok] * 0.5)
+
+
 @pytest.mark.parametrize("kind", ["one", "down", "sorted"])
 @pytest.mark.parametrize("T", [1, 32, 33, 512, 513, 700, 1024, 1025, 4097, 8192, 8193, 16385, 32768, 32769, 50001, 131073, 262145, 600001])
 def test_orders_of_tokens(kind, T):
