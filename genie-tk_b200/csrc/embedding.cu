@@ -10,7 +10,7 @@
 // Backward: HBM bound too -- it reads dy once and writes the whole of dW once -- if the rows
 // of one token can be found together. So the tokens are sorted first (stable, least digit first,
 // up to 8 bits a pass; four bytes of key and four of position per token, small beside dy; one
-// cluster of blocks does it up to 32,768 tokens), and the sorted list is cut into chunks of equal length,
+// cluster of blocks does it up to 8192 tokens), and the sorted list is cut into chunks of equal length,
 // whatever the tokens' frequencies: a group of 4 to 32 lanes (as the row is wide) sums the dy rows of
 // its chunk in registers, in list order, with the next twelve rows in flight, and writes a row of dW
 // at each change of token. Runs
@@ -29,14 +29,14 @@ namespace emb {
 
 constexpr int kSortThreads = 1024;
 constexpr int kMaxCluster = 8;                    // sorting blocks that exchange through their shared memory
-constexpr int kClusterPer = 4;                    // most tokens per thread of such a block
-constexpr int64_t kClusterTokens = static_cast<int64_t>(kSortThreads) * kClusterPer * kMaxCluster;
+constexpr int64_t kClusterTokens = static_cast<int64_t>(kSortThreads) * kMaxCluster;
 constexpr int kMaxPer = 8;                        // tokens per thread of the sort over many tiles
 constexpr int kMaxBits = 8;                       // of a digit
 constexpr int kBins = 1 << kMaxBits;
 constexpr int kWarps = kSortThreads / 32;
 constexpr int kSlices = kSortThreads / kBins;     // threads per bin
 constexpr int kMaxWidth = 1 << 20;
+constexpr int64_t kMaxSorted = int64_t(1) << 27;  // tokens of a backward call
 
 // The key of token v: itself, or V (sorted last and then ignored) when it is out of range or padding.
 __device__ __forceinline__ uint32_t key_of(int64_t v, uint32_t V, int64_t padding, bool* bad) {
@@ -132,12 +132,12 @@ __device__ __forceinline__ int tile_index(int i) {
   return (threadIdx.x >> 5) * 32 * N + i * 32 + (threadIdx.x & 31);
 }
 
-// The whole sort in one launch of one cluster: up to eight blocks of 1024 N tokens each, which
-// read one another's digit counts and send every token to the block of its next place
-// through distributed shared memory. Four launches over tiles took 14 us for 8192 tokens where
-// this takes 7.
+// The whole sort in one launch of one cluster: up to eight blocks of 1024 tokens, which read one
+// another's digit counts and send every token to the block of its next place through distributed
+// shared memory. (Four launches over tiles take 3 us longer for 8192 tokens in two passes. With more
+// tokens per thread the cluster falls behind the tiles from 10,000 tokens on.)
 // Further clusters, where `zero` is given, zero `zero_bytes` there meanwhile (16-byte multiples).
-template <typename I, int N>
+template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
     sort_cluster_kernel(const I* __restrict__ tokens, int T, uint32_t V, int64_t padding, int passes, int bits,
                         uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint4* __restrict__ zero,
@@ -151,10 +151,10 @@ __global__ void __launch_bounds__(kSortThreads)
       zero[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  extern __shared__ uint32_t buf[];  // [2][1024 N]: keys, positions
+  extern __shared__ uint32_t buf[];  // [2][1024]: keys, positions
   __shared__ SortShared s;
   __shared__ uint32_t totals[kBins];
-  constexpr int kHere = kSortThreads * N;
+  constexpr int kHere = kSortThreads, N = 1;  // tokens of a block, and of a thread
   const int blocks = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
   bool bad = false;
   uint32_t key[N], pos[N];
@@ -842,13 +842,13 @@ struct Args {
   cudaStream_t st;
 };
 
-template <typename I, int N>
+template <typename I>
 int sort_cluster(const Args& a, const Plan& p, uint32_t* keys, uint32_t* pos) {
-  auto kernel = sort_cluster_kernel<I, N>;
-  const int smem = 2 * kSortThreads * N * 4;
+  auto kernel = sort_cluster_kernel<I>;
+  const int smem = 2 * kSortThreads * 4;
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), smem)) return e;
   int blocks = 1;
-  while (static_cast<int64_t>(blocks) * kSortThreads * N < a.T) blocks <<= 1;
+  while (static_cast<int64_t>(blocks) * kSortThreads < a.T) blocks <<= 1;
   const int64_t zero_bytes = p.zero_first ? a.dw_bytes : 0;
   // two blocks per SM, in whole clusters, but no more than there are 64 KB pieces
   int64_t zero_blocks = (zero_bytes + 65535) / 65536;
@@ -892,10 +892,7 @@ int sort(const Args& a, const Plan& p, const uint32_t** keys, const uint32_t** p
   if (a.T <= kClusterTokens) {
     *keys = k[0];
     *pos = q[0];
-    // as few tokens per thread as the cluster allows: their ranks are found one after another
-    if (a.T <= kSortThreads * kMaxCluster) return sort_cluster<I, 1>(a, p, k[0], q[0]);
-    if (a.T <= 2 * kSortThreads * kMaxCluster) return sort_cluster<I, 2>(a, p, k[0], q[0]);
-    return sort_cluster<I, kClusterPer>(a, p, k[0], q[0]);
+    return sort_cluster<I>(a, p, k[0], q[0]);
   }
   switch (p.per) {
     case 1:
@@ -1021,6 +1018,8 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
                            int w_dtype, int64_t n_tokens, int64_t vocab, int64_t D, float scale, int64_t padding,
                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
   if (int e = emb::check_sizes(n_tokens, vocab, D)) return e;
+  // every tile of the sort reads all tiles' counts: beyond this it would take longer than it is worth
+  if (n_tokens > emb::kMaxSorted) return fail(GTK_ERR_UNSUPPORTED, "embedding: the gradient takes up to 2^27 tokens");
   if (!dtype_ok(dy_dtype) || !(w_dtype == dy_dtype || w_dtype == GTK_F32))
     return fail(GTK_ERR_UNSUPPORTED, "embedding: dy is fp32, bf16 or fp16, the table's gradient fp32 or dy's type");
   if (padding >= vocab) return fail(GTK_ERR_INVALID_ARG, "embedding: the padding token must be below the vocabulary");

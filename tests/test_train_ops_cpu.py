@@ -113,7 +113,8 @@ def test_embedding_entry_points(lib):
 
     assert bwd(gt=0, wt=1) == -2 and bwd(gt=1, wt=2) == -2 and bwd(pad=10) == -1 and bwd(nb=16) == L.GTK_ERR_WORKSPACE
     assert bwd(dy=None) == -1 and bwd(dw=q) == L.GTK_ERR_ALIGNMENT and bwd(n=1 << 31) == -1
-    assert bwd(ws=P((1 << 20) + 16)) == L.GTK_ERR_ALIGNMENT
+    assert bwd(ws=P((1 << 20) + 16)) == L.GTK_ERR_ALIGNMENT and bwd(n=(1 << 27) + 1) == -2
+    assert bwd(dy=P((1 << 20) + 4)) == L.GTK_ERR_ALIGNMENT and bwd(dw=P((1 << 20) + 8)) == L.GTK_ERR_ALIGNMENT
 
 
 def test_wrappers_refuse_before_the_device_is_needed():
