@@ -134,6 +134,8 @@ class LayerNormFn(torch.autograd.Function):
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = LN_EPS) -> Tensor:
     """Differentiable LayerNorm over the last axis on the library's kernels: x [*, D] fp32, bf16
     or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable."""
+    if weight is None and bias is not None:
+        weight = torch.ones_like(bias)  # the parameters' gradients have the weight's type
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return LayerNormFn.apply(x, weight, bias, eps)
     return ops.layernorm_forward(x, weight, bias, eps)[0]

@@ -255,6 +255,41 @@ def test_same_bits_every_time_on_any_stream_and_from_graphs():
     assert all(torch.equal(a, b_) for a, b_ in zip(graphs[0][1], want2))
 
 
+@pytest.mark.parametrize("rows,D", [(1, 384), (37, 384), (64, 128), (8, 5000), (5, 5003), (7, 8185), (250, 16), (300, 33)])
+def test_few_rows_join_in_one_cluster(rows, D):
+    """Grids of up to eight blocks: one launch that joins the parameters' gradients itself, on two
+    streams at once and from a graph; parts of the gradients only."""
+    dev = require_gpu()
+    from genie_tk import ops
+    args = [_inputs((rows, D), torch.float32, torch.float32, s, dev) for s in (1, 2)]
+    for a in args:
+        _run_and_check(*a)
+
+    def back(x, dy, w, b, *need):
+        _, mean, rstd = ops.layernorm_forward(x, w, b)
+        return ops.layernorm_backward(dy, x, w, mean, rstd, *need)
+
+    want = [back(*a) for a in args]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in args], []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, back(*args[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for i, g in got for p, q in zip(g, want[i]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = back(*args[0])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, want[0]))
+    dx, dw, db = back(*args[0], False, True)
+    assert dw is None and torch.equal(db, want[0][2]) and torch.equal(dx, want[0][0])
+    dx, dw, db = back(*args[0], True, False)
+    assert db is None and torch.equal(dw, want[0][1])
+
+
 def test_module_and_autograd():
     dev = require_gpu()
     torch.manual_seed(0)
