@@ -33,13 +33,13 @@
 //
 // Rows of a transposed pair tensor lie far apart in one axis and next to one another in the other.
 // They are visited in tiles of 8 x 4, which reads runs of eight rows and writes runs of four
-// (in plain order, the backward of 512 x 512 x 128 fp32 took 82 us instead of 70).
+// (in plain order, the backward of 512 x 512 x 128 fp32 takes 75 us instead of 73).
 //
 // dw and db: a thread meets the same columns in every row of its group, so it sums them in
 // registers over all the group's rows; the block's groups are then joined in shared memory,
 // the block writes one partial row, and a second kernel adds the partials in a fixed order. A grid
 // of up to eight blocks is launched as one cluster and adds them itself, through distributed shared
-// memory (37 rows of 384: 9.6 us a call instead of 7).
+// memory (37 rows of 384: 4.2 us instead of 5.0 from a graph, 8.5 instead of 10.7 from Python).
 // No atomics: the same inputs give the same bits.
 #include <cooperative_groups.h>
 
@@ -653,24 +653,25 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
   }
   __syncthreads();
   cols = reinterpret_cast<float*>(ring);
-  if (!direct) {
-    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
-      float t = 0.f;
-      for (int q = 0; q < parts; ++q) t += cols[q * 2 * D + i];
+  for (int i = threadIdx.x; i < 2 * D && (parts > 1 || !direct); i += blockDim.x) {
+    float t = 0.f;
+    for (int q = 0; q < parts; ++q) t += cols[q * 2 * D + i];
+    if (direct)
+      cols[i] = t;
+    else
       pw[i < D ? i : i - D + ld] = t;
-    }
-    return;
   }
+  if (!direct) return;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = static_cast<int>(cluster.num_blocks());
   cluster.sync();
   for (int i = cluster.block_rank() * blockDim.x + threadIdx.x; i < 2 * D; i += blocks * blockDim.x) {
-    float t = 0.f;
-    for (int r = 0; r < blocks; ++r) {
-      const float* there = cluster.map_shared_rank(cols, r);
-      for (int q = 0; q < parts; ++q) t += there[q * 2 * D + i];
-    }
+    float v[kMaxCluster], t = 0.f;  // all on their way together
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) v[r] = r < blocks ? cluster.map_shared_rank(cols, r)[i] : 0.f;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) t += v[r];
     if (i < D) {
       if (dw) dw[i] = Elem<W>::store(t);
     } else if (db) {
@@ -856,10 +857,10 @@ struct Args {
 };
 
 // The ring: stages, bytes, and the blocks of an SM. What is on its way should be about what HBM
-// needs for its latency, 64 KB an SM; 16-bit rows take twice that, as their arithmetic takes longer.
-// More costs: reads far ahead of the writes leave the DRAM pages that the writes need (512 x 512 x
-// 128 fp32, forward / backward: 46 / 66 us with 64 KB an SM, 49 / 71 us with 200 KB; 4096 x 4096
-// bf16: 14.4 / 28.7 us, against 16.4 / 29.1 us).
+// needs for its latency, 64 KB an SM; 16-bit rows take what there is, as their arithmetic takes longer.
+// More costs in fp32: reads far ahead of the writes leave the DRAM pages that the writes need (512 x
+// 512 x 128, backward: 66 us with 64 KB an SM, 70 with 200 KB; 4096 x 4096 bf16: 28.8 with 128 KB,
+// 26.8 with 200 KB).
 struct Ring {
   int stages, bytes, blocks;
 };
@@ -868,7 +869,7 @@ Ring ring_for(int threads, int K, int tensors, int most_blocks, int extra, size_
   Ring r = {1, 0, most_blocks < 1 ? 1 : most_blocks};
   const int stage = tensors * K * threads * R::kBytes + extra;
   if (R::kAsync) {
-    const int want = (elem_bytes == 4 ? 64 : 128) * 1024 / (kMaxStages * stage);
+    const int want = (elem_bytes == 4 ? 64 : 200) * 1024 / (kMaxStages * stage);
     if (r.blocks > want) r.blocks = want < 1 ? 1 : want;
     r.stages = kRingBytes / r.blocks / stage;
     r.stages = r.stages < 1 ? 1 : r.stages > kMaxStages ? kMaxStages : r.stages;
