@@ -532,8 +532,9 @@ GTK_API int gtk_clip_grad_norm(const void* const* grads, void* const* outs, cons
  *   dweight[v, :] = scale * sum over the t with tokens[t] = v of dy[t, :]
  * tokens int32 or int64 (index_bits) [n_tokens]; weight [vocab, D] and y [n_tokens, D] of one
  * type (dtype); dy [n_tokens, D] (dy_dtype), dweight [vocab, D] in GTK_F32 or dy's type, all of
- * it written. n_tokens, vocab < 2^31 (the gradient: n_tokens <= 2^27), D <= 2^20. The row `padding` (-1: none) of dweight is
- * zeros; the lookup reads it like any other. Tokens out of range set GTK_STATUS_BAD_TOKEN.
+ * it written. n_tokens, vocab < 2^31 (the gradient: n_tokens <= 2^27), D <= 2^20. The row
+ * `padding` (-1: none) of dweight is zeros; the lookup reads it like any other. Tokens out of
+ * range set GTK_STATUS_BAD_TOKEN.
  * fp32 sums in a fixed order, one rounding at the end; no floating-point atomics:
  * the same inputs give the same bits. dy and dweight are aligned to 16 bytes, the workspace to 256.
  * ------------------------------------------------------------------------------- */
