@@ -405,8 +405,9 @@ int run(const Request& r, int64_t n_given) {
   if (!r.scale || r.t.empty())
     return launch("gradient norm", norm_only_kernel, 1, kThreads, 0, r.st, !r.t.empty(), partial, partials,
                   r.inf_norm, r.norm);
+  auto scale = coarse(r.elements) ? clip_scale_kernel<kCoarse> : clip_scale_kernel<kFine>;
   for (size_t i = 0; i < launches; ++i)
-    if (int e = launch("gradient clipping", coarse(r.elements) ? clip_scale_kernel<kCoarse> : clip_scale_kernel<kFine>, parts[i].blocks, kThreads, 0, r.st, i == 0,
+    if (int e = launch("gradient clipping", scale, parts[i].blocks, kThreads, 0, r.st, i == 0,
                        static_cast<const Shadow*>(parts[i].shadow), parts[i].tensors, parts[i].chunks,
                        partial, partials, r.inf_norm, r.max_norm, r.in_place,
                        i == 0 ? r.norm : static_cast<float*>(nullptr)))

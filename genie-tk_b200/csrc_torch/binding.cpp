@@ -7,6 +7,7 @@
 // allocator on the current stream, and the kernels run on the tensors' device and its current
 // stream. Workspaces are allocated per call: two streams or two captured graphs never share one.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -97,13 +98,13 @@ int dtype_code(const Tensor& t, const char* name) {
 void require_cuda(const Tensor& t, const char* name) {
   if (!t.is_cuda())
     throw std::runtime_error(kPrefix + name + " must be a CUDA tensor; this package has no CPU path");
-  if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
+  if (t.layout() != at::kStrided || t.is_neg()) type_error(std::string(name) + " must be a dense tensor");
 }
 
 void same_device(const Tensor& t, c10::Device d, const char* name) {
   if (!t.is_cuda() || t.device() != d)
     throw std::runtime_error(kPrefix + name + " must be a CUDA tensor on device " + std::to_string(d.index()));
-  if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
+  if (t.layout() != at::kStrided || t.is_neg()) type_error(std::string(name) + " must be a dense tensor");
 }
 
 std::string shape_of(const Tensor& t) {
@@ -247,6 +248,11 @@ struct Gradients {
   std::vector<std::pair<Tensor, Tensor>> write_back;  // (gradient, its clipped copy)
 };
 
+// Dense, and holding its values as they are (not a lazily negated view).
+bool dense(const c10::TensorImpl* t) {
+  return t->layout() == at::kStrided && !t->key_set().has(c10::DispatchKey::Negative);
+}
+
 // Item i of a list of tensors. (Reads the TensorImpl directly from here on: a list may hold
 // hundreds of gradients, and every call on a Tensor counts.)
 c10::TensorImpl* tensor_at(PyObject* o, const char* name, Py_ssize_t i) {
@@ -302,7 +308,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     c10::TensorImpl* t = tensor_at(items[i], "grads", i);
     if (t->device() != device)
       throw std::runtime_error(kPrefix + "all gradients must be CUDA tensors on one device");
-    if (t->layout() != at::kStrided) type_error("gradients must be dense tensors");
+    if (!dense(t)) type_error("gradients must be dense tensors");
     const at::ScalarType st = c10::typeMetaToScalarType(t->dtype());
     const int code = code_of(st);
     if (code < 0) type_error("gradients must be float32, bfloat16 or float16, got " + name_of(st));
@@ -310,7 +316,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     if (outs) {
       prefetch(out_items, i, n);
       c10::TensorImpl* o = tensor_at(out_items[i], "out", i);
-      if (o->device() != device || o->layout() != at::kStrided)
+      if (o->device() != device || !dense(o))
         throw std::runtime_error(kPrefix + "out must hold dense CUDA tensors on the gradients' device");
       if (o->sizes() != t->sizes()) value_error("out[" + std::to_string(i) + "] must have its gradient's shape");
       const at::ScalarType ot = c10::typeMetaToScalarType(o->dtype());
@@ -329,6 +335,8 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     } else {
       if (clip && !t->is_inference()) t->bump_version();
       if (!plain && !t->is_non_overlapping_and_dense()) {
+        if (clip && at::has_internal_overlap(t) == at::MemOverlap::Yes)
+          value_error("grads[" + std::to_string(i) + "] holds an element more than once and cannot be clipped in place");
         g->keep.push_back(handle(t).contiguous());
         if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
         t = g->keep.back().unsafeGetTensorImpl();

@@ -163,14 +163,17 @@ def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: O
     """Differentiable scale * weight[tokens] on the library's kernels: tokens int32 or int64 [*],
     weight [vocabulary, D]; the row ``padding_idx`` gets no gradient. Once differentiable; the
     table's gradient is dense and the same from run to run."""
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"genie_tk (B200): padding_idx must be a token of the vocabulary, got {padding_idx}")
     if torch.is_grad_enabled() and weight.requires_grad:
         return EmbeddingFn.apply(tokens, weight, scale, padding_idx)
     return ops.embedding_forward(tokens, weight, scale)
 
 
 def _ln(x: Tensor, p: Dict[str, Tensor], name: str) -> Tensor:
-    """LayerNorm of a recompute: on the library's kernels (CPU tensors: PyTorch's)."""
-    w, b = p[name + ".weight"], p[name + ".bias"]
+    """LayerNorm of a recompute, in fp32 (under autocast too, where a product before it is not): on
+    the library's kernels (CPU tensors: PyTorch's)."""
+    x, w, b = x.float(), p[name + ".weight"], p[name + ".bias"]
     return layer_norm(x, w, b, LN_EPS) if x.is_cuda else F.layer_norm(x, (x.shape[-1],), w, b, LN_EPS)
 
 

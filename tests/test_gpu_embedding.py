@@ -307,3 +307,7 @@ def test_refusals():
                     (RuntimeError, lambda: ops.embedding_backward(dy, tok.cpu(), 10))):
         with pytest.raises(e):
             call()
+    from genie_tk import autograd
+    for bad in (-1, 10):
+        with pytest.raises(ValueError, match="padding_idx"):
+            autograd.embedding(tok, w, 1.0, bad)

@@ -273,4 +273,11 @@ def test_refusals():
         ops.clip_grad_norm([g.view(10, 10)], 1.0, out=[torch.empty(10, 20, device=dev)[:, ::2]])
     with pytest.raises(ValueError):
         ops.grad_norm([g], 1.0)
+    with pytest.raises(ValueError, match="more than once"):
+        ops.clip_grad_norm([g, torch.randn(1, 4, device=dev).expand(3, 4)], 1e-3)
+    with pytest.raises(TypeError, match="dense"):  # a lazily negated view
+        ops.grad_norm([torch.zeros(4, dtype=torch.complex64, device=dev).conj().imag])
     assert torch.equal(g, kept)
+    # read only, an expanded gradient is as good as any
+    e = torch.randn(1, 4, device=dev).expand(3, 4)
+    torch.testing.assert_close(ops.grad_norm([e]), e.double().norm().float(), rtol=1e-6, atol=0)

@@ -156,3 +156,69 @@ def test_functional_step_in_a_graph():
         want = step()
         assert all(torch.equal(a, c) for a, c in zip(out, want))
         assert float(out[-1]) > 1.0
+
+
+def test_modules_in_a_graph():
+    """Forward, backward and clipping through the modules in one graph, by PyTorch's rules for it: the
+    passes before the capture run on a side stream, and nothing of their autograd graph is left."""
+    dev = require_gpu()
+    torch.manual_seed(2)
+    emb, norm = genie_tk.Embedding(30, 64, padding_idx=3).to(dev), genie_tk.LayerNorm(64).to(dev)
+    params = [*emb.parameters(), *norm.parameters()]
+    tokens, target = torch.randint(0, 30, (3, 17), device=dev), torch.randn(3, 17, 64, device=dev)
+
+    def step():
+        loss = (norm(emb(tokens)) - target).square().mean()
+        loss.backward()
+        return loss.detach(), genie_tk.clip_grad_norm_(params, 1e-2)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            for p in params:
+                p.grad = None
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for p in params:
+        p.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, total = step()
+    for seed in range(2):
+        torch.manual_seed(seed)
+        tokens.copy_(torch.randint(0, 30, (3, 17)))
+        target.copy_(torch.randn(3, 17, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        y = F.layer_norm(F.embedding(tokens, emb.weight.double(), 3), (64,), norm.weight.double(), norm.bias.double())
+        want_loss = (y - target).square().mean()
+        want = torch.autograd.grad(want_loss, params)
+        full = torch.sqrt(sum(w.double().square().sum() for w in want))
+        torch.testing.assert_close(loss.double(), want_loss, rtol=1e-5, atol=0)
+        torch.testing.assert_close(total.double(), full, rtol=1e-5, atol=0)
+        for p, w in zip(params, want):
+            assert float((p.grad - w * (1e-2 / full)).norm()) <= 1e-4 * float((w * (1e-2 / full)).norm()) + 1e-9
+    assert_status_clean(dev)
+
+
+def test_block_backward_under_autocast():
+    """A block's gradients when its backward is called under autocast: the recomputation's products
+    are bf16 there (2^-8 a rounding at most, up to twelve in a row), its LayerNorms stay fp32."""
+    dev = require_gpu()
+    torch.manual_seed(4)
+    block = genie_tk.TriangleMultiplicationOutgoing(128, 128).to(dev)
+    for p in block.parameters():
+        torch.nn.init.normal_(p, std=0.1)
+    shape = (1, 20, 20, 128)
+    x = torch.randn(shape, device=dev, requires_grad=True)
+    mask = torch.ones(shape[:-1], device=dev)
+    dy = torch.randn(shape, device=dev)
+    grads = []
+    for cast in (False, True):
+        y = block(x, mask)
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=cast):
+            grads.append(torch.autograd.grad(y, [x, *block.parameters()], dy))
+    for a, b in zip(*grads):
+        assert a.dtype == b.dtype and float((a - b).norm()) <= 0.05 * float(a.norm())
