@@ -389,7 +389,8 @@ struct Rows {
       uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring + (slot * kBatch + u) * kRowBytes));
       if constexpr (!kEdge) {
         if (mine)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + lane * 16), "l"(row + lane * V) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + lane * 16), "l"(row + lane * V)
+                       : "memory");
       } else {
         const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u);
         const char* from = reinterpret_cast<const char*>(row) - before;
@@ -592,8 +593,8 @@ __global__ void __launch_bounds__(kSumThreads, 2)
   __shared__ uint32_t how[kGroups], run_key[kGroups];
   if (blockIdx.x < sum_blocks) {
     const int64_t unit = blockIdx.x / static_cast<uint32_t>(slabs);
-    sum_unit<T, W, V, S, kEdge>(dy, keys, pos, dw, partial, n, vocab, D, L, unit, static_cast<int>(blockIdx.x - unit * slabs),
-                         scale, edge, how, run_key, ring);
+    sum_unit<T, W, V, S, kEdge>(dy, keys, pos, dw, partial, n, vocab, D, L, unit,
+                                static_cast<int>(blockIdx.x - unit * slabs), scale, edge, how, run_key, ring);
     return;
   }
   const int lane = threadIdx.x & 31;
@@ -772,7 +773,8 @@ __global__ void __launch_bounds__(256)
 
 int check_sizes(int64_t T, int64_t vocab, int64_t D) {
   if (!dims_ok(T, (int64_t(1) << 31) - 1)) return fail(GTK_ERR_INVALID_ARG, "embedding: tokens must be 1..2^31-1");
-  if (!dims_ok(vocab, (int64_t(1) << 31) - 1)) return fail(GTK_ERR_INVALID_ARG, "embedding: vocabulary must be 1..2^31-1");
+  if (!dims_ok(vocab, (int64_t(1) << 31) - 1))
+    return fail(GTK_ERR_INVALID_ARG, "embedding: vocabulary must be 1..2^31-1");
   if (!dims_ok(D, kMaxWidth)) return fail(GTK_ERR_INVALID_ARG, "embedding: width must be 1..2^20");
   return GTK_OK;
 }
@@ -959,7 +961,9 @@ int forward_typed(const Args& a, const void* w, void* y) {
   constexpr int VX = 16 / static_cast<int>(sizeof(T));
   const bool edge = a.D % VX != 0 || !aligned16(w);  // rows of the table by element
   const bool vec = aligned16(y);                     // else the output too
-  auto kernel = !vec ? lookup_kernel<T, I, 1, false> : edge ? lookup_kernel<T, I, VX, true> : lookup_kernel<T, I, VX, false>;
+  auto kernel = !vec   ? lookup_kernel<T, I, 1, false>
+                : edge ? lookup_kernel<T, I, VX, true>
+                       : lookup_kernel<T, I, VX, false>;
   // Tiles of about 8192 elements, smaller where that leaves the device idle, in whole vectors.
   int64_t rows = 8192 / a.D, few = (a.T + 4 * num_sms() - 1) / (4 * num_sms());
   if (rows > few) rows = few;

@@ -340,7 +340,9 @@ struct Request {
 };
 
 // The workspace: kMaxBlocks partials and one shadow table per launch.
-size_t launches_for(int64_t n) { return static_cast<size_t>(n <= kMaxTensors ? 1 : (n + kMaxTensors - 1) / kMaxTensors); }
+size_t launches_for(int64_t n) {
+  return static_cast<size_t>(n <= kMaxTensors ? 1 : (n + kMaxTensors - 1) / kMaxTensors);
+}
 size_t partial_bytes(int64_t n) { return round_up(sizeof(double) * kMaxBlocks * launches_for(n), 256); }
 size_t workspace_bytes(int64_t n) {
   const size_t launches = launches_for(n);

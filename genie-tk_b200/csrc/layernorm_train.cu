@@ -331,7 +331,8 @@ template <typename T, int V, bool kPlain, bool kEdge>
 struct Rows {
   T* at;         // kPlain: of the next visit asked for
   int64_t step;  // elements from a visit of the group to its next
-  __device__ __forceinline__ Rows(T* base, const RowMap& m, uint32_t first, uint32_t visits_apart, const Lay<kEdge>& l) {
+  __device__ __forceinline__ Rows(T* base, const RowMap& m, uint32_t first, uint32_t visits_apart,
+                                  const Lay<kEdge>& l) {
     at = base + (kPlain ? static_cast<int64_t>(first) * l.D : 0) - l.lead() + l.lane * V;
     step = static_cast<int64_t>(visits_apart) * l.D;
   }
@@ -367,7 +368,8 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads)
   const uint32_t first = kBlock ? block_first : block_first + threadIdx.x / G;
   const uint32_t step = gridDim.x * per_block;
   const int lead = kEdge ? static_cast<int>(first * static_cast<uint32_t>(D) & (V - 1)) : 0;
-  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))),
+               kBlock ? static_cast<int>(blockDim.x) : G,
                (lead + D + V - 1) / V, lead, D};
   const bool full = l.nv >= l.G * K;  // every vector of the thread exists
   const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch, stage_bytes = N * row_bytes;
@@ -482,7 +484,8 @@ __global__ void __launch_bounds__(kBlock ? kMaxBlockGroup : kGroupThreads, kBloc
   const uint32_t first = kBlock ? block_first : block_first + threadIdx.x / G;
   const uint32_t step = gridDim.x * per_block;
   const int lead = kEdge ? static_cast<int>(first * static_cast<uint32_t>(D) & (V - 1)) : 0;
-  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))), kBlock ? static_cast<int>(blockDim.x) : G,
+  const L l = {static_cast<int>(kBlock ? threadIdx.x : (threadIdx.x & (G - 1))),
+               kBlock ? static_cast<int>(blockDim.x) : G,
                (lead + D + V - 1) / V, lead, D};
   const int pitch = blockDim.x * R::kBytes, row_bytes = K * pitch;
   const int share = kBlock ? 32 : G;  // threads that share a copy of the statistics
@@ -703,7 +706,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     constexpr int kStep = kWarps * kRows;  // a multiple of V: all rows of a thread lie alike
     int i = warp * kRows + lane / kCols;
     const int64_t row = 2 * static_cast<int64_t>(ld), apart = kStep * row;
-    const float* p = partial + c + (second ? ld : 0) + i * row + (static_cast<uint32_t>(i) * static_cast<uint32_t>(D) & shift);
+    const float* p =
+        partial + c + (second ? ld : 0) + i * row + (static_cast<uint32_t>(i) * static_cast<uint32_t>(D) & shift);
     for (; i + 3 * kStep < n; i += 4 * kStep, p += 4 * apart) s += (p[0] + p[apart]) + (p[2 * apart] + p[3 * apart]);
     for (; i < n; i += kStep, p += apart) s += *p;
   }
@@ -720,7 +724,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
-// ---- Rows of more than 16384 elements (a vector less where none divides the width) -----------------------------------------------------
+// ---- Rows of more than 16384 elements (a vector less where none divides the width) -----------------
 
 template <typename T, typename W>
 __global__ void __launch_bounds__(kMaxBlockGroup)
@@ -908,7 +912,8 @@ int run_forward(const Args& a, const Shape& s) {
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
-  if (R::kAsync && cap > static_cast<int64_t>(num_sms()) * ring.blocks) cap = static_cast<int64_t>(num_sms()) * ring.blocks;
+  const int64_t in_flight = static_cast<int64_t>(num_sms()) * ring.blocks;
+  if (R::kAsync && cap > in_flight) cap = in_flight;
   const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);
   return launch("layernorm forward", kernel, blocks, threads, ring.bytes, a.st, false, static_cast<const T*>(a.x),
                 a.xm, a.order, static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean,
@@ -939,7 +944,8 @@ int run_backward(const Args& a, const Shape& s) {
   if (int e = ensure_smem(reinterpret_cast<const void*>(kernel), kRingBytes)) return e;
   static std::atomic<int64_t> cache[kBlockSizes];
   int64_t cap = cached_residency(cache, kernel, threads, ring.bytes);
-  if (R::kAsync && cap > static_cast<int64_t>(num_sms()) * ring.blocks) cap = static_cast<int64_t>(num_sms()) * ring.blocks;
+  const int64_t in_flight = static_cast<int64_t>(num_sms()) * ring.blocks;
+  if (R::kAsync && cap > in_flight) cap = in_flight;
   const int64_t most = max_partials(a.rows, a.D);
   if (cap > most) cap = most;
   const int64_t blocks = grid_for(a.order.visits, kBlock ? 1 : kGroupThreads / s.G, N, cap, kEdge);

@@ -336,7 +336,8 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
       if (clip && !t->is_inference()) t->bump_version();
       if (!plain && !t->is_non_overlapping_and_dense()) {
         if (clip && at::has_internal_overlap(t) == at::MemOverlap::Yes)
-          value_error("grads[" + std::to_string(i) + "] holds an element more than once and cannot be clipped in place");
+          value_error("grads[" + std::to_string(i) +
+                      "] holds an element more than once and cannot be clipped in place");
         g->keep.push_back(handle(t).contiguous());
         if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
         t = g->keep.back().unsafeGetTensorImpl();

@@ -131,7 +131,8 @@ class LayerNormFn(torch.autograd.Function):
         return dx, dw, db, None
 
 
-def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = LN_EPS) -> Tensor:
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = LN_EPS) -> Tensor:
     """Differentiable LayerNorm over the last axis on the library's kernels: x [*, D] fp32, bf16
     or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable."""
     if weight is None and bias is not None:
