@@ -240,6 +240,7 @@ py::tuple layernorm_backward(const Tensor& dy_in, const Tensor& x_in, const OptT
 // ---- The global gradient norm -----------------------------------------------------------------
 
 struct Gradients {
+  py::object list, out_list;  // hold the items until the call has been queued (a sequence may have made them for it)
   std::vector<const void*> in;
   std::vector<void*> out;
   std::vector<int64_t> numel;
@@ -281,18 +282,17 @@ void prefetch(PyObject** items, Py_ssize_t i, Py_ssize_t n) {
 
 // Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
 c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip, Gradients* g) {
-  py::object fast = py::reinterpret_steal<py::object>(PySequence_Fast(grads.ptr(), "grads must be a sequence"));
-  if (!fast) throw py::error_already_set();
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
+  g->list = py::reinterpret_steal<py::object>(PySequence_Fast(grads.ptr(), "grads must be a sequence"));
+  if (!g->list) throw py::error_already_set();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(g->list.ptr());
   if (n == 0) value_error("the list of gradients is empty");
-  PyObject** items = PySequence_Fast_ITEMS(fast.ptr());
-  py::object fast_out;
+  PyObject** items = PySequence_Fast_ITEMS(g->list.ptr());
   PyObject** out_items = nullptr;
   if (outs) {
-    fast_out = py::reinterpret_steal<py::object>(PySequence_Fast(outs->ptr(), "out must be a sequence"));
-    if (!fast_out) throw py::error_already_set();
-    if (PySequence_Fast_GET_SIZE(fast_out.ptr()) != n) value_error("out must have one tensor for each gradient");
-    out_items = PySequence_Fast_ITEMS(fast_out.ptr());
+    g->out_list = py::reinterpret_steal<py::object>(PySequence_Fast(outs->ptr(), "out must be a sequence"));
+    if (!g->out_list) throw py::error_already_set();
+    if (PySequence_Fast_GET_SIZE(g->out_list.ptr()) != n) value_error("out must have one tensor for each gradient");
+    out_items = PySequence_Fast_ITEMS(g->out_list.ptr());
   }
   g->in.resize(n);
   g->numel.resize(n);
