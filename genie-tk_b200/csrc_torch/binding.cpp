@@ -14,8 +14,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
+#include <numeric>
 #include <optional>
 #include <string>
 #include <vector>
@@ -280,6 +282,101 @@ void prefetch(PyObject** items, Py_ssize_t i, Py_ssize_t n) {
   }
 }
 
+// The memory that a strided tensor stands for: runs of `run` bytes, at every combination of the axes'
+// steps. The axes' strides ascend.
+struct Memory {
+  struct Axis {
+    int64_t size, stride;  // in bytes
+  };
+  int64_t at, run;
+  std::vector<Axis> axes;
+  std::vector<int64_t> span;  // [k]: bytes that the first k axes reach over
+  Py_ssize_t index;           // in its list
+  bool output;
+  int64_t end() const { return at + span.back(); }
+};
+
+Memory memory_of(const c10::TensorImpl* t, Py_ssize_t index, bool output) {
+  const int64_t bytes = static_cast<int64_t>(t->itemsize());
+  Memory m{reinterpret_cast<int64_t>(t->data()), bytes, {}, {}, index, output};
+  std::vector<Memory::Axis> axes;
+  for (int64_t i = 0; i < t->dim(); ++i)
+    if (t->size(i) != 1 && t->stride(i) != 0) axes.push_back({t->size(i), t->stride(i) * bytes});
+  std::sort(axes.begin(), axes.end(), [](auto& a, auto& b) { return a.stride < b.stride; });
+  for (const auto& a : axes) {
+    if (m.axes.empty() && a.stride == m.run)
+      m.run *= a.size;
+    else if (!m.axes.empty() && a.stride == m.axes.back().stride * m.axes.back().size)
+      m.axes.back().size *= a.size;
+    else
+      m.axes.push_back(a);
+  }
+  m.span.push_back(m.run);
+  for (const auto& a : m.axes) m.span.push_back(m.span.back() + (a.size - 1) * a.stride);
+  return m;
+}
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether the first ka axes of `a`, from address `at_a` on, share a byte with the first kb axes of `b`.
+// `steps` bounds the work; without an answer by then, yes.
+bool meet(const Memory& a, int64_t at_a, size_t ka, const Memory& b, int64_t at_b, size_t kb, int64_t* steps) {
+  if (at_a + a.span[ka] <= at_b || at_b + b.span[kb] <= at_a) return false;
+  if (ka == 0 && kb == 0) return true;
+  if (--*steps < 0) return true;
+  // all runs begin at at_a or at_b plus multiples of g (columns of one matrix: its rows): the runs of
+  // the one lie in the gaps of the other, or may meet
+  int64_t g = 0;
+  for (size_t k = 0; k < ka; ++k) g = std::gcd(g, a.axes[k].stride);
+  for (size_t k = 0; k < kb; ++k) g = std::gcd(g, b.axes[k].stride);
+  const int64_t r = (at_b - at_a) - floor_div(at_b - at_a, g) * g;
+  if (r >= a.run && r + b.run <= g) return false;
+  // the parts of the wider one that reach into the other
+  if (ka == 0 || (kb && b.span[kb] > a.span[ka])) return meet(b, at_b, kb, a, at_a, ka, steps);
+  const auto& axis = a.axes[ka - 1];
+  const int64_t first = std::max<int64_t>(0, floor_div(at_b - at_a - a.span[ka - 1], axis.stride) + 1);
+  const int64_t last = std::min(axis.size - 1, floor_div(at_b + b.span[kb] - at_a - 1, axis.stride));
+  for (int64_t i = first; i <= last; ++i)
+    if (meet(a, at_a + i * axis.stride, ka - 1, b, at_b, kb, steps)) return true;
+  return false;
+}
+
+constexpr int64_t kMeetSteps = int64_t(1) << 20;  // of a call: some 10 ms
+
+// Whether a tensor (without strides of zero) holds an element of memory more than once.
+bool repeats(const Memory& m, int64_t* steps) {
+  for (size_t k = 0; k < m.axes.size(); ++k)
+    for (int64_t d = 1; d < m.axes[k].size && d * m.axes[k].stride < m.span[k]; ++d)
+      if (meet(m, m.at, k, m, m.at + d * m.axes[k].stride, k, steps)) return true;
+  return false;
+}
+
+// Refuses overlaps that the library cannot see, as it gets copies of the strided gradients: in place, of
+// any two gradients; with outputs, of a `copied` gradient and any output.
+void check_memory(PyObject** items, PyObject** out_items, Py_ssize_t n, const std::vector<Py_ssize_t>& copied,
+                  int64_t* steps) {
+  std::vector<Memory> all;
+  auto add = [&](c10::TensorImpl* t, Py_ssize_t i, bool output) {
+    if (t->numel()) all.push_back(memory_of(t, i, output));
+  };
+  if (out_items) {
+    for (Py_ssize_t i : copied) add(tensor_at(items[i], "grads", i), i, false);
+    for (Py_ssize_t i = 0; i < n; ++i) add(tensor_at(out_items[i], "out", i), i, true);
+  } else {
+    for (Py_ssize_t i = 0; i < n; ++i) add(tensor_at(items[i], "grads", i), i, false);
+  }
+  std::sort(all.begin(), all.end(), [](auto& a, auto& b) { return a.at < b.at; });
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t j = i + 1; j < all.size() && all[j].at < all[i].end(); ++j) {
+      const Memory &a = all[i], &b = all[j];
+      if (out_items && a.output == b.output) continue;
+      if (meet(a, a.at, a.axes.size(), b, b.at, b.axes.size(), steps))
+        throw std::runtime_error(kPrefix + (a.output ? "out[" : "grads[") + std::to_string(a.index) + "] and " +
+                                 (b.output ? "out[" : "grads[") + std::to_string(b.index) +
+                                 "] overlap (the same tensor twice?)");
+    }
+}
+
 // Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
 c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip, Gradients* g) {
   g->list = py::reinterpret_steal<py::object>(PySequence_Fast(grads.ptr(), "grads must be a sequence"));
@@ -303,6 +400,8 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
   }
   require_cuda(handle(tensor_at(items[0], "grads", 0)), "grads[0]");
   const c10::Device device = tensor_at(items[0], "grads", 0)->device();
+  std::vector<Py_ssize_t> copied;
+  int64_t steps = kMeetSteps;
   for (Py_ssize_t i = 0; i < n; ++i) {
     prefetch(items, i, n);
     c10::TensorImpl* t = tensor_at(items[i], "grads", i);
@@ -326,6 +425,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
                          (t->is_non_overlapping_and_dense() && t->strides() == o->strides());
       if (!alike) {
         if (!o->is_contiguous()) value_error("out[" + std::to_string(i) + "] must be contiguous");
+        copied.push_back(i);
         g->keep.push_back(handle(t).contiguous());
         t = g->keep.back().unsafeGetTensorImpl();
       }
@@ -335,9 +435,11 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     } else {
       if (clip && !t->is_inference()) t->bump_version();
       if (!plain && !t->is_non_overlapping_and_dense()) {
-        if (clip && at::has_internal_overlap(t) == at::MemOverlap::Yes)
+        if (clip && t->numel() &&
+            (at::has_internal_overlap(t) == at::MemOverlap::Yes || repeats(memory_of(t, i, false), &steps)))
           value_error("grads[" + std::to_string(i) +
                       "] holds an element more than once and cannot be clipped in place");
+        copied.push_back(i);
         g->keep.push_back(handle(t).contiguous());
         if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
         t = g->keep.back().unsafeGetTensorImpl();
@@ -347,6 +449,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     g->numel[i] = t->numel();
     g->in_type[i] = code;
   }
+  if (clip && !copied.empty()) check_memory(items, out_items, n, copied, &steps);
   return device;
 }
 
