@@ -247,6 +247,7 @@ struct Gradients {
   std::vector<void*> out;
   std::vector<int64_t> numel;
   std::vector<int> in_type, out_type;
+  std::vector<c10::TensorImpl*> written;              // by the library, once the call has succeeded
   std::vector<Tensor> keep;                           // copies of strided gradients
   std::vector<std::pair<Tensor, Tensor>> write_back;  // (gradient, its clipped copy)
 };
@@ -394,6 +395,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
   g->in.resize(n);
   g->numel.resize(n);
   g->in_type.resize(n);
+  if (clip) g->written.resize(n);
   if (outs) {
     g->out.resize(n);
     g->out_type.resize(n);
@@ -431,9 +433,9 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
       }
       g->out[i] = o->mutable_data();
       g->out_type[i] = code_of(ot);
-      if (!o->is_inference()) o->bump_version();
+      g->written[i] = o;
     } else {
-      if (clip && !t->is_inference()) t->bump_version();
+      if (clip) g->written[i] = t;
       if (!plain && !t->is_non_overlapping_and_dense()) {
         if (clip && t->numel() &&
             (at::has_internal_overlap(t) == at::MemOverlap::Yes || repeats(memory_of(t, i, false), &steps)))
@@ -441,7 +443,10 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
                       "] holds an element more than once and cannot be clipped in place");
         copied.push_back(i);
         g->keep.push_back(handle(t).contiguous());
-        if (clip) g->write_back.emplace_back(handle(t), g->keep.back());
+        if (clip) {
+          g->write_back.emplace_back(handle(t), g->keep.back());
+          g->written[i] = nullptr;  // `copy_` counts its version
+        }
         t = g->keep.back().unsafeGetTensorImpl();
       }
     }
@@ -489,6 +494,8 @@ Tensor clip_grad_norm(const py::sequence& grads, double max_norm, double norm_ty
                            in_place ? nullptr : g.out_type.data(), g.in.size(), kind, max_norm,
                            static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes, stream_of(device)),
         "gtk_clip_grad_norm");
+  for (c10::TensorImpl* t : g.written)
+    if (t && !t->is_inference()) t->bump_version();
   for (auto& p : g.write_back) p.first.copy_(p.second);
   return norm;
 }

@@ -91,6 +91,35 @@ def test_many_columns_of_one_buffer():
         ops.clip_grad_norm([a[:, c] for c in range(300)] + [a[2999, 299:]], 3.0)
 
 
+def test_refused_calls_leave_the_versions():
+    """A refused call has written nothing, and autograd must not think that it had."""
+    dev = require_gpu()
+    from genie_tk import ops
+    g = [torch.randn(6, 5, device=dev) for _ in range(3)]
+    o = [torch.empty(6, 5, device=dev) for _ in range(3)]
+    s = torch.randn(6, 10, device=dev)
+    before = [t._version for t in g + o + [s]]
+    calls = [lambda: ops.clip_grad_norm([g[0], s[:, ::2], g[1].double()], 1.0), lambda: ops.clip_grad_norm([g[0], g[0]], 1.0),
+             lambda: ops.clip_grad_norm([g[0], 1.0], 1.0), lambda: ops.clip_grad_norm(g[:2], 1.0, out=[o[0], o[1].half()]),
+             lambda: ops.clip_grad_norm(g[:2], 1.0, out=[o[0], o[0]]), lambda: ops.clip_grad_norm(g[:2], 1.0, out=[o[0], s[:, ::2]])]
+    for call in calls:
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            call()
+        assert [t._version for t in g + o + [s]] == before
+    ops.clip_grad_norm(g[:2] + [s[:, ::2]], 1.0)
+    assert all(t._version > v for t, v in zip(g[:2] + [s], before[:2] + before[-1:])) and g[2]._version == before[2]
+    ops.clip_grad_norm(g, 1.0, out=o)
+    assert all(t._version > v for t, v in zip(o, before[3:])) and g[2]._version == before[2]
+    # the same through autograd: a saved tensor that a refused call named is as it was
+    x = torch.randn(7, device=dev, requires_grad=True)
+    y = x.detach().clone()
+    loss = (x * y).sum()
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.clip_grad_norm([y, y], 1.0)
+    loss.backward()
+    assert torch.equal(x.grad, y)
+
+
 class _Made:
     """A sequence that makes each item when it is asked for and keeps none."""
 
