@@ -378,8 +378,11 @@ void check_memory(PyObject** items, PyObject** out_items, Py_ssize_t n, const st
     }
 }
 
-// Checks the lists and fills the arrays. `outs` NULL: in place (`clip`) or the norm alone.
-c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip, Gradients* g) {
+// Checks the lists, fills the arrays and makes the gradients' device current. `outs` NULL: in place
+// (`clip`) or the norm alone. What will be written is asked for as mutable, so that a lazy clone gets
+// memory of its own.
+c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip, Gradients* g,
+                    c10::cuda::OptionalCUDAGuard* guard) {
   g->list = py::reinterpret_steal<py::object>(PySequence_Fast(grads.ptr(), "grads must be a sequence"));
   if (!g->list) throw py::error_already_set();
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(g->list.ptr());
@@ -402,6 +405,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
   }
   require_cuda(handle(tensor_at(items[0], "grads", 0)), "grads[0]");
   const c10::Device device = tensor_at(items[0], "grads", 0)->device();
+  guard->set_device(device);
   std::vector<Py_ssize_t> copied;
   int64_t steps = kMeetSteps;
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -450,7 +454,7 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
         t = g->keep.back().unsafeGetTensorImpl();
       }
     }
-    g->in[i] = t->data();
+    g->in[i] = clip && !outs ? t->mutable_data() : t->data();
     g->numel[i] = t->numel();
     g->in_type[i] = code;
   }
@@ -468,8 +472,8 @@ Tensor grad_norm(const py::sequence& grads, double norm_type) {
   const int kind = norm_kind(norm_type);
   at::NoGradGuard no_grad;
   Gradients g;
-  const c10::Device device = collect(grads, nullptr, false, &g);
-  c10::cuda::CUDAGuard guard(device);
+  c10::cuda::OptionalCUDAGuard guard;
+  const c10::Device device = collect(grads, nullptr, false, &g, &guard);
   Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
   const size_t bytes = api.grad_norm_workspace_bytes(g.in.size());
   Tensor ws = scratch(bytes, norm);
@@ -485,8 +489,8 @@ Tensor clip_grad_norm(const py::sequence& grads, double max_norm, double norm_ty
   at::NoGradGuard no_grad;
   Gradients g;
   const bool in_place = out.is_none();
-  const c10::Device device = collect(grads, in_place ? nullptr : &out, true, &g);
-  c10::cuda::CUDAGuard guard(device);
+  c10::cuda::OptionalCUDAGuard guard;
+  const c10::Device device = collect(grads, in_place ? nullptr : &out, true, &g, &guard);
   Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
   const size_t bytes = api.grad_norm_workspace_bytes(g.in.size());
   Tensor ws = scratch(bytes, norm);

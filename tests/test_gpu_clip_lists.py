@@ -153,6 +153,20 @@ def test_sequences_that_make_their_items(n):
         assert abs(float(ops.grad_norm(_Made(grads))) - total) <= 10 * U * total
 
 
+def test_copies_on_write():
+    """Clipping a lazy clone leaves its source, and two lazy clones are two tensors."""
+    dev = require_gpu()
+    from genie_tk import ops
+    src = torch.randn(1000, device=dev)
+    kept = src.clone()
+    a, b = torch._lazy_clone(src), torch._lazy_clone(src)
+    n = _norm([a, b])
+    ops.clip_grad_norm([a, b], 0.5 * n)
+    assert torch.equal(src, kept)
+    for t in (a, b):
+        _check_scaled(t, kept, 0.5 * n / (n + 1e-6))
+
+
 def test_random_views_against_their_elements():
     """Random views of one buffer: refused exactly where two share an element, or one holds an element
     twice."""
