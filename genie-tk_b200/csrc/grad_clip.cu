@@ -285,6 +285,17 @@ __device__ __forceinline__ void scale_chunk(const void* in, void* out, int64_t o
   }
 }
 
+// The same by element in 64 bits, for factors that fp32 has few bits of or none (below 2^-126, where
+// the norm is near fp32's largest or above it).
+template <typename T, typename O>
+__device__ __forceinline__ void scale_wide(const void* in, void* out, int64_t off, int n, double q) {
+  const T* p = static_cast<const T*>(in) + off;
+  O* o = static_cast<O*>(out) + off;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    o[i] = Elem<O>::store(static_cast<float>(static_cast<double>(Elem<T>::load(p[i])) * q));
+}
+
 template <int kPer>
 __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoarseBlocks)
     clip_scale_kernel(const Shadow* __restrict__ shadow, int tensors, uint32_t chunks,
@@ -300,6 +311,25 @@ __global__ void __launch_bounds__(kThreads, kPer == kFine ? kFineBlocks : kCoars
   const float k = static_cast<float>(q < 1.0 || isnan(q) ? q : 1.0);
   if (in_place && k == 1.f) return;
   constexpr int kChunk = kThreads * kPer;
+  if (q > 0.0 && q < 0x1p-126) {
+#pragma unroll 1
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+      const int t = find([&](int i) { return first[i]; }, tensors, c);
+      const Tensor e = shadow->t[t];
+      const Span sp = span_of(e, c - first[t], c + 1 == first[t + 1], kChunk);
+      if (e.in_type == GTK_F32)
+        scale_wide<float, float>(e.in, e.out, sp.off, sp.n, q);
+      else if (e.in_type == GTK_BF16 && e.out_type == GTK_BF16)
+        scale_wide<__nv_bfloat16, __nv_bfloat16>(e.in, e.out, sp.off, sp.n, q);
+      else if (e.in_type == GTK_BF16)
+        scale_wide<__nv_bfloat16, float>(e.in, e.out, sp.off, sp.n, q);
+      else if (e.out_type == GTK_F16)
+        scale_wide<__half, __half>(e.in, e.out, sp.off, sp.n, q);
+      else
+        scale_wide<__half, float>(e.in, e.out, sp.off, sp.n, q);
+    }
+    return;
+  }
 #pragma unroll 1
   for (uint32_t back = blockIdx.x; back < chunks; back += gridDim.x) {
     const uint32_t c = chunks - 1 - back;

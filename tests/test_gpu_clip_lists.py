@@ -167,6 +167,29 @@ def test_copies_on_write():
         _check_scaled(t, kept, 0.5 * n / (n + 1e-6))
 
 
+@pytest.mark.parametrize("out", [None, torch.float32, "same"])
+@pytest.mark.parametrize("n", [1003, 2100007])
+def test_factors_below_the_fp32_range(n, out):
+    """Values near fp32's largest under a small limit: the factor is below 2^-126, where fp32 has
+    fewer bits, or below 2^-150, where it has none; the scaled values are ordinary numbers."""
+    dev = require_gpu()
+    from genie_tk import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        for limit in (1e3, 1e-1, 1e-5):
+            gen = torch.Generator(device=dev).manual_seed(n)
+            g = ((torch.rand(n, generator=gen, device=dev) + 1) * 1.2e38).to(dtype)[1:]
+            kept = g.clone()
+            norm = _norm([g])
+            if out is None:
+                ops.clip_grad_norm([g], limit)
+                got = g
+            else:
+                got = torch.empty(n - 1, device=dev, dtype=dtype if out == "same" else out)
+                ops.clip_grad_norm([g], limit, out=[got])
+                assert torch.equal(g, kept)
+            _check_scaled(got, kept, limit / norm)
+
+
 def test_random_views_against_their_elements():
     """Random views of one buffer: refused exactly where two share an element, or one holds an element
     twice."""
