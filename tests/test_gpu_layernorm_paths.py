@@ -1,0 +1,53 @@
+"""GPU tests of the LayerNorm kernels that few calls reach: rows of more than 16384 elements in
+numbers, rows that begin anywhere (element by element), and the statistics' shape.
+
+Tolerances as in test_gpu_layernorm_train.py, unless a test says its own."""
+
+import pytest
+import torch
+
+import genie_tk
+from gpu_util import require_gpu
+from test_gpu_layernorm_train import DT, U, _inputs, _run_and_check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(130, 16379), (130, 20000), (700, 16379), (700, 20000), (65, 40001)])
+def test_wide_rows_in_numbers(rows, D, dtype):
+    """More rows than the partial sums have slabs, and than four to an SM."""
+    dev = require_gpu()
+    _run_and_check(*_inputs((rows, D), DT[dtype], torch.float32, rows + D, dev))
+
+
+@pytest.mark.parametrize("B,N,D", [(1, 9, 16379), (2, 11, 20000)])
+def test_wide_rows_transposed(B, N, D):
+    dev = require_gpu()
+    x, dy, w, b = _inputs((B, N, N, D), torch.bfloat16, torch.float32, N, dev)
+    _run_and_check(x.transpose(1, 2), dy.transpose(1, 2), w, b)
+    _run_and_check(x, dy.transpose(1, 2), w, b)
+
+
+def test_wide_rows_sum_their_columns_in_short_chains():
+    """dw and db of many wide rows: a value of 1 in each 256 rows and 255 that half a step of 1 is
+    more than (one after another onto it, they are all lost: 254 u of the sum). Sixteen rows are
+    added in fp32 (15 u), the sixteens in 64 bits, stored (u), and 64 such sums are joined (four to a
+    thread, two shuffles, five over the warps: 10 u): 32 u."""
+    dev = require_gpu()
+    from genie_tk import ops
+    rows, D = 16384, 16385
+    small = 2.0 ** -24 * (1 - 2.0 ** -8)
+    column = torch.full((rows, 1), small, dtype=torch.float64, device=dev)
+    column[::256] = 1.0
+    dy = column.to(torch.bfloat16).expand(rows, D).contiguous()
+    assert torch.equal(dy[:, :1].double(), column)
+    x = torch.ones(rows, D, dtype=torch.bfloat16, device=dev)
+    x[:, 1::2] = -1.0
+    mean, rstd = torch.zeros(rows, device=dev), torch.ones(rows, device=dev)
+    w = torch.ones(D, device=dev)
+    _, dw, db = ops.layernorm_backward(dy, x, w, mean, rstd)
+    want = float(column.sum())
+    sign = x[0].double()
+    assert float((db.double() - want).abs().max()) <= 32 * U * want
+    assert float((dw.double() * sign - want).abs().max()) <= 32 * U * want
