@@ -198,6 +198,14 @@ py::tuple layernorm_forward(const Tensor& x_in, const OptTensor& weight, const O
   return py::make_tuple(std::move(y), std::move(mean), std::move(rstd));
 }
 
+// Whether t has x's leading axes (and perhaps a last one of one), or all rows in one axis.
+bool one_per_row(const Tensor& t, const Tensor& x) {
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const bool keepdim = t.dim() == x.dim() && t.size(-1) == 1;
+  return (keepdim ? t.sizes().slice(0, x.dim() - 1) : t.sizes()) == lead ||
+         (t.dim() == 1 && t.numel() == c10::multiply_integers(lead));
+}
+
 py::tuple layernorm_backward(const Tensor& dy_in, const Tensor& x_in, const OptTensor& weight, const Tensor& mean_in,
                              const Tensor& rstd_in, bool need_weight, bool need_bias) {
   require_cuda(x_in, "x");
@@ -209,8 +217,9 @@ py::tuple layernorm_backward(const Tensor& dy_in, const Tensor& x_in, const OptT
     value_error("dy must have x's shape and type, got " + shape_of(dy_in) + " " + name_of(dy_in.scalar_type()));
   if (x_in.dim() < 1 || x_in.size(-1) < 1) value_error("x must have a last axis of at least one element");
   const int64_t D = x_in.size(-1), n = mean_in.numel();
-  if (n * D != x_in.numel() || rstd_in.numel() != n)
-    value_error("mean and rstd must have one element for each row of x");
+  if (n * D != x_in.numel() || !one_per_row(mean_in, x_in) || !one_per_row(rstd_in, x_in))
+    value_error("mean and rstd must have one element for each row of x, in x's leading axes or in one, got " +
+                shape_of(mean_in) + " and " + shape_of(rstd_in));
   if (mean_in.scalar_type() != at::kFloat || rstd_in.scalar_type() != at::kFloat)
     type_error("mean and rstd must be float32");
   at::NoGradGuard no_grad;

@@ -621,9 +621,10 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
                        rstd: torch.Tensor, need_weight: bool = True, need_bias: bool = True):
     """(dx, dweight, dbias) of ``layernorm_forward`` for the output gradient ``dy``.
 
-    dy has x's shape and type; mean and rstd are the forward's. dx is contiguous. The
-    parameters' gradients have ``weight``'s type (x's without a weight); one that is not
-    needed is None. The same inputs give the same bits."""
+    dy has x's shape and type; mean and rstd are the forward's, in x's leading axes or as one axis of
+    its rows (of a transposed x: transposed too). dx is contiguous. The parameters' gradients have
+    ``weight``'s type (x's without a weight); one that is not needed is None. The same inputs give the
+    same bits."""
     return _lib.native().layernorm_backward(dy, x, weight, mean, rstd, need_weight, need_bias)
 
 

@@ -51,3 +51,27 @@ def test_wide_rows_sum_their_columns_in_short_chains():
     sign = x[0].double()
     assert float((db.double() - want).abs().max()) <= 32 * U * want
     assert float((dw.double() * sign - want).abs().max()) <= 32 * U * want
+
+
+def test_statistics_lie_as_the_rows_do():
+    """mean and rstd have one element for each row in x's own axes (or in one axis, or with a last
+    axis of one): statistics of the transposed tensor are refused, not read in another order."""
+    dev = require_gpu()
+    from genie_tk import ops
+    x, dy, w, b = _inputs((3, 5, 7, 24), torch.float32, torch.float32, 1, dev)
+    y, mean, rstd = ops.layernorm_forward(x, w, b)
+    want = ops.layernorm_backward(dy, x, w, mean, rstd)
+    for m, r in ((mean.reshape(-1), rstd.reshape(-1)), (mean.unsqueeze(-1), rstd.unsqueeze(-1)), (mean, rstd.reshape(-1))):
+        assert all(torch.equal(p, q) for p, q in zip(ops.layernorm_backward(dy, x, w, m, r), want))
+    xt, dyt = x.transpose(1, 2), dy.transpose(1, 2)
+    with pytest.raises(ValueError, match="one element for each row"):
+        ops.layernorm_backward(dyt, xt, w, mean, rstd)
+    with pytest.raises(ValueError, match="one element for each row"):
+        ops.layernorm_backward(dyt, xt, w, mean.transpose(1, 2), rstd)
+    got = ops.layernorm_backward(dyt, xt, w, mean.transpose(1, 2), rstd.transpose(1, 2))
+    torch.testing.assert_close(got[0], want[0].transpose(1, 2), rtol=0, atol=0)
+    with pytest.raises(ValueError, match="one element for each row"):
+        ops.layernorm_backward(dy, x, w, mean.reshape(15, 7), rstd)
+    one = torch.randn(24, device=dev)
+    _, m, r = ops.layernorm_forward(one, w, b)
+    assert m.dim() == 0 and ops.layernorm_backward(one, one, w, m, r)[0].shape == (24,)
