@@ -11,6 +11,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -97,6 +98,25 @@ int dtype_code(const Tensor& t, const char* name) {
   return c;
 }
 
+// The operators have no forward-mode formula: a tangent that they would lose is an error. Tensors have
+// tangents while a level of forward mode is open only.
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+
+void refuse_tangent(const Tensor& t, const char* name) {
+  if (!t.defined() || !t._fw_grad(0).defined()) return;
+  PyErr_SetString(PyExc_NotImplementedError,
+                  (kPrefix + name + " has a tangent, and this operator no forward-mode derivative").c_str());
+  throw py::error_already_set();
+}
+
+void refuse_tangents(std::initializer_list<std::pair<const Tensor*, const char*>> tensors) {
+  if (!forward_mode()) return;
+  for (const auto& t : tensors)
+    if (t.first) refuse_tangent(*t.first, t.second);
+}
+
+const Tensor* given(const OptTensor& t) { return t ? &*t : nullptr; }
+
 void require_cuda(const Tensor& t, const char* name) {
   if (!t.is_cuda())
     throw std::runtime_error(kPrefix + name + " must be a CUDA tensor; this package has no CPU path");
@@ -175,6 +195,7 @@ py::tuple layernorm_forward(const Tensor& x_in, const OptTensor& weight, const O
   require_cuda(x_in, "x");
   if (x_in.dim() < 1 || x_in.size(-1) < 1) value_error("x must have a last axis of at least one element");
   const int xt = dtype_code(x_in, "x");
+  refuse_tangents({{&x_in, "x"}, {given(weight), "weight"}, {given(bias), "bias"}});
   at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(x_in.device());
   int wt = -1;
@@ -222,6 +243,7 @@ py::tuple layernorm_backward(const Tensor& dy_in, const Tensor& x_in, const OptT
                 shape_of(mean_in) + " and " + shape_of(rstd_in));
   if (mean_in.scalar_type() != at::kFloat || rstd_in.scalar_type() != at::kFloat)
     type_error("mean and rstd must be float32");
+  refuse_tangents({{&dy_in, "dy"}, {&x_in, "x"}, {given(weight), "weight"}, {&mean_in, "mean"}, {&rstd_in, "rstd"}});
   at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(x_in.device());
   int wt = -1;
@@ -489,6 +511,11 @@ c10::Device collect(const py::sequence& grads, const py::object* outs, bool clip
     throw;
   }
   if (clip) g->n_counted = n;
+  if (forward_mode())
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      refuse_tangent(THPVariable_Unpack(items[k]), "a gradient");
+      if (outs) refuse_tangent(THPVariable_Unpack(out_items[k]), "an output");
+    }
   if (clip && !copied.empty()) check_memory(items, out_items, n, copied, &steps);
   return device;
 }
@@ -549,6 +576,7 @@ Tensor embedding_forward(const Tensor& tokens_in, const Tensor& weight_in, doubl
   const int dt = dtype_code(weight_in, "weight");
   if (weight_in.dim() != 2 || weight_in.size(0) < 1)
     value_error("weight must be [vocabulary, width], got " + shape_of(weight_in));
+  refuse_tangents({{&weight_in, "weight"}});
   at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(weight_in.device());
   std::vector<int64_t> shape = tokens_in.sizes().vec();
@@ -578,6 +606,7 @@ Tensor embedding_backward(const Tensor& dy_in, const Tensor& tokens_in, int64_t 
     type_error("the table's gradient must be float32 or dy's type, got " + name_of(wd));
   if (padding && (*padding < 0 || *padding >= vocab))
     value_error("padding_idx must be a token of the vocabulary, got " + std::to_string(*padding));
+  refuse_tangents({{&dy_in, "dy"}});
   at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(dy_in.device());
   const int64_t D = dy_in.size(-1), n = tokens_in.numel();

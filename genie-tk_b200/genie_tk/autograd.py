@@ -134,7 +134,8 @@ class LayerNormFn(torch.autograd.Function):
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
                eps: float = LN_EPS) -> Tensor:
     """Differentiable LayerNorm over the last axis on the library's kernels: x [*, D] fp32, bf16
-    or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable."""
+    or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable, in reverse mode
+    (a forward-mode tangent raises)."""
     if weight is None and bias is not None:
         weight = torch.ones_like(bias)  # the parameters' gradients have the weight's type
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
@@ -162,8 +163,8 @@ class EmbeddingFn(torch.autograd.Function):
 
 def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
     """Differentiable scale * weight[tokens] on the library's kernels: tokens int32 or int64 [*],
-    weight [vocabulary, D]; the row ``padding_idx`` gets no gradient. Once differentiable; the
-    table's gradient is dense and the same from run to run."""
+    weight [vocabulary, D]; the row ``padding_idx`` gets no gradient. Once differentiable, in reverse
+    mode (a forward-mode tangent raises); the table's gradient is dense and the same from run to run."""
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"genie_tk (B200): padding_idx must be a token of the vocabulary, got {padding_idx}")
     if torch.is_grad_enabled() and weight.requires_grad:
