@@ -126,7 +126,8 @@ class LayerNormFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = ops.layernorm_backward(dy.to(x.dtype), x, weight, mean, rstd, ctx.needs_input_grad[1],
+        dy = dy.to(x.dtype).resolve_neg()
+        dx, dw, db = ops.layernorm_backward(dy, x, weight, mean, rstd, ctx.needs_input_grad[1],
                                             ctx.needs_input_grad[2])
         return dx, dw, db, None
 
@@ -158,7 +159,8 @@ class EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dy):
         tokens, = ctx.saved_tensors
         rows, dtype = ctx.table
-        return None, ops.embedding_backward(dy.to(dtype), tokens, rows, ctx.scale, ctx.padding_idx), None, None
+        dy = dy.to(dtype).resolve_neg()
+        return None, ops.embedding_backward(dy, tokens, rows, ctx.scale, ctx.padding_idx), None, None
 
 
 def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:

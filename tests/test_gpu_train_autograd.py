@@ -44,3 +44,20 @@ def test_tangents_are_refused_not_dropped():
         assert torch.equal(autograd.layer_norm(x, w.detach(), b), y)
         torch.autograd.grad(out, leaf, t)
     assert float(ops.grad_norm([t])) > 0
+
+
+def test_lazily_negated_output_gradients():
+    """A gradient that reaches the operators through a complex view may be a lazily negated one; torch's
+    own layer_norm and embedding take it."""
+    dev = require_gpu()
+    x, w, b = torch.randn(5, 24, device=dev), torch.randn(24, device=dev), torch.randn(24, device=dev)
+    table, tok = torch.randn(9, 24, device=dev), torch.tensor([1, 5, 8, 1], device=dev)
+    v = torch.randn(5, 24, device=dev)
+    neg = torch.complex(torch.zeros_like(v), v).conj().imag
+    assert neg.is_neg() and torch.equal(neg, -v)
+    for make, n in ((lambda t: autograd.layer_norm(t, w, b), x), (lambda t: autograd.embedding(tok, t), table)):
+        leaf = n.clone().requires_grad_(True)
+        out = make(leaf)
+        got, = torch.autograd.grad(out, leaf, neg[:out.shape[0]], retain_graph=True)
+        want, = torch.autograd.grad(out, leaf, -v[:out.shape[0]])
+        assert torch.equal(got, want)
