@@ -137,6 +137,8 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     """Differentiable LayerNorm over the last axis on the library's kernels: x [*, D] fp32, bf16
     or fp16, weight and bias [D] in fp32 or x's type (or None). Once differentiable, in reverse mode
     (a forward-mode tangent raises)."""
+    # the kernels' gradients have one axis
+    weight, bias = (t if t is None or t.dim() == 1 else t.reshape(-1) for t in (weight, bias))
     if weight is None and bias is not None:
         weight = torch.ones_like(bias)  # the parameters' gradients have the weight's type
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):

@@ -61,3 +61,20 @@ def test_lazily_negated_output_gradients():
         got, = torch.autograd.grad(out, leaf, neg[:out.shape[0]], retain_graph=True)
         want, = torch.autograd.grad(out, leaf, -v[:out.shape[0]])
         assert torch.equal(got, want)
+
+
+def test_parameters_with_an_axis_more():
+    """Weights of D elements in another shape: their gradients have that shape."""
+    dev = require_gpu()
+    x = torch.randn(5, 24, device=dev, requires_grad=True)
+    w, b = (torch.randn(24, device=dev) for _ in range(2))
+    v = torch.randn(5, 24, device=dev)
+    flat = [w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+    want = torch.autograd.grad((autograd.layer_norm(x, *flat) * v).sum(), [x, *flat])
+    for shape in ((1, 24), (24, 1), (2, 12)):
+        more = [t.view(shape).clone().requires_grad_(True) for t in (w, b)]
+        got = torch.autograd.grad((autograd.layer_norm(x, *more) * v).sum(), [x, *more])
+        assert got[1].shape == shape and got[2].shape == shape
+        assert all(torch.equal(p, q.view(p.shape)) for p, q in zip(got, want))
+        only, = torch.autograd.grad((autograd.layer_norm(x, None, more[1]) * v).sum(), more[1])
+        assert only.shape == shape and torch.equal(only.view(-1), want[2])
