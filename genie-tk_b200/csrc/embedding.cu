@@ -999,7 +999,7 @@ using namespace gtk;
 extern "C" {
 
 int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight, int dtype, void* y, int64_t n_tokens,
-                          int64_t vocab, int64_t D, float scale, uint32_t* status, void* stream) {
+                          int64_t vocab, int64_t D, float scale, uint32_t* status, void* stream) try {
   if (int e = emb::check_sizes(n_tokens, vocab, D)) return e;
   if (!dtype_ok(dtype)) return fail(GTK_ERR_UNSUPPORTED, "embedding: the table is fp32, bf16 or fp16");
   if (int e = emb::check_tokens(tokens, index_bits)) return e;
@@ -1011,6 +1011,8 @@ int gtk_embedding_forward(const void* tokens, int index_bits, const void* weight
   a.st = static_cast<cudaStream_t>(stream);
   return index_bits == 64 ? emb::forward_by_type<int64_t>(a, weight, y, dtype)
                           : emb::forward_by_type<int32_t>(a, weight, y, dtype);
+} catch (...) {
+  return fail_no_memory();
 }
 
 size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t D, int dy_dtype) {
@@ -1020,7 +1022,7 @@ size_t gtk_embedding_backward_workspace_bytes(int64_t n_tokens, int64_t vocab, i
 
 int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int index_bits, void* dweight,
                            int w_dtype, int64_t n_tokens, int64_t vocab, int64_t D, float scale, int64_t padding,
-                           void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
+                           void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) try {
   if (int e = emb::check_sizes(n_tokens, vocab, D)) return e;
   // every tile of the sort reads all tiles' counts: beyond this it would take longer than it is worth
   if (n_tokens > emb::kMaxSorted) return fail(GTK_ERR_UNSUPPORTED, "embedding: the gradient takes up to 2^27 tokens");
@@ -1049,6 +1051,8 @@ int gtk_embedding_backward(const void* dy, int dy_dtype, const void* tokens, int
                               : emb::backward_typed<__nv_bfloat16, __nv_bfloat16>(a, p, keys, pos);
   return w_dtype == GTK_F32 ? emb::backward_typed<__half, float>(a, p, keys, pos)
                             : emb::backward_typed<__half, __half>(a, p, keys, pos);
+} catch (...) {
+  return fail_no_memory();
 }
 
 }  // extern "C"

@@ -566,7 +566,7 @@ int gtk_grad_norm(const void* const* grads, const int64_t* numel, const int* dty
   return clip::start(grads, nullptr, numel, dtypes, nullptr, n_tensors, norm_kind, norm, workspace, workspace_bytes,
                      stream, &r);
 } catch (...) {
-  return fail(GTK_ERR_INVALID_ARG, "gradient norm: out of host memory");
+  return fail_no_memory();
 }
 
 int gtk_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* numel, const int* dtypes,
@@ -579,7 +579,7 @@ int gtk_clip_grad_norm(const void* const* grads, void* const* outs, const int64_
   return clip::start(grads, outs, numel, dtypes, out_dtypes, n_tensors, norm_kind, norm, workspace, workspace_bytes,
                      stream, &r);
 } catch (...) {
-  return fail(GTK_ERR_INVALID_ARG, "gradient clipping: out of host memory");
+  return fail_no_memory();
 }
 
 }  // extern "C"

@@ -10,11 +10,20 @@ namespace gtk {
 
 namespace {
 thread_local std::string g_last_error;
+thread_local const char* g_fixed_error = nullptr;  // in its place, where there was no memory for a string
 std::mutex g_mu;
 }  // namespace
 
-void set_error(const std::string& msg) { g_last_error = msg; }
-const char* last_error() { return g_last_error.c_str(); }
+void set_error(const std::string& msg) {
+  g_last_error = msg;
+  g_fixed_error = nullptr;
+}
+const char* last_error() { return g_fixed_error ? g_fixed_error : g_last_error.c_str(); }
+
+int fail_no_memory() noexcept {
+  g_fixed_error = "out of host memory";
+  return GTK_ERR_INVALID_ARG;
+}
 
 int fail(int code, const std::string& msg) {
   set_error(msg);

@@ -20,6 +20,9 @@ const char* last_error();
 // Report a failed check: stores the message and returns `code`.
 int fail(int code, const std::string& msg);
 
+// For the `catch` of an entry point: host memory has run out (messages are strings). Needs none itself.
+int fail_no_memory() noexcept;
+
 // Map a CUDA runtime error after a launch to GTK_ERR_CUDA with the CUDA message.
 int check_launch(const char* what);
 

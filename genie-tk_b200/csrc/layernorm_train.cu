@@ -1140,7 +1140,7 @@ size_t gtk_layernorm_backward_workspace_bytes(int64_t rows, int64_t D) {
 
 int gtk_layernorm_forward(const void* x, const gtk_rows* x_rows, int x_dtype, const void* weight, const void* bias,
                           int w_dtype, void* y, float* mean, float* rstd, int64_t rows, int64_t D, float eps,
-                          void* stream) {
+                          void* stream) try {
   if (int e = ln::check_common(rows, D, x_dtype, w_dtype)) return e;
   if (!(eps >= 0.f)) return fail(GTK_ERR_INVALID_ARG, "layernorm: eps must be >= 0");
   if (int e = ln::check_elem_ptr(x, "x", x_dtype)) return e;
@@ -1159,12 +1159,14 @@ int gtk_layernorm_forward(const void* x, const gtk_rows* x_rows, int x_dtype, co
   a.x = x, a.w = weight, a.b = bias, a.y = y, a.mean = mean, a.rstd = rstd;
   a.rows = rows, a.D = static_cast<int>(D), a.eps = eps, a.st = static_cast<cudaStream_t>(stream);
   return ln::run(a, x_dtype, w_dtype, vec, false);
+} catch (...) {
+  return fail_no_memory();
 }
 
 int gtk_layernorm_backward(const void* dy, const gtk_rows* dy_rows, const void* x, const gtk_rows* x_rows,
                            int x_dtype, const void* weight, int w_dtype, const float* mean, const float* rstd,
                            void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
-                           int64_t rows, int64_t D, void* stream) {
+                           int64_t rows, int64_t D, void* stream) try {
   if (int e = ln::check_common(rows, D, x_dtype, w_dtype)) return e;
   const bool params = dweight || dbias;
   if (params && workspace_bytes < gtk_layernorm_backward_workspace_bytes(rows, D))
@@ -1196,6 +1198,8 @@ int gtk_layernorm_backward(const void* dy, const gtk_rows* dy_rows, const void* 
   a.partial = params ? static_cast<float*>(workspace) : nullptr;
   a.rows = rows, a.D = static_cast<int>(D), a.st = static_cast<cudaStream_t>(stream);
   return ln::run(a, x_dtype, w_dtype, vec, true);
+} catch (...) {
+  return fail_no_memory();
 }
 
 }  // extern "C"
