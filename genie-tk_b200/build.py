@@ -6,7 +6,8 @@ Usage: ``python genie-tk_b200/build.py [--force] [-j N]``. Objects go to
 the Python package so it travels with the repository snapshot. The library links the
 CUDA runtime statically and resolves the driver's tensor-map encoder at run time, so it
 has no libcuda link dependency. The binding is compiled against the installed PyTorch and
-gets the library's entry points by address when it is loaded.
+gets the library's entry points by address when it is loaded; without PyTorch the C library is
+built alone.
 """
 
 from __future__ import annotations
@@ -67,7 +68,11 @@ def _build_binding(force):
     if not force and os.path.exists(BINDING_OUT) and os.path.getmtime(BINDING_OUT) >= max(map(os.path.getmtime, deps)):
         return ""
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:
+        print("PyTorch is not installed: the C library is built without its Python binding", file=sys.stderr)
+        return ""
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
@@ -88,7 +93,6 @@ def build(force: bool = False, jobs: int = 4, verbose: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         binding = ex.submit(_build_binding, force)
         results = list(ex.map(lambda s: _compile(s, force), sources()))
-        binding.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, log in results:
@@ -100,6 +104,7 @@ def build(force: bool = False, jobs: int = 4, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    binding.result()  # the C library does not depend on it
     return OUT
 
 
