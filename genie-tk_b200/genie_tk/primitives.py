@@ -82,6 +82,24 @@ class Embedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = float(scale)
 
+    @classmethod
+    def from_pretrained(cls, embeddings: Tensor, freeze: bool = True, padding_idx: Optional[int] = None,
+                        max_norm: Optional[float] = None, norm_type: float = 2.0, scale_grad_by_freq: bool = False,
+                        sparse: bool = False, scale: float = 1.0) -> "Embedding":
+        """nn.Embedding.from_pretrained: a layer on ``embeddings`` [vocabulary, D] itself. Rows are not
+        renormalised and gradients are dense sums, so max_norm, scale_grad_by_freq and sparse are
+        refused."""
+        for name, value in (("max_norm", max_norm), ("scale_grad_by_freq", scale_grad_by_freq), ("sparse", sparse)):
+            if value is not None and value is not False:
+                raise ValueError(f"genie_tk (B200): Embedding does not take {name}, got {value}")
+        if embeddings.dim() != 2:
+            raise ValueError("genie_tk (B200): embeddings must be 2-D [vocabulary, width], got "
+                             f"{tuple(embeddings.shape)}")
+        rows, width = embeddings.shape
+        layer = cls(rows, width, padding_idx, scale, device="meta", dtype=embeddings.dtype)
+        layer.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return layer
+
     def forward(self, tokens: Tensor) -> Tensor:
         return autograd.embedding(tokens, self.weight, self.scale, self.padding_idx)
 
