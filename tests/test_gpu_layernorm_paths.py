@@ -53,6 +53,31 @@ def test_wide_rows_sum_their_columns_in_short_chains():
     assert float((dw.double() * sign - want).abs().max()) <= 32 * U * want
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,D", [(9, 33), (40, 33), (9, 601), (40, 601), (10, 5003), (9, 9001), (13, 16377)])
+def test_transposed_rows_that_begin_anywhere(N, D, dtype):
+    """Odd widths at strides: no vectors. Tiles of rows from N = 8 on; groups in a warp, one group
+    a block, and 32 elements a thread."""
+    dev = require_gpu()
+    x, dy, w, b = _inputs((1, N, N, D), DT[dtype], torch.float32, N + D, dev)
+    _run_and_check(x.transpose(1, 2), dy.transpose(1, 2), w, b)
+    _run_and_check(x.transpose(1, 2), dy, w, b)
+    _run_and_check(x, dy.transpose(1, 2), w, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("D", [40, 600, 5003, 9001])
+def test_bases_off_a_vector(rows, D, dtype):
+    dev = require_gpu()
+    x, dy, w, b = _inputs((rows * D + 5,), DT[dtype], torch.float32, rows + D, dev)
+    w, b = w[:D].contiguous(), b[:D].contiguous()
+    shift = lambda t, k: t[k:k + rows * D].view(rows, D)  # noqa: E731
+    _run_and_check(shift(x, 1), shift(dy, 3), w, b)
+    _run_and_check(shift(x, 0), shift(dy, 1), w, b)
+    _run_and_check(shift(x, 1), shift(dy, 0), w, b)
+
+
 def test_statistics_lie_as_the_rows_do():
     """mean and rstd have one element for each row in x's own axes (or in one axis, or with a last
     axis of one): statistics of the transposed tensor are refused, not read in another order."""
