@@ -366,11 +366,10 @@ Memory memory_of(const c10::TensorImpl* t, Py_ssize_t index, bool output) {
 int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
 
 // Whether the first ka axes of `a`, from address `at_a` on, share a byte with the first kb axes of `b`.
-// `steps` bounds the work; without an answer by then, yes.
+// `steps` bounds how often one is taken apart; without an answer by then, yes.
 bool meet(const Memory& a, int64_t at_a, size_t ka, const Memory& b, int64_t at_b, size_t kb, int64_t* steps) {
   if (at_a + a.span[ka] <= at_b || at_b + b.span[kb] <= at_a) return false;
   if (ka == 0 && kb == 0) return true;
-  if (--*steps < 0) return true;
   // all runs begin at at_a or at_b plus multiples of g (columns of one matrix: its rows): the runs of
   // the one lie in the gaps of the other, or may meet
   int64_t g = 0;
@@ -378,6 +377,7 @@ bool meet(const Memory& a, int64_t at_a, size_t ka, const Memory& b, int64_t at_
   for (size_t k = 0; k < kb; ++k) g = std::gcd(g, b.axes[k].stride);
   const int64_t r = (at_b - at_a) - floor_div(at_b - at_a, g) * g;
   if (r >= a.run && r + b.run <= g) return false;
+  if (--*steps < 0) return true;
   // the parts of the wider one that reach into the other
   if (ka == 0 || (kb && b.span[kb] > a.span[ka])) return meet(b, at_b, kb, a, at_a, ka, steps);
   const auto& axis = a.axes[ka - 1];

@@ -89,6 +89,9 @@ def test_many_columns_of_one_buffer():
     assert abs(float(a.double().norm()) - 3.0) <= 1e-5
     with pytest.raises(RuntimeError, match="overlap"):
         ops.clip_grad_norm([a[:, c] for c in range(300)] + [a[2999, 299:]], 3.0)
+    b = torch.ones(3, 1700, device=dev)  # 1.4 million pairs
+    ops.clip_grad_norm([b[:, c] for c in range(1700)], 3.0)
+    assert abs(float(b.double().norm()) - 3.0) <= 1e-5
 
 
 def test_refused_calls_leave_the_versions():
