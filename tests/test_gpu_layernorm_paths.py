@@ -8,7 +8,7 @@ import torch
 
 import genie_tk
 from gpu_util import require_gpu
-from test_gpu_layernorm_train import DT, U, _inputs, _run_and_check
+from test_gpu_layernorm_train import DT, EPS, U, _bounds, _check, _inputs, _reference, _run_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,56 @@ def test_statistics_lie_as_the_rows_do():
     one = torch.randn(24, device=dev)
     _, m, r = ops.layernorm_forward(one, w, b)
     assert m.dim() == 0 and ops.layernorm_backward(one, one, w, m, r)[0].shape == (24,)
+
+
+def _check_rows(x, dy, w, b, got, rows):
+    """y, mean, rstd and dx of some rows (indices into the flattened leading axes)."""
+    y, mean, rstd, dx = got
+    D = x.shape[-1]
+    pick = lambda t: torch.stack([t[tuple(i)] for i in rows])  # noqa: E731
+    xs, gs = pick(x), pick(dy)
+    r = _reference(xs, w, b, gs)
+    bound = _bounds(r, x.dtype, w.dtype)
+    for k, t in (("y", pick(y)), ("mean", pick(mean)), ("rstd", pick(rstd)), ("dx", pick(dx))):
+        _check(t, r[k], bound[k], k)
+    assert xs.shape[-1] == D
+
+
+@pytest.mark.parametrize("shape,swap", [(((1 << 24) + 77, 130), False), ((4100, 4100, 128), True), ((4100, 4099, 129), True)])
+def test_more_than_2_31_elements(shape, swap):
+    """The last and some other rows against 64 bits, and the parameters' gradients against sums by
+    parts: xhat is off by 64 u (3 + 2 |xhat|) at most for this data, and a sum of R rows by
+    (64 + R / 148) u of its magnitudes."""
+    dev = require_gpu()
+    from genie_tk import ops
+    gen = torch.Generator(device=dev).manual_seed(1)
+    x = torch.empty(shape, dtype=torch.bfloat16, device=dev).normal_(generator=gen)
+    dy = torch.empty(shape, dtype=torch.bfloat16, device=dev).normal_(generator=gen)
+    D = shape[-1]
+    w, b = 1 + 0.1 * torch.randn(D, generator=gen, device=dev), torch.randn(D, generator=gen, device=dev)
+    if swap:
+        x, dy = x.transpose(0, 1), dy.transpose(0, 1)
+    y, mean, rstd = ops.layernorm_forward(x, w, b)
+    dx, dw, db = ops.layernorm_backward(dy, x, w, mean, rstd)
+    lead = x.shape[:-1]
+    rows = [[n - 1 for n in lead], [0] * len(lead), [n // 2 for n in lead]]
+    rows += [[lead[0] - 2 - i] + [n - 3 for n in lead[1:]] for i in range(40)]
+    _check_rows(x, dy, w, b, (y, mean, rstd, dx), rows)
+    del y, dx
+    R = x.numel() // D
+    want_w = torch.zeros(D, dtype=torch.float64, device=dev)
+    want_b, mag_w, mag_b, part = (torch.zeros_like(want_w) for _ in range(4))
+    step = 1 << 20 if not swap else 256
+    for i in range(0, lead[0], step):
+        xs, gs = x[i:i + step].double(), dy[i:i + step].double()
+        xh = (xs - xs.mean(-1, keepdim=True)) * (xs.var(-1, correction=0, keepdim=True) + EPS) ** -0.5
+        axes = tuple(range(xs.dim() - 1))
+        want_w += (gs * xh).sum(axes)
+        want_b += gs.sum(axes)
+        mag_w += (gs * xh).abs().sum(axes)
+        mag_b += gs.abs().sum(axes)
+        part += (gs.abs() * (3 + 2 * xh.abs())).sum(axes)
+    tree = (64 + R / 148) * U
+    for got, want, bound in ((db, want_b, tree * mag_b), (dw, want_w, tree * mag_w + 64 * U * part)):
+        assert ((got.double() - want).abs() <= bound + 2 * U * want.abs()).all()
+        assert float((got.double() - want).norm()) <= 1e-5 * float(mag_b.norm())
