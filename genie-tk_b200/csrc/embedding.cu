@@ -17,9 +17,11 @@
 // that cross chunks are joined in the block, and those that cross blocks from a scratch buffer
 // of at most two rows a block, by a last kernel and in order. Rows of tokens that do not occur are
 // zeroed by further blocks of the same launch, which look them up in the sorted keys.
-// No atomics on floating-point values: the same inputs give the same bits. Sums are fp32, of at
-// most 1024 rows one after another (by fours) and of partial rows in trees, and dW is rounded once.
-// (64-bit additions between the chunks took twice the time of the joining kernel.)
+// No atomics on floating-point values: the same inputs give the same bits. Sums are fp32: a chunk's
+// rows of one token by fours, one four after another (at most 256, and a few single rows at the run's
+// ends), the chunks of a block one after another (8 to 64), and the blocks of a run over the 16 warps of
+// the last kernel, which add eight at a time (one addition for each 128 blocks) and meet in a tree. dW
+// is rounded once. (64-bit additions between the chunks took twice the time of the joining kernel.)
 #include <cooperative_groups.h>
 
 #include "train_common.cuh"
