@@ -57,7 +57,8 @@ class Linear(nn.Linear):
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm whose forward and backward run on the library's kernels (CUDA tensors only;
     fp32, bf16 or fp16 inputs with parameters in fp32 or the input's type). Same constructor,
-    parameters and state dict; several normalised axes are normalised as one."""
+    parameters and state dict; several normalised axes are normalised as one. The result has the
+    input's type, under autocast too (nn.LayerNorm returns fp32 there)."""
 
     def forward(self, x: Tensor) -> Tensor:
         shape = self.normalized_shape
